@@ -43,6 +43,13 @@ extern "C" {
 #define PCLIP_FILIP_MAX_T 256    /* FILIP tokens per sequence handled by the fast kernels */
 #define PCLIP_FILIP_MAX_T_LONG 4096 /* FILIP tokens per sequence at most (general kernel)  */
 #define PCLIP_HEAD_MAX_BLOCKS 4  /* Linear-ReLU-LayerNorm-Dropout blocks of the embedding head */
+#define PCLIP_LINEAR_MAX_DIM 65536 /* input and output width of pclip_linear_*              */
+#define PCLIP_NORM_MAX_D 4096    /* row width of pclip_norm_gate_*                          */
+
+/* element types of the token-head operators (pclip_linear_*, pclip_norm_gate_*, pclip_grad_clip) */
+#define PCLIP_DT_F32 0
+#define PCLIP_DT_BF16 1
+#define PCLIP_DT_F16 2
 
 int pclip_version(void);
 const char* pclip_last_error(void);
@@ -325,6 +332,84 @@ int pclip_filip_bwd_fused(const uint16_t* hnA, const uint32_t* maskwA, int Br, i
  * when tsign (as in prep) is negative.  When `accumulate` is nonzero dh += instead of dh =. */
 int pclip_filip_prep_bwd(const float* h, const float* dn, int B, int T, int d, int normalise, const float* tsign,
                          int accumulate, float* dh, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Linear layer with bias, activation and residual in its epilogue: one layer of the
+ * per-residue network (projection and amino_acid_ffn, modules/models.py:32-52, 54-73), and of any
+ * block with a residual stream.
+ *   z = x W^T + b;  y = act(z) + residual
+ * x [M,K], W [N,K] (nn.Linear's layout), bias [N] or NULL, residual [M,N] or NULL, y [M,N], all of
+ * one `dtype` (PCLIP_DT_*), contiguous, aligned to one element.  1 <= M <= 2^31 - 2^16;
+ * 1 <= K, N <= PCLIP_LINEAR_MAX_DIM.  Products and sums are f32 (bf16 / f16 operands on the matrix cores, f32
+ * operands on their f32 form); y is rounded once.
+ * activation: 0 none, 1 relu, 2 gelu (the exact one, with erf), 3 silu.
+ * slope: NULL, or [M,N] of `dtype`: act'(z), kept for the backward.  Not needed for activation 0, nor
+ * for relu without a residual, where the backward reads the sign of y.
+ *
+ * Backward: dy [M,N] -> dz = dy * act'(z), rounded to `dtype`;
+ *   dx [M,K] = dz W;  dW [N,K] = dz^T x;  db [N] = sum_rows dz      (the residual's gradient is dy)
+ * saved: the forward's slope, or y with saved_is_output = 1 (relu without a residual), NULL for
+ * activation 0.  dx, dW, db are overwritten; each may be NULL.  Sums over rows run in a fixed
+ * order: the same inputs give the same bits.
+ * ------------------------------------------------------------------------------------- */
+#define PCLIP_ACT_NONE 0
+#define PCLIP_ACT_RELU 1
+#define PCLIP_ACT_GELU 2
+#define PCLIP_ACT_SILU 3
+int pclip_linear_fwd(const void* x, const void* w, const void* bias, const void* residual, int M, int K, int N, int dtype, int activation,
+                     void* y, void* slope, void* stream);
+size_t pclip_linear_bwd_workspace_bytes(int M, int K, int N, int dtype, int activation);
+int pclip_linear_bwd(const void* x, const void* w, const void* dy, const void* saved, int saved_is_output, int M, int K, int N, int dtype,
+                     int activation, void* dx, void* dw, void* db, void* ws, size_t ws_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Norms after a block and before the next one, with the block's gate, scale and residual: the
+ * LayerNorm and Dropout behind each Linear-ReLU of the per-residue network (modules/models.py:54-73)
+ * and the join of a residual stream.
+ *   v = norm_after(u) * wa + ba (or u);  y = r + scale * g * v;  n = norm_before(y) * wb + bb
+ * u, r (or NULL), y, n [rows,d] of `dtype`, contiguous, aligned to one element; rows <= 2^31 - 2^16,
+ * d <= PCLIP_NORM_MAX_D.
+ * gate_kind PCLIP_GATE_ROWS: gate [rows / gate_rows, d] of `dtype`, row i of the operands uses row
+ *   i / gate_rows (1: elementwise; rows: one gate for every channel; T: one row for each sequence);
+ *   PCLIP_GATE_BYTES: a mask [rows,d] of bytes, nonzero = kept (dropout with scale = 1 / (1 - p)).
+ * after, before: PCLIP_NORM_*; wa, ba, wb, bb [d] of `param_type` (PCLIP_DT_F32 or `dtype`), NULL = ones / zeros.
+ * n is written when before != PCLIP_NORM_NONE; it is computed from the f32 y, before y is rounded.
+ * stats: [rows,4] f32, 16-byte aligned (NULL in inference), kept for the backward.
+ *
+ * Backward: dy, dn (either may be NULL: zero) -> du, dr [rows,d], dgate (shaped like gate), dwa, dba,
+ * dwb, dbb [d] of `param_type`, each overwritten or NULL.  ws: the query's gate_rows is that of the
+ * gate when dgate is wanted, else 0; needed for affine gradients and dgate with gate_rows > 1.
+ * Sums over rows run in a fixed order.
+ * ------------------------------------------------------------------------------------- */
+#define PCLIP_NORM_NONE 0
+#define PCLIP_NORM_LAYER 1
+#define PCLIP_NORM_RMS 2
+#define PCLIP_GATE_NONE 0
+#define PCLIP_GATE_ROWS 1
+#define PCLIP_GATE_BYTES 2
+int pclip_norm_gate_fwd(const void* u, const void* r, const void* gate, int gate_kind, int gate_rows, float scale, int after, const void* wa,
+                        const void* ba, int before, const void* wb, const void* bb, int param_type, float eps, int rows, int d, int dtype,
+                        void* y, void* n, float* stats, void* stream);
+size_t pclip_norm_gate_bwd_workspace_bytes(int rows, int d, int dtype, int gate_rows);
+int pclip_norm_gate_bwd(const void* u, const void* r, const void* gate, int gate_kind, int gate_rows, float scale, int after, const void* wa,
+                        const void* ba, int before, const void* wb, const void* bb, int param_type, float eps, int rows, int d, int dtype,
+                        const float* stats, const void* dy, const void* dn, void* du, void* dr, void* dgate, void* dwa, void* dba, void* dwb,
+                        void* dbb, void* ws, size_t ws_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Global gradient norm over many tensors, and clipping (between loss.backward() and
+ * optimizer.step() of the loops at modules/training_utils.py:7, 92; the reference itself does not clip).
+ *   norm = sqrt(sum over all elements of x^2);  dst = src * min(1, max_norm / (norm + eps))
+ * src, numel, src_type, dst, dst_type: HOST arrays of n entries (device pointers aligned to one
+ * element, element counts, PCLIP_DT_* types); tensors are contiguous, at most 2^43 elements in all.
+ * dst = NULL: the norm only.  dst[i] may be src[i] (then of one type; nothing is written when the factor is 1);
+ * apart from that no destination may overlap another tensor of the call.
+ * Squares are summed in f64 in a fixed order.  norm: device scalar.  A norm that is NaN makes every
+ * result NaN; an infinite one makes the factor zero (infinite elements become NaN).
+ * ------------------------------------------------------------------------------------- */
+size_t pclip_grad_clip_workspace_bytes(int n);
+int pclip_grad_clip(const void* const* src, const int64_t* numel, const int* src_type, void* const* dst, const int* dst_type, int n,
+                    float max_norm, float eps, float* norm, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,459 @@
+// Linear layer with bias, activation and residual in its epilogue, and its backward.
+//
+//   z = x W^T + b,  y = act(z) + r;   dz = dy * act'(z),  dx = dz W,  dW = dz^T x,  db = sum_rows dz
+//
+// All three products are D[i][j] = sum_k P(i,k) Q(j,k) on the matrix cores (16x16x32 for bf16 / f16, 16x16x4 for f32),
+// with f32 sums, and differ in which way P and Q lie in memory: along k (rows x, W, dz in the forward and dx) or along
+// i / j (W in dx; dz and x in dW).
+#include "elem.h"
+#include <math.h>
+#include <type_traits>
+
+namespace {
+
+// ---- element types on the matrix cores ------------------------------------------------------
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T> struct Mfma;   // Frag: 16 bytes, the k values of one row that a lane feeds to one step
+template <> struct Mfma<__bf16> {
+    typedef bf16x8 Frag;
+    static __device__ __forceinline__ f32x4 step(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mfma<_Float16> {
+    typedef f16x8 Frag;
+    static __device__ __forceinline__ f32x4 step(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mfma<float> {
+    typedef f32x4 Frag;
+    static __device__ __forceinline__ f32x4 step(Frag a, Frag b, f32x4 c) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[t], b[t], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// ---- tiles in LDS -----------------------------------------------------------------------------
+// A tile holds ROWS rows (i or j) of 128 bytes of k (64 16-bit or 32 f32 values), in 16-byte chunks.
+//   along k:  chunk (row, c) at row * 128 + ((c ^ row % 8) * 16)
+//   along i:  k rows of ROWS elements; chunks permuted by k so that the four k rows which a fragment's read touches
+//             at once lie in different banks
+// The exchange keeps both the writes (8 lanes a 128-byte row) and the fragment reads (16 rows, or 4 k rows, a step)
+// off each other's banks.
+template <typename T> constexpr int KSTEP = 128 / (int)sizeof(T);   // k values of a tile
+
+template <typename T, int ROWS, bool ALONG_K>
+struct Tile {
+    static constexpr int V = PclipVec<T>::N;
+    static constexpr int CHUNKS = ROWS * 8;               // of 16 bytes
+    static constexpr int ICH = ROWS / V;                  // along i: chunks of a k row
+    typedef typename Mfma<T>::Frag Frag;
+
+    static __device__ __forceinline__ int swizzle_i(int k) {
+        if constexpr (sizeof(T) == 2) return (((k & 3) | ((k >> 1) & 4)) << 1) & (ICH - 1);
+        else return (((k >> 2) & 3) << 2) & (ICH - 1);
+    }
+    // byte offset of chunk number c, and the (row, k) of its first element within the tile
+    static __device__ __forceinline__ int slot(int c, int& row, int& k) {
+        if constexpr (ALONG_K) {
+            row = c >> 3;
+            k = (c & 7) * V;
+            return row * 128 + (((c & 7) ^ (row & 7)) << 4);
+        } else {
+            k = c / ICH;
+            const int ch = c % ICH;
+            row = ch * V;
+            return k * ROWS * (int)sizeof(T) + ((ch ^ swizzle_i(k)) << 4);
+        }
+    }
+    // the fragment of rows i0 .. i0 + 15 at k step kk: lane l holds row l % 16, group l / 16 of the step's k values
+    static __device__ __forceinline__ Frag frag(const char* lds, int i0, int kk, int lane) {
+        const int r = lane & 15, q = lane >> 4;
+        if constexpr (ALONG_K) {
+            const int row = i0 + r;
+            return *(const Frag*)(lds + row * 128 + (((kk * 4 + q) ^ (row & 7)) << 4));
+        } else if constexpr (sizeof(T) == 2) {
+            // two transposing reads of 4 k rows x 16 elements: the lane gives the address of 4 elements of k row
+            // 8q + 4j + r / 4 and receives the 4 k values of its own element
+            union { s16x4 h[2]; Frag f; } u;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int k = kk * 32 + q * 8 + j * 4 + (r >> 2), i = i0 + (r & 3) * 4;
+                const char* p = lds + k * ROWS * 2 + (((i >> 3) ^ swizzle_i(k)) << 4) + (i & 4) * 2;
+                u.h[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+            }
+            return u.f;
+        } else {
+            Frag f;
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const int k = kk * 16 + q * 4 + t, i = i0 + r;
+                f[t] = *(const float*)(lds + k * ROWS * 4 + (((i >> 2) ^ swizzle_i(k)) << 4) + (i & 3) * 4);
+            }
+            return f;
+        }
+    }
+    // chunk c of the tile whose first row is i0 and first k is k0: elements outside rows x k are zero
+    static __device__ __forceinline__ u32x4 fetch(const T* p, int ld, int i0, int rows, long long k0, long long k_end, int c) {
+        int row, k;
+        slot(c, row, k);
+        const long long kk = k0 + k;
+        const int i = i0 + row;
+        long long valid;
+        const T* at;
+        if constexpr (ALONG_K) {
+            valid = i < rows ? k_end - kk : 0;
+            at = p + (long long)i * ld + kk;
+        } else {
+            valid = kk < k_end ? rows - i : 0;
+            at = p + kk * ld + i;
+        }
+        if (valid >= V) return __builtin_bit_cast(u32x4, *(const PclipPack<T, V>*)at);
+        PclipPack<T, V> a;
+#pragma unroll
+        for (int e = 0; e < V; e++) a.v[e] = e < valid ? at[e] : (T)0.f;
+        return __builtin_bit_cast(u32x4, a);
+    }
+};
+
+// ---- activations --------------------------------------------------------------------------------
+// act(z) and its slope.  f32 results use the library's erf and exp.  For 16-bit results the Gaussian tail is
+// Phi(-a) = exp(-a^2 / 2) * P(1 / (1 + 0.3 a)), P a polynomial fitted to erfcx(a / sqrt 2) / 2 by reweighted least
+// squares over 0 <= a <= 13: 1.9e-6 relative error, a hundredth of an f16 half step, in one exp and one reciprocal,
+// which the slope's density shares.  Far arguments are cut at 40 where only their product with a vanished density
+// enters, so an infinite z has the limit's slope.
+template <bool EXACT>
+__device__ __forceinline__ float activate(float z, int act, float& slope) {
+    if (act == PCLIP_ACT_RELU) {
+        slope = z > 0.f ? 1.f : 0.f;
+        return z > 0.f ? z : (z != z ? z : 0.f);   // NaN stays
+    }
+    if (act == PCLIP_ACT_GELU) {
+        const float c = fminf(fmaxf(z, -40.f), 40.f);
+        float phi, density;
+        if constexpr (EXACT) {
+            density = expf(-0.5f * c * c);
+            phi = 0.5f * erfcf(z * -0.70710678118654752f);
+        } else {
+            const float t = __builtin_amdgcn_rcpf(fmaf(0.3f, fabsf(c), 1.f));
+            density = __builtin_amdgcn_exp2f(c * c * -0.72134752044448170f);
+            float g = -0.0845887363f;
+            g = fmaf(g, t, 0.240555853f);
+            g = fmaf(g, t, -0.0486187227f);
+            g = fmaf(g, t, 0.164744467f);
+            g = fmaf(g, t, 0.106712937f);
+            g = fmaf(g, t, 0.121272907f);
+            g = fmaf(g, t, -7.96368695e-05f);
+            g *= density;
+            phi = c < 0.f ? g : 1.f - g;
+        }
+        slope = fmaf(c * 0.39894228040143268f, density, phi);
+        return z * phi;
+    }
+    if (act == PCLIP_ACT_SILU) {
+        float s;
+        if constexpr (EXACT) s = 1.f / (1.f + expf(-z));
+        else s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
+        const float c = fminf(fmaxf(z, -100.f), 100.f);
+        slope = s * fmaf(c, 1.f - s, 1.f);
+        return z * s;
+    }
+    slope = 1.f;
+    return z;
+}
+
+// ---- the product -----------------------------------------------------------------------------------
+enum { EPI_FORWARD, EPI_STORE, EPI_SLAB };
+
+struct GemmArgs {
+    const void *P, *Q;
+    int ldp, ldq, I, J;
+    long long K, k_split;           // contraction length, and the part of one workgroup (a multiple of KSTEP)
+    int tiles_i, tiles_j, splits;
+    const void *bias, *residual;    // EPI_FORWARD
+    void *out, *slope;
+    int act;
+    float *slab, *row_sum;          // EPI_SLAB: [splits][I][J], [splits][I] or NULL
+};
+
+// Workgroups go to the eight XCDs in turn; give each XCD a run of neighbouring tiles, which share rows of P or Q in its L2.
+__device__ __forceinline__ int xcd_order(int b, int n) {
+    const int xcd = b & 7, q = n >> 3, r = n & 7;
+    return xcd * q + min(xcd, r) + (b >> 3);
+}
+
+template <typename T, int BI, int BJ, int WI, int WJ, bool PK, bool QK, int EPI>
+__global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(const GemmArgs A) {
+    typedef Tile<T, BI, PK> TP;
+    typedef Tile<T, BJ, QK> TQ;
+    typedef typename Mfma<T>::Frag Frag;
+    constexpr int N = 64 * WI * WJ, NP = TP::CHUNKS / N, NQ = TQ::CHUNKS / N;
+    constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16, BYTES = (BI + BJ) * 128;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int b = xcd_order(blockIdx.x, gridDim.x);
+    const int tj = b % A.tiles_j;
+    b /= A.tiles_j;
+    const int ti = b % A.tiles_i, split = b / A.tiles_i;
+    const int i0 = ti * BI, j0 = tj * BJ;
+    const int wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
+    const long long k_first = split * A.k_split, k_end = k_first + A.k_split < A.K ? k_first + A.k_split : A.K;
+    const T *P = (const T*)A.P, *Q = (const T*)A.Q;
+
+    u32x4 rp[NP], rq[NQ];
+    auto fetch = [&](long long k0) {
+#pragma unroll
+        for (int n = 0; n < NP; n++) rp[n] = TP::fetch(P, A.ldp, i0, A.I, k0, k_end, tid + n * N);
+#pragma unroll
+        for (int n = 0; n < NQ; n++) rq[n] = TQ::fetch(Q, A.ldq, j0, A.J, k0, k_end, tid + n * N);
+    };
+    f32x4 acc[FI][FJ], ones[FI];
+#pragma unroll
+    for (int i = 0; i < FI; i++) {
+        ones[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < FJ; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    Frag one;
+#pragma unroll
+    for (int e = 0; e < PclipVec<T>::N; e++) one[e] = (T)1.f;
+    const bool sum_rows = EPI == EPI_SLAB && A.row_sum && tj == 0 && wj == 0;
+
+    fetch(k_first);
+    int buf = 0;
+    for (long long k = k_first; k < k_end; k += KSTEP<T>) {
+        char *lp = lds + buf * BYTES, *lq = lp + BI * 128;
+        int row, kk;
+#pragma unroll
+        for (int n = 0; n < NP; n++) *(u32x4*)(lp + TP::slot(tid + n * N, row, kk)) = rp[n];
+#pragma unroll
+        for (int n = 0; n < NQ; n++) *(u32x4*)(lq + TQ::slot(tid + n * N, row, kk)) = rq[n];
+        __syncthreads();   // the other buffer's readers were done before they came here
+        if (k + KSTEP<T> < k_end) fetch(k + KSTEP<T>);
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            Frag fp[FI], fq[FJ];
+#pragma unroll
+            for (int i = 0; i < FI; i++) fp[i] = TP::frag(lp, wi + i * 16, s, lane);
+#pragma unroll
+            for (int j = 0; j < FJ; j++) fq[j] = TQ::frag(lq, wj + j * 16, s, lane);
+#pragma unroll
+            for (int i = 0; i < FI; i++)
+#pragma unroll
+                for (int j = 0; j < FJ; j++) acc[i][j] = Mfma<T>::step(fq[j], fp[i], acc[i][j]);
+            if (sum_rows)
+#pragma unroll
+                for (int i = 0; i < FI; i++) ones[i] = Mfma<T>::step(one, fp[i], ones[i]);
+        }
+        buf ^= 1;
+    }
+
+    // a lane holds, of every 16 x 16 tile, row i = lane % 16 and the four columns from j = 4 * (lane / 16) on
+#pragma unroll
+    for (int fi = 0; fi < FI; fi++) {
+        const int i = i0 + wi + fi * 16 + (lane & 15);
+        if (i >= A.I) continue;
+#pragma unroll
+        for (int fj = 0; fj < FJ; fj++) {
+            const int j = j0 + wj + fj * 16 + (lane >> 4) * 4, left = A.J - j;
+            if (left <= 0) continue;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = acc[fi][fj][e];
+            const size_t at = (size_t)i * A.J + j;
+            if constexpr (EPI == EPI_FORWARD) {
+                if (A.bias) {
+                    float bias[4];
+                    load_f32<T, 4>((const T*)A.bias + j, left, bias);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] += bias[e];
+                }
+                float slope[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = activate<sizeof(T) == 4>(v[e], A.act, slope[e]);
+                if (A.slope) store_f32<T, 4>((T*)A.slope + at, left, slope);
+                if (A.residual) {
+                    float res[4];
+                    load_f32<T, 4>((const T*)A.residual + at, left, res);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] += res[e];
+                }
+                store_f32<T, 4>((T*)A.out + at, left, v);
+            } else if constexpr (EPI == EPI_STORE) {
+                store_f32<T, 4>((T*)A.out + at, left, v);
+            } else {
+                store_f32<float, 4>(A.slab + (size_t)split * A.I * A.J + at, left, v);
+            }
+        }
+        if (sum_rows && lane < 16) A.row_sum[(size_t)split * A.I + i] = ones[fi][0];
+    }
+}
+
+// out[e] = sum over the splits' slabs, in their order, rounded once; 64 x 4 elements and four parts of the splits a workgroup
+template <typename T>
+__global__ __launch_bounds__(256) void slab_sum_kernel(const float* __restrict__ slab, int splits, long long n, T* __restrict__ out) {
+    __shared__ float lds[3][64][4];
+    const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
+    const long long e = ((long long)blockIdx.x * 64 + lane) * 4;
+    const long long left = n - e;
+    const int valid = left < 4 ? (int)left : 4;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (valid > 0)
+#pragma unroll 4
+        for (int k = part; k < splits; k += 4) {
+            float v[4];
+            load_f32<float, 4>(slab + (size_t)k * n + e, valid, v);
+#pragma unroll
+            for (int c = 0; c < 4; c++) s[c] += v[c];
+        }
+    if (part)
+#pragma unroll
+        for (int c = 0; c < 4; c++) lds[part - 1][lane][c] = s[c];
+    __syncthreads();
+    if (part == 0 && valid > 0) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) s[c] += (lds[0][lane][c] + lds[1][lane][c]) + lds[2][lane][c];
+        store_f32<T, 4>(out + e, valid, s);
+    }
+}
+
+// dz = dy * slope, or dy where the output is positive
+template <typename T>
+__global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, const T* __restrict__ saved, int is_output, long long n, T* __restrict__ dz) {
+    constexpr int V = PclipVec<T>::N;
+    for (long long e = ((long long)blockIdx.x * 256 + threadIdx.x) * V; e < n; e += (long long)gridDim.x * 256 * V) {
+        const long long left = n - e;
+        const int valid = left < V ? (int)left : V;
+        float d[V], s[V];
+        load_f32<T, V>(dy + e, valid, d);
+        load_f32<T, V>(saved + e, valid, s);
+#pragma unroll
+        for (int i = 0; i < V; i++) d[i] = is_output ? (s[i] > 0.f ? d[i] : 0.f) : d[i] * s[i];
+        store_f32<T, V>(dz + e, valid, d);
+    }
+}
+
+// ---- host side -----------------------------------------------------------------------------------------
+template <typename T, int BI, int BJ, int WI, int WJ, bool PK, bool QK, int EPI>
+int launch_tile(GemmArgs A, hipStream_t st) {
+    static PclipLdsLimit limit;
+    constexpr size_t bytes = 2 * (size_t)(BI + BJ) * 128;
+    auto* fn = gemm_kernel<T, BI, BJ, WI, WJ, PK, QK, EPI>;
+    const int rc = pclip_ensure_lds(limit, (const void*)fn, bytes, "linear");
+    if (rc) return rc;
+    A.tiles_i = (A.I + BI - 1) / BI;
+    A.tiles_j = (A.J + BJ - 1) / BJ;
+    const long long blocks = (long long)A.tiles_i * A.tiles_j * A.splits;
+    PCLIP_REQUIRE(blocks <= 0x7fffffffll, "linear: too many tiles (%lld)", blocks);
+    fn<<<(int)blocks, 64 * WI * WJ, bytes, st>>>(A);
+    return PCLIP_OK;
+}
+
+long long tiles(long long i, long long j, int bi, int bj) { return ((i + bi - 1) / bi) * ((j + bj - 1) / bj); }
+
+template <typename T, bool PK, bool QK, int EPI>
+int launch_rows(const GemmArgs& A, hipStream_t st) {
+    if (tiles(A.I, A.J, 128, 128) >= 256) return launch_tile<T, 128, 128, 2, 2, PK, QK, EPI>(A, st);
+    return launch_tile<T, 64, 64, 2, 2, PK, QK, EPI>(A, st);
+}
+
+// the product over the rows (dW): tile size and the number of splits
+struct RowPlan { int tile, splits; long long k_split; };
+RowPlan row_plan(int M, int K, int N, int dtype) {
+    const int step = dtype == PCLIP_DT_F32 ? 32 : 64, tile = K > 64 && N > 64 ? 128 : 64;
+    const long long t = tiles(N, K, tile, tile), steps = ((long long)M + step - 1) / step;
+    long long s = (512 + t - 1) / t;
+    if (s > (steps + 3) / 4) s = (steps + 3) / 4;   // four steps a workgroup at least
+    if (s < 1) s = 1;
+    const long long per = (steps + s - 1) / s;
+    return {tile, (int)((steps + per - 1) / per), per * step};
+}
+
+template <typename T>
+int forward(const GemmArgs& A, hipStream_t st) { return launch_rows<T, true, true, EPI_FORWARD>(A, st); }
+
+template <typename T>
+int backward(const T* x, const T* w, const T* dy, const T* saved, int is_output, int M, int K, int N, int dtype, int act, T* dx, T* dw, T* db, char* ws,
+             hipStream_t st) {
+    const T* dz = dy;
+    if (act != PCLIP_ACT_NONE) {
+        const long long n = (long long)M * N, want = (n + 256 * PclipVec<T>::N - 1) / (256 * PclipVec<T>::N);
+        slope_kernel<T><<<want < 4096 ? (int)want : 4096, 256, 0, st>>>(dy, saved, is_output, n, (T*)ws);
+        dz = (const T*)ws;
+        ws += pclip_align_up((size_t)n * sizeof(T), 256);
+    }
+    if (dx) {
+        GemmArgs A = {};
+        A.P = dz, A.Q = w, A.ldp = N, A.ldq = K, A.I = M, A.J = K, A.K = N, A.k_split = (N + 63) / 64 * 64, A.splits = 1, A.out = dx;
+        const int rc = launch_rows<T, true, false, EPI_STORE>(A, st);
+        if (rc) return rc;
+    }
+    if (dw || db) {
+        const RowPlan p = row_plan(M, K, N, dtype);
+        GemmArgs A = {};
+        A.P = dz, A.Q = x, A.ldp = N, A.ldq = K, A.I = N, A.J = K, A.K = M, A.k_split = p.k_split, A.splits = p.splits;
+        A.slab = (float*)ws;
+        A.row_sum = db ? A.slab + (size_t)p.splits * N * K : nullptr;
+        const int rc = p.tile == 128 ? launch_tile<T, 128, 128, 2, 2, false, false, EPI_SLAB>(A, st) : launch_tile<T, 64, 64, 2, 2, false, false, EPI_SLAB>(A, st);
+        if (rc) return rc;
+        const long long n = (long long)N * K;
+        if (dw) slab_sum_kernel<T><<<(int)((n + 255) / 256), 256, 0, st>>>(A.slab, p.splits, n, dw);
+        if (db) slab_sum_kernel<T><<<(N + 255) / 256, 256, 0, st>>>(A.row_sum, p.splits, N, db);
+    }
+    return PCLIP_OK;
+}
+
+int check_sizes(const char* who, int M, int K, int N, int dtype, int act) {
+    PCLIP_REQUIRE(pclip_dtype_ok(dtype), "%s: unknown type %d", who, dtype);
+    PCLIP_REQUIRE(M >= 1 && M <= 0x7fff0000 && K >= 1 && N >= 1 && K <= PCLIP_LINEAR_MAX_DIM && N <= PCLIP_LINEAR_MAX_DIM, "%s: M=%d K=%d N=%d (1 <= M <= 2147418112, 1 <= K, N <= %d)", who, M, K,
+                  N, PCLIP_LINEAR_MAX_DIM);
+    PCLIP_REQUIRE(act >= PCLIP_ACT_NONE && act <= PCLIP_ACT_SILU, "%s: unknown activation %d", who, act);
+    return PCLIP_OK;
+}
+
+}  // namespace
+
+extern "C" int pclip_linear_fwd(const void* x, const void* w, const void* bias, const void* residual, int M, int K, int N, int dtype, int activation,
+                                void* y, void* slope, void* stream) {
+    int rc = check_sizes("linear_fwd", M, K, N, dtype, activation);
+    if (rc) return rc;
+    PCLIP_REQUIRE(x && w && y, "linear_fwd: null pointer");
+    GemmArgs A = {};
+    A.P = x, A.Q = w, A.ldp = K, A.ldq = K, A.I = M, A.J = N, A.K = K, A.k_split = (K + 63) / 64 * 64, A.splits = 1;
+    A.bias = bias, A.residual = residual, A.out = y, A.slope = slope, A.act = activation;
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == PCLIP_DT_F32) rc = forward<float>(A, st);
+    else if (dtype == PCLIP_DT_BF16) rc = forward<__bf16>(A, st);
+    else rc = forward<_Float16>(A, st);
+    return rc ? rc : pclip_check_launch("linear_fwd");
+}
+
+extern "C" size_t pclip_linear_bwd_workspace_bytes(int M, int K, int N, int dtype, int activation) {
+    if (check_sizes("linear_bwd", M, K, N, dtype, activation)) return 0;
+    const RowPlan p = row_plan(M, K, N, dtype);
+    const size_t dz = activation == PCLIP_ACT_NONE ? 0 : pclip_align_up((size_t)M * N * pclip_dtype_size(dtype), 256);
+    return dz + (size_t)p.splits * N * ((size_t)K + 1) * sizeof(float);
+}
+
+extern "C" int pclip_linear_bwd(const void* x, const void* w, const void* dy, const void* saved, int saved_is_output, int M, int K, int N, int dtype,
+                                int activation, void* dx, void* dw, void* db, void* ws, size_t ws_bytes, void* stream) {
+    int rc = check_sizes("linear_bwd", M, K, N, dtype, activation);
+    if (rc) return rc;
+    PCLIP_REQUIRE(dy && ws && (!dx || w) && (!dw || x), "linear_bwd: null pointer");
+    PCLIP_REQUIRE(x || !db, "linear_bwd: the bias gradient runs with the weight's product and needs x");
+    PCLIP_REQUIRE(activation == PCLIP_ACT_NONE || saved, "linear_bwd: what the forward saved is needed");
+    PCLIP_REQUIRE(!saved_is_output || activation == PCLIP_ACT_RELU, "linear_bwd: only relu's slope can be read from the output");
+    const size_t need = pclip_linear_bwd_workspace_bytes(M, K, N, dtype, activation);
+    PCLIP_REQUIRE(ws_bytes >= need, "linear_bwd: workspace too small (%zu bytes, need %zu)", ws_bytes, need);
+    PCLIP_REQUIRE(((uintptr_t)ws & 15) == 0, "linear_bwd: the workspace must be 16-byte aligned");
+    hipStream_t st = (hipStream_t)stream;
+#define PCLIP_LINEAR_BWD(T)                                                                                                                         backward<T>((const T*)x, (const T*)w, (const T*)dy, (const T*)saved, saved_is_output, M, K, N, dtype, activation, (T*)dx, (T*)dw, (T*)db, (char*)ws, st)
+    if (dtype == PCLIP_DT_F32) rc = PCLIP_LINEAR_BWD(float);
+    else if (dtype == PCLIP_DT_BF16) rc = PCLIP_LINEAR_BWD(__bf16);
+    else rc = PCLIP_LINEAR_BWD(_Float16);
+#undef PCLIP_LINEAR_BWD
+    return rc ? rc : pclip_check_launch("linear_bwd");
+}

@@ -1,0 +1,507 @@
+// Norms before and after a block, with the block's gate, scale and residual, in one pass each way.
+//
+//   v = norm_after(u) * wa + ba          the block's output, normalised (or v = u)
+//   y = r + scale * g * v                g: none, a row for every `gate_rows` rows, or a byte mask
+//   n = norm_before(y) * wb + bb         what the next block reads (optional)
+//   norm: "layer" (x - mean) / sqrt(var + eps), "rms" x / sqrt(mean(x^2) + eps)
+//
+// Backward, with a^ and b^ the normalised values, dt = dy + norm_before'(dn):
+//   norm'(d) = rstd * (d w - mean(d w) - ^ mean(d w ^))   (the first mean only for "layer")
+//   dr = dt;  dg = scale v dt;  dv = scale g dt;  du = norm_after'(dv);  dw = sum_rows d ^;  db = sum_rows d
+//
+// Bound: HBM.  Every operand is read once and every result written once; a row lives in the registers of the lanes
+// that read it (16 lanes up to 128 16-bit elements, a wave up to 1024, a workgroup up to 4096), y is made again in
+// the backward from u and r instead of being read.  Statistics, sums and y are f32; n is taken from the f32 y, not
+// from its rounded copy.  Column sums (affine and broadcast-gate gradients) stay in registers over a workgroup's
+// rows, then go to the workspace, one row a workgroup, and are added by a second kernel in a fixed order: no atomics.
+#include "elem.h"
+
+namespace {
+
+constexpr int THREADS = 256;
+constexpr int MAX_D = PCLIP_NORM_MAX_D;
+
+struct NormGateArgs {
+    const void *u, *r, *gate;
+    const void *wa, *ba, *wb, *bb;
+    void *y, *n;
+    float4* stats;                    // [rows] {mean_a, rstd_a, mean_b, rstd_b}
+    const void *dy, *dn;
+    void *du, *dr, *dg;
+    float *part_w, *part_g;           // [blocks][4][d], [gate rows][chunks][d]
+    int rows, d, gate_rows;           // gate_rows: rows that share a row of the gate (1: elementwise)
+    int gate_kind, after, before, param_f32;
+    float scale, eps;
+    // division of the rows: a workgroup takes `groups_per_block` whole groups of `group_rows` rows, or (chunks > 1) a
+    // chunk of `chunk_rows` rows of one group
+    int groups, group_rows, groups_per_block, chunks, chunk_rows;
+    int sum_gate;                     // the gate's gradient is a sum over the rows of a group
+    int wanted;                       // which affine gradients: bit 0 dwa, 1 dba, 2 dwb, 3 dbb
+};
+
+// sums of two values over the G lanes that hold a row (16, 64, or the whole workgroup), in every lane
+template <int G>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float (*lds)[2]) {
+#define PCLIP_DPP_ADD2(ctrl)                                                                     \
+    a += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(a), ctrl, 0xF, 0xF, true)); \
+    b += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(b), ctrl, 0xF, 0xF, true))
+    PCLIP_DPP_ADD2(0xB1);
+    PCLIP_DPP_ADD2(0x4E);
+    PCLIP_DPP_ADD2(0x141);
+    PCLIP_DPP_ADD2(0x140);
+#undef PCLIP_DPP_ADD2
+    if constexpr (G >= 64) {
+        a += __shfl_xor(a, 16);
+        b += __shfl_xor(b, 16);
+        a += __shfl_xor(a, 32);
+        b += __shfl_xor(b, 32);
+    }
+    if constexpr (G == 256) {
+        __syncthreads();   // the previous sum's readers are done
+        if ((threadIdx.x & 63) == 0) {
+            lds[threadIdx.x >> 6][0] = a;
+            lds[threadIdx.x >> 6][1] = b;
+        }
+        __syncthreads();
+        a = (lds[0][0] + lds[1][0]) + (lds[2][0] + lds[3][0]);
+        b = (lds[0][1] + lds[1][1]) + (lds[2][1] + lds[3][1]);
+    }
+}
+
+// The elements of one lane: NV vectors of V, vector k at column (k * G + lane) * V.
+template <typename T, int G, int NV>
+struct Row {
+    static constexpr int V = PclipVec<T>::N, E = NV * V, NG = THREADS / G;
+    static __device__ __forceinline__ int col(int k) { return (k * G + (int)(threadIdx.x % G)) * V; }
+    template <typename S>
+    static __device__ __forceinline__ void load(const S* p, int d, float (&x)[E]) {
+#pragma unroll
+        for (int k = 0; k < NV; k++) load_f32<S, V>(p + col(k), d - col(k), *(float(*)[V])(x + k * V));
+    }
+    template <typename S>
+    static __device__ __forceinline__ void store(S* p, int d, const float (&x)[E]) {
+#pragma unroll
+        for (int k = 0; k < NV; k++) store_f32<S, V>(p + col(k), d - col(k), *(const float(*)[V])(x + k * V));
+    }
+    static __device__ __forceinline__ void load_param(const void* p, bool f32, int d, float other, float (&x)[E]) {
+        if (!p) {
+#pragma unroll
+            for (int i = 0; i < E; i++) x[i] = other;
+        } else if (f32) {
+            load((const float*)p, d, x);
+        } else {
+            load((const T*)p, d, x);
+        }
+    }
+    static __device__ __forceinline__ void load_gate(const NormGateArgs& A, int row, float (&g)[E]) {
+        if (A.gate_kind == PCLIP_GATE_BYTES) {
+            load((const uint8_t*)A.gate + (size_t)row * A.d, A.d, g);
+#pragma unroll
+            for (int i = 0; i < E; i++) g[i] = g[i] != 0.f ? 1.f : 0.f;
+        } else {
+            load((const T*)A.gate + (size_t)((unsigned)row / (unsigned)A.gate_rows) * A.d, A.d, g);
+        }
+    }
+    // mean (zero for rms) and 1 / sqrt(mean square of the centred values + eps)
+    static __device__ __forceinline__ void stats(const float (&x)[E], int kind, int d, float eps, float& mean, float& rstd, float (*lds)[2]) {
+        const float inv = 1.f / (float)d;
+        mean = 0.f;
+        float s = 0.f, q = 0.f;
+        if (kind == PCLIP_NORM_LAYER) {
+#pragma unroll
+            for (int i = 0; i < E; i++) s += x[i];   // the places behind the row are zero
+            row_sum2<G>(s, q, lds);
+            mean = s * inv;
+        }
+        q = 0.f;
+        s = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int i = 0; i < V; i++)
+                if (col(k) + i < d) {
+                    const float c = x[k * V + i] - mean;
+                    q = fmaf(c, c, q);
+                }
+        row_sum2<G>(q, s, lds);
+        rstd = 1.f / sqrtf(q * inv + eps);
+    }
+};
+
+template <typename T, int G, int NV>
+__global__ __launch_bounds__(THREADS) void norm_gate_fwd_kernel(const NormGateArgs A) {
+    using R = Row<T, G, NV>;
+    constexpr int E = R::E;
+    __shared__ float lds[4][2];
+    const int d = A.d;
+    for (int row = blockIdx.x * R::NG + (int)threadIdx.x / G; row < A.rows; row += gridDim.x * R::NG) {
+        const size_t at = (size_t)row * d;
+        float u[E], y[E];
+        R::load((const T*)A.u + at, d, u);
+        if (A.r) R::load((const T*)A.r + at, d, y);
+        else {
+#pragma unroll
+            for (int i = 0; i < E; i++) y[i] = 0.f;
+        }
+        float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
+        if (A.after) {
+            float w[E], b[E];
+            R::load_param(A.wa, A.param_f32, d, 1.f, w);
+            R::load_param(A.ba, A.param_f32, d, 0.f, b);
+            R::stats(u, A.after, d, A.eps, st.x, st.y, lds);
+#pragma unroll
+            for (int i = 0; i < E; i++) u[i] = fmaf((u[i] - st.x) * st.y, w[i], b[i]);
+        }
+        if (A.gate_kind) {
+            float g[E];
+            R::load_gate(A, row, g);
+#pragma unroll
+            for (int i = 0; i < E; i++) u[i] *= g[i];
+        }
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int i = 0; i < R::V; i++) y[k * R::V + i] = R::col(k) + i < d ? fmaf(A.scale, u[k * R::V + i], y[k * R::V + i]) : 0.f;
+        R::store((T*)A.y + at, d, y);
+        if (A.before) {
+            float w[E], b[E];
+            R::load_param(A.wb, A.param_f32, d, 1.f, w);
+            R::load_param(A.bb, A.param_f32, d, 0.f, b);
+            R::stats(y, A.before, d, A.eps, st.z, st.w, lds);
+#pragma unroll
+            for (int i = 0; i < E; i++) y[i] = fmaf((y[i] - st.z) * st.w, w[i], b[i]);
+            R::store((T*)A.n + at, d, y);
+        }
+        if (A.stats && threadIdx.x % G == 0) A.stats[row] = st;
+    }
+}
+
+// Adds the accumulators of a workgroup's row slots (`buf`: one row of E * G floats a wave) and hands each column's sum
+// to `put(column, value)`.  Every thread of the workgroup calls it.
+template <typename T, int G, int NV, typename Put>
+__device__ __forceinline__ void flush_columns(float (&acc)[NV * PclipVec<T>::N], float* buf, int d, Put put) {
+    using R = Row<T, G, NV>;
+    if constexpr (G == 256) {   // one row at a time: every column has one owner
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int i = 0; i < R::V; i++)
+                if (R::col(k) + i < d) put(R::col(k) + i, acc[k * R::V + i]);
+    } else {
+        constexpr int W = G * NV * R::V;   // columns of a wave's row of buf
+        if constexpr (G == 16) {
+#pragma unroll
+            for (int i = 0; i < R::E; i++) {
+                acc[i] += __shfl_xor(acc[i], 16);
+                acc[i] += __shfl_xor(acc[i], 32);
+            }
+        }
+        __syncthreads();   // the previous call's readers are done
+        if ((threadIdx.x & 63) < G)
+#pragma unroll
+            for (int k = 0; k < NV; k++)
+#pragma unroll
+                for (int i = 0; i < R::V; i++) buf[(threadIdx.x >> 6) * W + R::col(k) + i] = acc[k * R::V + i];
+        __syncthreads();
+        for (int c = threadIdx.x; c < d; c += THREADS) put(c, (buf[c] + buf[W + c]) + (buf[2 * W + c] + buf[3 * W + c]));
+    }
+#pragma unroll
+    for (int i = 0; i < R::E; i++) acc[i] = 0.f;
+}
+
+template <typename T, int G, int NV>
+__global__ __launch_bounds__(THREADS) void norm_gate_bwd_kernel(const NormGateArgs A) {
+    using R = Row<T, G, NV>;
+    constexpr int E = R::E;
+    __shared__ float lds[4][2];
+    __shared__ float buf[G == 256 ? 1 : 4 * G * E];
+    const int d = A.d, slot = (int)threadIdx.x / G;
+    const float inv = 1.f / (float)d;
+    float swa[E], sba[E], swb[E], sbb[E], sg[E];
+#pragma unroll
+    for (int i = 0; i < E; i++) swa[i] = sba[i] = swb[i] = sbb[i] = sg[i] = 0.f;
+    const int g0 = A.chunks > 1 ? (int)blockIdx.x / A.chunks : (int)blockIdx.x * A.groups_per_block;
+    const int g1 = A.chunks > 1 ? g0 + 1 : min(g0 + A.groups_per_block, A.groups);
+    for (int grp = g0; grp < g1; grp++) {
+        // (group + 1) * group_rows <= rows: no overflow
+        int first = grp * A.group_rows, last = first + A.group_rows;
+        if (A.chunks > 1) {
+            const long long from = first + (long long)((int)blockIdx.x % A.chunks) * A.chunk_rows;
+            first = (int)min(from, (long long)last);
+            last = (int)min(from + A.chunk_rows, (long long)last);
+        }
+        for (int row = first + slot; row < last; row += R::NG) {
+            const size_t at = (size_t)row * d;
+            float u[E], t[E], g[E];
+            R::load((const T*)A.u + at, d, u);
+            const float4 st = A.stats ? A.stats[row] : make_float4(0.f, 1.f, 0.f, 1.f);
+            if (A.dy) R::load((const T*)A.dy + at, d, t);
+            else {
+#pragma unroll
+                for (int i = 0; i < E; i++) t[i] = 0.f;
+            }
+            if (A.gate_kind) R::load_gate(A, row, g);
+            else {
+#pragma unroll
+                for (int i = 0; i < E; i++) g[i] = 1.f;
+            }
+            float w[E], v[E];   // w: weight of the norm in hand; v: the value that the gate multiplies
+            if (A.after) {
+                float b[E];
+                R::load_param(A.wa, A.param_f32, d, 1.f, w);
+                R::load_param(A.ba, A.param_f32, d, 0.f, b);
+#pragma unroll
+                for (int i = 0; i < E; i++) {
+                    u[i] = (u[i] - st.x) * st.y;   // from here on the normalised value
+                    v[i] = fmaf(u[i], w[i], b[i]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < E; i++) {
+                    w[i] = 1.f;
+                    v[i] = u[i];
+                }
+            }
+            if (A.before && A.dn) {
+                float h[E], q[E], wb[E];
+                if (A.r) R::load((const T*)A.r + at, d, h);
+                else {
+#pragma unroll
+                    for (int i = 0; i < E; i++) h[i] = 0.f;
+                }
+                R::load((const T*)A.dn + at, d, q);
+                R::load_param(A.wb, A.param_f32, d, 1.f, wb);
+                float m1 = 0.f, m2 = 0.f;
+#pragma unroll
+                for (int i = 0; i < E; i++) {
+                    h[i] = (fmaf(A.scale, g[i] * v[i], h[i]) - st.z) * st.w;
+                    swb[i] = fmaf(q[i], h[i], swb[i]);   // q is zero behind the row
+                    sbb[i] += q[i];
+                    q[i] *= wb[i];
+                    m1 += q[i];
+                    m2 = fmaf(q[i], h[i], m2);
+                }
+                row_sum2<G>(m1, m2, lds);
+                m1 = A.before == PCLIP_NORM_LAYER ? m1 * inv : 0.f;
+                m2 *= inv;
+#pragma unroll
+                for (int i = 0; i < E; i++) t[i] = fmaf(st.w, q[i] - m1 - h[i] * m2, t[i]);
+            }
+            if (A.dr) R::store((T*)A.dr + at, d, t);
+            if (A.dg && !A.sum_gate) {
+                float e[E];
+#pragma unroll
+                for (int i = 0; i < E; i++) e[i] = A.scale * v[i] * t[i];
+                R::store((T*)A.dg + at, d, e);
+            }
+            float m1 = 0.f, m2 = 0.f;
+#pragma unroll
+            for (int k = 0; k < NV; k++)
+#pragma unroll
+                for (int j = 0; j < R::V; j++) {
+                    const int i = k * R::V + j;
+                    const float in = R::col(k) + j < d ? A.scale * t[i] : 0.f;   // nothing behind the row enters the sums
+                    sg[i] = fmaf(v[i], in, sg[i]);
+                    t[i] = g[i] * in;                                            // dv
+                    swa[i] = fmaf(t[i], u[i], swa[i]);
+                    sba[i] += t[i];
+                    t[i] *= w[i];
+                    m1 += t[i];
+                    m2 = fmaf(t[i], u[i], m2);
+                }
+            if (A.after) {
+                row_sum2<G>(m1, m2, lds);
+                m1 = A.after == PCLIP_NORM_LAYER ? m1 * inv : 0.f;
+                m2 *= inv;
+#pragma unroll
+                for (int i = 0; i < E; i++) t[i] = st.y * (t[i] - m1 - u[i] * m2);
+            }
+            if (A.du) R::store((T*)A.du + at, d, t);
+        }
+        if (A.sum_gate) {
+            float* to = A.part_g + ((size_t)grp * A.chunks + (A.chunks > 1 ? (int)blockIdx.x % A.chunks : 0)) * d;
+            T* out = (T*)A.dg + (size_t)grp * d;
+            flush_columns<T, G, NV>(sg, buf, d, [&](int c, float s) {
+                if (A.chunks > 1) to[c] = s;
+                else out[c] = (T)s;
+            });
+        }
+    }
+    if (A.part_w) {
+        float* to = A.part_w + (size_t)blockIdx.x * 4 * d;
+        if (A.wanted & 1) flush_columns<T, G, NV>(swa, buf, d, [&](int c, float s) { to[c] = s; });
+        if (A.wanted & 2) flush_columns<T, G, NV>(sba, buf, d, [&](int c, float s) { to[d + c] = s; });
+        if (A.wanted & 4) flush_columns<T, G, NV>(swb, buf, d, [&](int c, float s) { to[2 * d + c] = s; });
+        if (A.wanted & 8) flush_columns<T, G, NV>(sbb, buf, d, [&](int c, float s) { to[3 * d + c] = s; });
+    }
+}
+
+// Column sums of the workspace: blockIdx.y < 4 an affine gradient over the `blocks` workgroups, behind that a gate row
+// over its chunks.  64 columns x 16 rows of threads, the 16 added through LDS.
+struct ColumnSumArgs {
+    const float *part_w, *part_g;
+    void* out[4];
+    void* dg;
+    int blocks, chunks, d, first_y, param_type, type;
+};
+__device__ __forceinline__ void store_as(void* p, int type, size_t i, float v) {
+    if (type == PCLIP_DT_F32) ((float*)p)[i] = v;
+    else if (type == PCLIP_DT_BF16) ((__bf16*)p)[i] = (__bf16)v;
+    else ((_Float16*)p)[i] = (_Float16)v;
+}
+__global__ __launch_bounds__(1024) void column_sum_kernel(const ColumnSumArgs A) {
+    __shared__ float lds[16][65];
+    const int lane = threadIdx.x & 63, part = threadIdx.x >> 6, c = blockIdx.x * 64 + lane, k = blockIdx.y + A.first_y, d = A.d;
+    const bool gate = k >= 4;
+    if (!gate && !A.out[k]) return;
+    const float* p = gate ? A.part_g + (size_t)(k - 4) * A.chunks * d : A.part_w + (size_t)k * d;
+    const size_t stride = gate ? (size_t)d : (size_t)4 * d;
+    const int count = gate ? A.chunks : A.blocks;
+    float s = 0.f;
+    if (c < d)
+        for (int i = part; i < count; i += 16) s += p[i * stride + c];
+    lds[part][lane] = s;
+    __syncthreads();
+    if (part == 0 && c < d) {
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) s += lds[i][lane];
+        if (gate) store_as(A.dg, A.type, (size_t)(k - 4) * d + c, s);
+        else store_as(A.out[k], A.param_type, c, s);
+    }
+}
+
+// Lanes and vectors of a row: the fewest lanes whose vectors hold it with at most 16 elements a lane (the backward keeps
+// five column sums of that many registers).
+struct Shape { int lanes, vectors; };
+Shape shape_of(int d, int dtype) {
+    const int V = dtype == PCLIP_DT_F32 ? 4 : 8, most = 16 / V, vecs = (d + V - 1) / V;
+    for (int lanes : {16, 64, 256})
+        for (int nv = 1; nv <= most; nv *= 2)
+            if (vecs <= lanes * nv) return {lanes, nv};
+    return {256, most};
+}
+
+// How the backward divides the rows over workgroups (see NormGateArgs).  512 workgroups, two a compute unit, are aimed
+// at: more would write more partial sums than the rows themselves hold at the training sizes.
+void plan(NormGateArgs& A, int dtype, bool sums, int& blocks) {
+    const int slots = THREADS / shape_of(A.d, dtype).lanes;
+    const int target = sums ? 512 : 2048;
+    A.group_rows = A.sum_gate ? A.gate_rows : A.rows;
+    A.groups = A.rows / A.group_rows;
+    A.groups_per_block = 1;
+    A.chunks = 1;
+    A.chunk_rows = A.group_rows;
+    if (A.groups >= target) {
+        A.groups_per_block = (A.groups + target - 1) / target;
+    } else {
+        const int want = target / A.groups, most = (A.group_rows + slots - 1) / slots;   // a chunk has a row for every slot at least
+        A.chunks = want < most ? want : most;
+        A.chunk_rows = (A.group_rows + A.chunks - 1) / A.chunks;
+        A.chunks = (A.group_rows + A.chunk_rows - 1) / A.chunk_rows;
+    }
+    blocks = A.chunks > 1 ? A.groups * A.chunks : (A.groups + A.groups_per_block - 1) / A.groups_per_block;
+}
+
+template <typename T, int G, int NV>
+void launch(const NormGateArgs& A, bool fwd, int blocks, hipStream_t st) {
+    if (fwd) norm_gate_fwd_kernel<T, G, NV><<<blocks, THREADS, 0, st>>>(A);
+    else norm_gate_bwd_kernel<T, G, NV><<<blocks, THREADS, 0, st>>>(A);
+}
+template <typename T>
+void launch_shape(const NormGateArgs& A, Shape s, bool fwd, int blocks, hipStream_t st) {
+    constexpr int MOST = 16 / PclipVec<T>::N;
+    const int key = s.lanes * 8 + s.vectors;
+    switch (key) {
+        case 16 * 8 + 1: launch<T, 16, 1>(A, fwd, blocks, st); break;
+        case 16 * 8 + 2: launch<T, 16, 2>(A, fwd, blocks, st); break;
+        case 64 * 8 + 1: launch<T, 64, 1>(A, fwd, blocks, st); break;
+        case 64 * 8 + 2: launch<T, 64, 2>(A, fwd, blocks, st); break;
+        case 256 * 8 + 1: launch<T, 256, 1>(A, fwd, blocks, st); break;
+        case 256 * 8 + 2: launch<T, 256, 2>(A, fwd, blocks, st); break;
+        case 16 * 8 + 4: launch<T, 16, MOST>(A, fwd, blocks, st); break;     // f32 only
+        case 64 * 8 + 4: launch<T, 64, MOST>(A, fwd, blocks, st); break;
+        case 256 * 8 + 4: launch<T, 256, MOST>(A, fwd, blocks, st); break;
+    }
+}
+void launch_type(const NormGateArgs& A, int dtype, bool fwd, int blocks, hipStream_t st) {
+    const Shape s = shape_of(A.d, dtype);
+    if (dtype == PCLIP_DT_F32) launch_shape<float>(A, s, fwd, blocks, st);
+    else if (dtype == PCLIP_DT_BF16) launch_shape<__bf16>(A, s, fwd, blocks, st);
+    else launch_shape<_Float16>(A, s, fwd, blocks, st);
+}
+
+int check_common(const char* who, int rows, int d, int dtype, int param_type, const void* gate, int gate_kind, int gate_rows, int after, int before,
+                 float eps) {
+    PCLIP_REQUIRE(pclip_dtype_ok(dtype), "%s: unknown type %d", who, dtype);
+    PCLIP_REQUIRE(param_type == PCLIP_DT_F32 || param_type == dtype, "%s: affine parameters are f32 or of the rows' type", who);
+    PCLIP_REQUIRE(rows >= 1 && rows <= 0x7fff0000 && d >= 1 && d <= MAX_D, "%s: rows=%d d=%d (1 <= rows <= 2147418112, 1 <= d <= %d)", who, rows, d, MAX_D);
+    PCLIP_REQUIRE(after >= PCLIP_NORM_NONE && after <= PCLIP_NORM_RMS && before >= PCLIP_NORM_NONE && before <= PCLIP_NORM_RMS, "%s: unknown norm", who);
+    PCLIP_REQUIRE(gate_kind >= PCLIP_GATE_NONE && gate_kind <= PCLIP_GATE_BYTES && (gate_kind == PCLIP_GATE_NONE || gate), "%s: gate kind and pointer", who);
+    PCLIP_REQUIRE(gate_kind != PCLIP_GATE_ROWS || (gate_rows >= 1 && rows % gate_rows == 0), "%s: gate_rows=%d does not divide rows=%d", who, gate_rows, rows);
+    PCLIP_REQUIRE(eps >= 0.f, "%s: eps must be zero or more", who);
+    return PCLIP_OK;
+}
+
+}  // namespace
+
+extern "C" int pclip_norm_gate_fwd(const void* u, const void* r, const void* gate, int gate_kind, int gate_rows, float scale, int after, const void* wa,
+                                   const void* ba, int before, const void* wb, const void* bb, int param_type, float eps, int rows, int d, int dtype,
+                                   void* y, void* n, float* stats, void* stream) {
+    int rc = check_common("norm_gate_fwd", rows, d, dtype, param_type, gate, gate_kind, gate_rows, after, before, eps);
+    if (rc) return rc;
+    PCLIP_REQUIRE(u && y && (before == PCLIP_NORM_NONE || n), "norm_gate_fwd: null pointer");
+    PCLIP_REQUIRE(((uintptr_t)stats & 15) == 0, "norm_gate_fwd: stats must be 16-byte aligned");
+    NormGateArgs A = {};
+    A.u = u, A.r = r, A.gate = gate, A.wa = wa, A.ba = ba, A.wb = wb, A.bb = bb, A.y = y, A.n = n, A.stats = (float4*)stats;
+    A.rows = rows, A.d = d, A.gate_rows = gate_kind == PCLIP_GATE_ROWS ? gate_rows : 1, A.gate_kind = gate_kind, A.after = after, A.before = before;
+    A.param_f32 = param_type == PCLIP_DT_F32, A.scale = scale, A.eps = eps;
+    const int slots = THREADS / shape_of(d, dtype).lanes;
+    const long long want = ((long long)rows + slots - 1) / slots;
+    launch_type(A, dtype, true, want < 4096 ? (int)want : 4096, (hipStream_t)stream);
+    return pclip_check_launch("norm_gate_fwd");
+}
+
+extern "C" size_t pclip_norm_gate_bwd_workspace_bytes(int rows, int d, int dtype, int gate_rows) {
+    if (rows < 1 || rows > 0x7fff0000 || d < 1 || d > MAX_D || !pclip_dtype_ok(dtype) || gate_rows < 0 || (gate_rows && rows % gate_rows)) return 0;
+    NormGateArgs A = {};
+    A.rows = rows, A.d = d, A.gate_rows = gate_rows ? gate_rows : 1, A.sum_gate = gate_rows > 1;
+    int blocks = 0;
+    plan(A, dtype, true, blocks);
+    return ((size_t)blocks * 4 + (A.chunks > 1 && A.sum_gate ? (size_t)A.groups * A.chunks : 0)) * d * sizeof(float);
+}
+
+extern "C" int pclip_norm_gate_bwd(const void* u, const void* r, const void* gate, int gate_kind, int gate_rows, float scale, int after, const void* wa,
+                                   const void* ba, int before, const void* wb, const void* bb, int param_type, float eps, int rows, int d, int dtype,
+                                   const float* stats, const void* dy, const void* dn, void* du, void* dr, void* dgate, void* dwa, void* dba, void* dwb,
+                                   void* dbb, void* ws, size_t ws_bytes, void* stream) {
+    int rc = check_common("norm_gate_bwd", rows, d, dtype, param_type, gate, gate_kind, gate_rows, after, before, eps);
+    if (rc) return rc;
+    PCLIP_REQUIRE(u && (dy || dn), "norm_gate_bwd: null pointer");
+    PCLIP_REQUIRE((after == PCLIP_NORM_NONE && before == PCLIP_NORM_NONE) || stats, "norm_gate_bwd: the forward's statistics are needed");
+    PCLIP_REQUIRE(((uintptr_t)stats & 15) == 0, "norm_gate_bwd: stats must be 16-byte aligned");
+    PCLIP_REQUIRE(!dgate || gate_kind == PCLIP_GATE_ROWS, "norm_gate_bwd: a byte mask has no gradient");
+    PCLIP_REQUIRE((!dwa || after) && (!dba || after) && (!dwb || before) && (!dbb || before), "norm_gate_bwd: affine gradient of a norm that is not there");
+    NormGateArgs A = {};
+    A.u = u, A.r = r, A.gate = gate, A.wa = wa, A.ba = ba, A.wb = wb, A.bb = bb, A.stats = (float4*)stats, A.dy = dy, A.dn = dn, A.du = du, A.dr = dr;
+    A.dg = dgate, A.rows = rows, A.d = d, A.gate_rows = gate_kind == PCLIP_GATE_ROWS ? gate_rows : 1, A.gate_kind = gate_kind, A.after = after;
+    A.before = before, A.param_f32 = param_type == PCLIP_DT_F32, A.scale = scale, A.eps = eps, A.sum_gate = dgate && A.gate_rows > 1;
+    A.wanted = (dwa ? 1 : 0) | (dba ? 2 : 0) | (dwb ? 4 : 0) | (dbb ? 8 : 0);
+    const bool affine = A.wanted != 0;
+    int blocks = 0;
+    plan(A, dtype, affine || A.sum_gate, blocks);
+    const bool gate_parts = A.sum_gate && A.chunks > 1;
+    const size_t w_floats = affine ? (size_t)blocks * 4 * d : 0, need = (w_floats + (gate_parts ? (size_t)A.groups * A.chunks * d : 0)) * sizeof(float);
+    PCLIP_REQUIRE(need == 0 || (ws && ws_bytes >= need), "norm_gate_bwd: workspace too small (%zu bytes, need %zu)", ws_bytes, need);
+    A.part_w = affine ? (float*)ws : nullptr;
+    A.part_g = gate_parts ? (float*)ws + w_floats : nullptr;
+    launch_type(A, dtype, false, blocks, (hipStream_t)stream);
+    if (affine || gate_parts) {
+        ColumnSumArgs S = {};
+        S.part_w = A.part_w, S.part_g = A.part_g, S.out[0] = dwa, S.out[1] = dba, S.out[2] = dwb, S.out[3] = dbb, S.dg = dgate;
+        S.blocks = blocks, S.chunks = A.chunks, S.d = d, S.first_y = affine ? 0 : 4, S.param_type = param_type, S.type = dtype;
+        const int ny = (affine ? 4 : 0) + (gate_parts ? A.groups : 0);
+        column_sum_kernel<<<dim3((d + 63) / 64, ny), 1024, 0, (hipStream_t)stream>>>(S);
+    }
+    return pclip_check_launch("norm_gate_bwd");
+}

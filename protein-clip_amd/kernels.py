@@ -2,6 +2,7 @@
 workspace allocation through torch, one C call each.  No arithmetic happens here."""
 from __future__ import annotations
 
+import bisect
 import collections
 import ctypes
 import threading
@@ -188,6 +189,230 @@ def head_tail_bwd(pooled, params, keep, keep_scale: float, ln_eps: float, t, sav
     check(lib.pclip_head_tail_bwd(ptr(pooled), _head_pointers(params), nblk, ptr(keep), float(keep_scale), ptr(tt), ptr(save), ptr(dout), B, d,
                                   ptr(dpooled), _head_pointers(dparams), ptr(dt), ptr(ws), ws.numel(), stream_of(pooled)), "pclip_head_tail_bwd")
     return dpooled, dparams, dt
+
+
+# ---- token head: linear layer, norms around a block, gradient clipping --------------------
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # PCLIP_DT_*
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}                # PCLIP_ACT_*
+NORMS = {None: 0, "layer": 1, "rms": 2}                                   # PCLIP_NORM_*
+GATE_NONE, GATE_ROWS, GATE_BYTES = 0, 1, 2                                # PCLIP_GATE_*
+LINEAR_MAX_DIM = 65536
+NORM_MAX_D = 4096
+MAX_ROWS = 2**31 - 2**16
+
+
+class _on:
+    """Makes ``device`` the current one for a call into the library when it is not (a launch needs the device
+    of its stream to be current)."""
+
+    def __init__(self, device):
+        self.device, self.other = device, None
+
+    def __enter__(self):
+        if torch.cuda.current_device() != self.device.index:
+            self.other = torch.cuda.device(self.device)
+            self.other.__enter__()
+
+    def __exit__(self, *exc):
+        if self.other is not None:
+            self.other.__exit__(*exc)
+        return False
+
+
+def _operand(t, name: str, shape, dtype, device):
+    """A contiguous GPU tensor of this shape, type and device (or None) -> its pointer."""
+    if t is None:
+        return None
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous():
+        require_gpu_tensor(t, dtype, name)
+        raise _lib.PclipError(f"{name}: expected shape {tuple(shape)} on {device}, got {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _typed(t, name: str, dim: int):
+    """Element type code of a contiguous GPU tensor with ``dim`` dimensions."""
+    code = DTYPES.get(t.dtype)
+    if code is None:
+        raise _lib.PclipError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    require_gpu_tensor(t, t.dtype, name)
+    if t.dim() != dim:
+        raise _lib.PclipError(f"{name}: expected {dim} dimensions, got shape {tuple(t.shape)}")
+    return code
+
+
+def _check_rows(rows: int, what: str):
+    if not 1 <= rows <= MAX_ROWS:
+        raise _lib.PclipError(f"{what}: {rows} rows (1 to {MAX_ROWS})")
+
+
+def _linear_sizes(x, w):
+    code = _typed(x, "x", 2)
+    _typed(w, "weight", 2)
+    (M, K), N = x.shape, w.shape[0]
+    if w.dtype != x.dtype or w.shape[1] != K or w.device != x.device:
+        raise _lib.PclipError(f"linear: weight {tuple(w.shape)} {w.dtype} on {w.device} does not fit x {tuple(x.shape)} {x.dtype} on {x.device}")
+    _check_rows(M, "linear")
+    if not (1 <= K <= LINEAR_MAX_DIM and 1 <= N <= LINEAR_MAX_DIM):
+        raise _lib.PclipError(f"linear: widths {K} -> {N} (1 to {LINEAR_MAX_DIM})")
+    return M, K, N, code
+
+
+def linear_fwd(x, w, bias=None, residual=None, activation: str = "none", want_slope: bool = False):
+    """``act(x @ w.T + bias) + residual`` for x [M,K], w [N,K], bias [N], residual [M,N] of one type.
+    Returns (y [M,N], slope): slope = act'(z) [M,N] when asked for (what :func:`linear_bwd` needs), else None."""
+    M, K, N, code = _linear_sizes(x, w)
+    dev = x.device
+    b, r = _operand(bias, "bias", (N,), x.dtype, dev), _operand(residual, "residual", (M, N), x.dtype, dev)
+    y = _empty((M, N), x.dtype, dev)
+    slope = _empty((M, N), x.dtype, dev) if want_slope else None
+    with _on(dev):
+        check(_lib.load().pclip_linear_fwd(x.data_ptr(), w.data_ptr(), b, r, M, K, N, code, ACTIVATIONS[activation], y.data_ptr(),
+                                           slope.data_ptr() if want_slope else None, stream_of(x)), "pclip_linear_fwd")
+    return y, slope
+
+
+def linear_bwd(x, w, dy, saved=None, saved_is_output: bool = False, activation: str = "none", want_dx: bool = True, want_dw: bool = True,
+               want_db: bool = True):
+    """Returns (dx, dw, db), None where not wanted.  ``saved``: the forward's slope, or its output with
+    ``saved_is_output`` (relu without a residual), None for activation "none"."""
+    M, K, N, code = _linear_sizes(x, w)
+    dev, act = x.device, ACTIVATIONS[activation]
+    g, s = _operand(dy, "dy", (M, N), x.dtype, dev), _operand(saved, "saved", (M, N), x.dtype, dev)
+    lib = _lib.load()
+    dx = _empty((M, K), x.dtype, dev) if want_dx else None
+    dw = _empty((N, K), x.dtype, dev) if want_dw else None
+    db = _empty((N,), x.dtype, dev) if want_db else None
+    # scratch of the call's own (not the stream's shared buffer): a captured graph keeps it for its replays
+    ws = _empty((lib.pclip_linear_bwd_workspace_bytes(M, K, N, code, act),), torch.uint8, dev)
+    with _on(dev):
+        check(lib.pclip_linear_bwd(x.data_ptr(), w.data_ptr(), g, s, int(saved_is_output), M, K, N, code, act, ptr(dx), ptr(dw), ptr(db),
+                                   ws.data_ptr(), ws.numel(), stream_of(x)), "pclip_linear_bwd")
+    return dx, dw, db
+
+
+def _norm_gate_args(u, r, gate, gate_rows, after, wa, ba, before, wb, bb):
+    code = _typed(u, "u", 2)
+    rows, d = u.shape
+    dev = u.device
+    _check_rows(rows, "norm_gate")
+    if not 1 <= d <= NORM_MAX_D:
+        raise _lib.PclipError(f"norm_gate: row width {d} (1 to {NORM_MAX_D})")
+    params = [p for p in (wa, ba, wb, bb) if p is not None]
+    ptype = params[0].dtype if params else torch.float32
+    if ptype not in (torch.float32, u.dtype):
+        raise _lib.PclipError(f"norm_gate: affine parameters must be float32 or {u.dtype}, got {ptype}")
+    kind = GATE_NONE
+    if gate is not None:
+        kind = GATE_BYTES if gate.dtype == torch.uint8 else GATE_ROWS
+        if kind == GATE_BYTES:
+            _operand(gate, "gate", (rows, d), torch.uint8, dev)
+        else:
+            if gate_rows < 1 or rows % gate_rows:
+                raise _lib.PclipError(f"norm_gate: gate_rows={gate_rows} does not divide {rows} rows")
+            _operand(gate, "gate", (rows // gate_rows, d), u.dtype, dev)
+    ops = [_operand(p, n, (d,), ptype, dev) for p, n in ((wa, "wa"), (ba, "ba"), (wb, "wb"), (bb, "bb"))]
+    return (rows, d, code, kind, DTYPES[ptype], ptype, u.data_ptr(), _operand(r, "residual", (rows, d), u.dtype, dev), ptr(gate)) + tuple(ops)
+
+
+def norm_gate_fwd(u, r=None, gate=None, gate_rows: int = 1, scale: float = 1.0, after=None, wa=None, ba=None, before=None, wb=None, bb=None,
+                  eps: float = 1e-5, want_stats: bool = False):
+    """``y = r + scale * gate * norm_after(u)`` and ``n = norm_before(y)`` for u, r [rows,d]; gate [rows / gate_rows, d] of u's
+    type or a byte mask [rows,d]; ``after`` / ``before``: None, "layer" or "rms" with their affine vectors [d].
+    Returns (y, n or None, stats or None); ``stats`` is what :func:`norm_gate_bwd` needs."""
+    rows, d, code, kind, pcode, _, pu, pr, pg, pwa, pba, pwb, pbb = _norm_gate_args(u, r, gate, gate_rows, after, wa, ba, before, wb, bb)
+    dev = u.device
+    y = _empty((rows, d), u.dtype, dev)
+    n = _empty((rows, d), u.dtype, dev) if before else None
+    stats = _empty((rows, 4), F32, dev) if want_stats and (after or before) else None
+    with _on(dev):
+        check(_lib.load().pclip_norm_gate_fwd(pu, pr, pg, kind, gate_rows, scale, NORMS[after], pwa, pba, NORMS[before], pwb, pbb, pcode, eps, rows, d,
+                                              code, y.data_ptr(), ptr(n), ptr(stats), stream_of(u)), "pclip_norm_gate_fwd")
+    return y, n, stats
+
+
+def norm_gate_bwd(u, r, gate, gate_rows, scale, after, wa, ba, before, wb, bb, eps, stats, dy, dn, want=(True,) * 7):
+    """Gradients (du, dr, dgate, dwa, dba, dwb, dbb) of :func:`norm_gate_fwd`, None where ``want`` says so or the operand is
+    absent.  ``dy`` / ``dn`` may be None (zero), not both."""
+    rows, d, code, kind, pcode, ptype, pu, pr, pg, pwa, pba, pwb, pbb = _norm_gate_args(u, r, gate, gate_rows, after, wa, ba, before, wb, bb)
+    dev = u.device
+    pdy, pdn = _operand(dy, "dy", (rows, d), u.dtype, dev), _operand(dn, "dn", (rows, d), u.dtype, dev)
+    pst = _operand(stats, "stats", (rows, 4), F32, dev)
+    outs = [_empty(shape, dt, dev) if w and there else None
+            for w, there, shape, dt in zip(want, (True, r is not None, kind == GATE_ROWS, wa is not None, ba is not None, wb is not None, bb is not None),
+                                           ((rows, d), (rows, d), (rows // gate_rows, d)) + ((d,),) * 4, (u.dtype,) * 3 + (ptype,) * 4)]
+    lib = _lib.load()
+    sum_rows = gate_rows if outs[2] is not None else 0
+    nbytes = lib.pclip_norm_gate_bwd_workspace_bytes(rows, d, code, sum_rows) if sum_rows > 1 or any(o is not None for o in outs[3:]) else 0
+    ws = _empty((nbytes,), torch.uint8, dev) if nbytes else None   # the call's own, see linear_bwd
+    with _on(dev):
+        check(lib.pclip_norm_gate_bwd(pu, pr, pg, kind, gate_rows, scale, NORMS[after], pwa, pba, NORMS[before], pwb, pbb, pcode, eps, rows, d, code, pst,
+                                      pdy, pdn, *[ptr(o) for o in outs], ptr(ws), nbytes, stream_of(u)), "pclip_norm_gate_bwd")
+    return tuple(outs)
+
+
+def _dense(t) -> bool:
+    """Whether the tensor's elements fill one stretch of memory, in any order of its dimensions."""
+    if t.is_contiguous():
+        return True
+    expected = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
+        if stride != expected:
+            return False
+        expected *= size
+    return True
+
+
+def _check_disjoint(src, dst):
+    """No destination may share memory with another tensor of the call (its own source excepted): workgroups of
+    different tensors run side by side."""
+    spans = sorted((d.data_ptr(), d.data_ptr() + d.numel() * d.element_size()) for d in dst if d.numel())
+    for (_, end), (start, _) in zip(spans, spans[1:]):
+        if start < end:
+            raise _lib.PclipError("grad_clip: two of the written tensors share memory (the same gradient twice?)")
+    starts = [s for s, _ in spans]
+    for s, d in zip(src, dst):
+        p = s.data_ptr()
+        if p == d.data_ptr() or not s.numel():
+            continue
+        k = bisect.bisect_left(starts, p + s.numel() * s.element_size()) - 1   # the last span that begins before s ends
+        if k >= 0 and spans[k][1] > p:
+            raise _lib.PclipError("grad_clip: a written tensor shares memory with another tensor that is read")
+
+
+def grad_clip(src, dst=None, max_norm: float = 0.0, eps: float = 1e-6) -> torch.Tensor:
+    """Norm [1] of all elements of the tensors ``src``; with ``dst`` (tensors of the same shapes; ``src`` itself: in place)
+    also ``dst = src * min(1, max_norm / (norm + eps))``.  One launch a pass for every 120 tensors."""
+    src = list(src)
+    if not src:
+        raise _lib.PclipError("grad_clip: no tensors")
+    n, dev = len(src), src[0].device
+    for i, t in enumerate(src):
+        if t.dtype not in DTYPES or t.device != dev or not t.is_cuda or t.layout != torch.strided:
+            raise _lib.PclipError(f"grad_clip: tensor {i}: expected a dense float32, bfloat16 or float16 GPU tensor on {dev}, got {t.dtype} on {t.device}")
+        if not _dense(t):
+            raise _lib.PclipError(f"grad_clip: tensor {i} has gaps or shared elements (strides {t.stride()} of shape {tuple(t.shape)})")
+    out, out_types = None, None
+    if dst is not None:
+        dst = list(dst)
+        if len(dst) != n:
+            raise _lib.PclipError(f"grad_clip: {len(dst)} destinations for {n} tensors")
+        for i, (s, d) in enumerate(zip(src, dst)):
+            if d is s:
+                continue
+            if d.dtype not in DTYPES or d.device != dev or d.shape != s.shape or d.layout != torch.strided or (d.stride() != s.stride() and not (
+                    d.is_contiguous() and s.is_contiguous())):
+                raise _lib.PclipError(f"grad_clip: destination {i} must have the shape, layout and device of its tensor and a supported type")
+        _check_disjoint(src, dst)
+        out = (ctypes.c_void_p * n)(*[d.data_ptr() for d in dst])
+        out_types = (ctypes.c_int * n)(*[DTYPES[d.dtype] for d in dst])
+    lib = _lib.load()
+    norm = _empty((1,), F32, dev)
+    ws = _empty((lib.pclip_grad_clip_workspace_bytes(n),), torch.uint8, dev)   # the call's own, see linear_bwd
+    with _on(dev):
+        check(lib.pclip_grad_clip((ctypes.c_void_p * n)(*[t.data_ptr() for t in src]), (ctypes.c_int64 * n)(*[t.numel() for t in src]),
+                                  (ctypes.c_int * n)(*[DTYPES[t.dtype] for t in src]), out, out_types, n, max_norm, eps, norm.data_ptr(), ws.data_ptr(),
+                                  ws.numel(), stream_of(norm)), "pclip_grad_clip")
+    return norm
 
 
 # ---- L2 normalise + scale ---------------------------------------------------------------

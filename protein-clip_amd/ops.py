@@ -14,10 +14,12 @@ logic can be exercised on CPU by tests that bring their own stand-in.
 """
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
 import torch.distributed as dist
+from torch.autograd.function import once_differentiable
 
 from . import kernels as _hip_kernels
 
@@ -130,6 +132,199 @@ def embedding_head(pooled: torch.Tensor, params, temperature: torch.Tensor, keep
     ``[W, b]`` of the last Linear; ``keep`` = the dropout masks ``[blocks, B, d]`` (uint8, None in
     eval mode) with ``keep_scale = 1 / (1 - p)``.  Returns ``normalize(z) * exp(temperature / 2)``."""
     return _HeadTail.apply(_f32(pooled), _f32(temperature), keep, float(keep_scale), float(ln_eps), kernels or _hip_kernels, *params)
+
+
+# --------------------------------------------------------------------------------------
+# token head: linear layers, norms around a block   (modules/models.py:54-73)
+# --------------------------------------------------------------------------------------
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation, K):
+        product = any(ctx.needs_input_grad[:3])
+        output = activation == "relu" and residual is None   # the sign of y says where the slope is one
+        if x.shape[0] == 0:
+            y, slope = x.new_empty(0, weight.shape[0]), None
+        else:
+            y, slope = K.linear_fwd(x, weight, bias, residual, activation, want_slope=product and activation != "none" and not output)
+        ctx.K, ctx.activation, ctx.output = K, activation, output
+        ctx.save_for_backward(x, weight, y if output and product else slope)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, saved = ctx.saved_tensors
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        dx = dw = db = None
+        if x.shape[0] == 0:
+            dx, dw, db = torch.zeros_like(x), torch.zeros_like(weight), weight.new_zeros(weight.shape[0])
+        elif need_x or need_w or need_b:
+            dx, dw, db = ctx.K.linear_bwd(x, weight, dy.contiguous(), saved, ctx.output, ctx.activation, need_x, need_w, need_b)
+        return dx if need_x else None, dw if need_w else None, db if need_b else None, dy if need_r else None, None, None
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+               activation: str = "none", kernels=None) -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual`` with everything behind the product in its epilogue: a layer of the towers'
+    projection and per-residue network (modules/models.py:32-52, 54-73).
+
+    ``x [..., K]`` float32, bfloat16 or float16 (f32 sums; one rounding at the end), ``weight [N, K]``, ``bias [N]``,
+    ``residual`` broadcastable to ``[..., N]``; operands of another type are cast to ``x``'s, through autograd.
+    ``activation``: "none", "relu", "gelu" (with erf) or "silu".  First derivatives only."""
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"linear_act: x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise ValueError(f"linear_act: bias must have shape ({weight.shape[0]},), got {tuple(bias.shape)}")
+    if activation not in _hip_kernels.ACTIVATIONS:
+        raise ValueError(f"linear_act: unknown activation {activation!r}")
+    K = kernels or _hip_kernels
+    shape = x.shape[:-1] + (weight.shape[0],)
+    x2 = x.reshape(-1, x.shape[-1]) if x.numel() else x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
+    x2 = x2.contiguous()
+    weight = weight.to(x.dtype).contiguous()
+    if bias is not None:
+        bias = bias.to(x.dtype).contiguous()
+    if residual is not None:
+        residual = residual.to(x.dtype).expand(shape).reshape(x2.shape[0], weight.shape[0]).contiguous()
+    if x2.shape[0] == 0 or _wants_grad(x2, weight, bias, residual):
+        y = _LinearAct.apply(x2, weight, bias, residual, activation, K)
+    else:
+        y, _ = K.linear_fwd(x2, weight, bias, residual, activation)
+    return y.reshape(shape)
+
+
+class _NormGate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, u, r, gate, wa, ba, wb, bb, gate_rows, scale, after, before, eps, K):
+        ctx.set_materialize_grads(False)
+        if u.shape[0] == 0:
+            y, n, stats = torch.empty_like(u), torch.empty_like(u) if before else None, None
+        else:
+            y, n, stats = K.norm_gate_fwd(u, r, gate, gate_rows, scale, after, wa, ba, before, wb, bb, eps, want_stats=True)
+        ctx.K, ctx.cfg = K, (gate_rows, scale, after, before, eps)
+        ctx.save_for_backward(u, r, gate, wa, ba, wb, bb, stats)
+        return (y, n) if before else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dn=None):
+        u, r, gate, wa, ba, wb, bb, stats = ctx.saved_tensors
+        gate_rows, scale, after, before, eps = ctx.cfg
+        need = ctx.needs_input_grad[:7]
+        if dy is None and dn is None:
+            return (None,) * 13
+        if u.shape[0] == 0:
+            return tuple(torch.zeros_like(t) if w else None for t, w in zip((u, r, gate, wa, ba, wb, bb), need)) + (None,) * 6
+        dy = None if dy is None else dy.contiguous()
+        dn = None if dn is None else dn.contiguous()
+        grads = ctx.K.norm_gate_bwd(u, r, gate, gate_rows, scale, after, wa, ba, before, wb, bb, eps, stats, dy, dn, want=need)
+        return tuple(grads) + (None,) * 6
+
+
+def _gate_rows(gate: torch.Tensor, lead, d: int):
+    """(gate as [groups, d], rows of the operand that share a row of it), or None when its shape is no such pattern: its
+    leading dimensions must be the operand's first ones followed by ones."""
+    if gate.shape[-1] != d:
+        return None
+    dims = (1,) * (len(lead) + 1 - gate.dim()) + tuple(gate.shape[:-1])
+    j = 0
+    while j < len(lead) and dims[j] == lead[j]:
+        j += 1
+    if any(s != 1 for s in dims[j:]):
+        return None
+    return gate.reshape(-1, d), math.prod(lead[j:])
+
+
+def norm_gate_residual(u: torch.Tensor, residual: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, scale: float = 1.0,
+                       after=None, before=None, norm: str = "layer", eps: float = 1e-5, kernels=None):
+    """``y = residual + scale * gate * norm(u)``, and with ``before`` also ``norm(y)``: what stands between two blocks of a
+    network, in one pass (in the per-residue network: the LayerNorm and Dropout of modules/models.py:54-73).
+
+    ``u [..., d]`` a block's output (float32, bfloat16 or float16; statistics, sums and ``y`` in f32, rounded once);
+    ``after``: ``(weight, bias)`` of the norm that closes the block, either may be None, or None for no norm;
+    ``before``: the same of the norm that opens the next one; ``norm``: "layer" or "rms" (no mean), with ``eps``.
+    ``gate``: a tensor broadcastable to ``u`` (a channel's, a sequence's, an element's; with a gradient) or a bool / uint8
+    dropout mask of ``u``'s shape, used with ``scale = 1 / (1 - p)``.
+    Returns ``y``, or ``(y, norm(y))`` when ``before`` is given.  First derivatives only."""
+    if u.dim() < 1 or norm not in ("layer", "rms"):
+        raise ValueError("norm_gate_residual: expected u [..., d] and norm 'layer' or 'rms'")
+    if isinstance(scale, torch.Tensor):
+        raise ValueError("norm_gate_residual: scale is a number (a learned scale is a gate)")
+    K = kernels or _hip_kernels
+    d, lead = u.shape[-1], tuple(u.shape[:-1])
+    rows = math.prod(lead)
+    u2 = u.reshape(rows, d).contiguous()
+    wa, ba = (None, None) if after is None else after
+    wb, bb = (None, None) if before is None else before
+    params = [wa, ba, wb, bb]
+    for p in params:
+        if p is not None and tuple(p.shape) != (d,):
+            raise ValueError(f"norm_gate_residual: affine parameters must have shape ({d},), got {tuple(p.shape)}")
+    types = {p.dtype for p in params if p is not None}
+    if types and types not in ({torch.float32}, {u.dtype}):
+        params = [None if p is None else p.float() for p in params]
+    params = [None if p is None else p.contiguous() for p in params]
+    gate_rows = 1
+    if gate is not None:
+        if gate.dtype == torch.bool:
+            gate = gate.to(torch.uint8)
+        if gate.dtype == torch.uint8:
+            gate = gate.expand(u.shape).reshape(rows, d).contiguous()
+        else:
+            if gate.dim() > u.dim():
+                raise ValueError(f"norm_gate_residual: gate {tuple(gate.shape)} does not broadcast to u {tuple(u.shape)}")
+            gate = gate.to(u.dtype)
+            found = _gate_rows(gate, lead, d) if gate.dim() and rows else None
+            if found is None:   # any other broadcast is written out
+                found = gate.expand(u.shape).reshape(rows, d), 1
+            gate, gate_rows = found[0].contiguous(), found[1]
+    if residual is not None:
+        residual = residual.to(u.dtype).expand(u.shape).reshape(rows, d).contiguous()
+    kinds = [norm if pair is not None else None for pair in (after, before)]
+    if rows == 0 or _wants_grad(u2, residual, gate, *params):
+        out = _NormGate.apply(u2, residual, gate, *params, gate_rows, float(scale), kinds[0], kinds[1], float(eps), K)
+    else:
+        y, n, _ = K.norm_gate_fwd(u2, residual, gate, gate_rows, float(scale), kinds[0], params[0], params[1], kinds[1], params[2], params[3], float(eps))
+        out = (y, n) if kinds[1] else y
+    return tuple(o.reshape(u.shape) for o in out) if kinds[1] else out.reshape(u.shape)
+
+
+# --------------------------------------------------------------------------------------
+# gradient norm and clipping   (between backward and step of modules/training_utils.py:7, 92)
+# --------------------------------------------------------------------------------------
+def grad_norm(grads, kernels=None) -> torch.Tensor:
+    """L2 norm of all elements of the tensors ``grads`` as a 0-d float32 tensor on their device, without a host sync."""
+    return (kernels or _hip_kernels).grad_clip(grads).reshape(())
+
+
+def clip_grads(grads, max_norm: float, out=None, eps: float = 1e-6, kernels=None) -> torch.Tensor:
+    """``out = grads * min(1, max_norm / (norm + eps))`` for a list of tensors and their global L2 norm, which is returned
+    (0-d float32, on the device; nothing waits for the host).  ``out``: tensors of the same shapes, of any supported
+    type (the 32-bit gradients of an optimizer filled from a bfloat16 all-reduce buffer, say); None: in place."""
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"clip_grads: max_norm must be zero or more, got {max_norm}")
+    grads = list(grads)
+    return (kernels or _hip_kernels).grad_clip(grads, grads if out is None else out, max_norm, float(eps)).reshape(())
+
+
+def clip_grad_norm_(parameters, max_norm: float, eps: float = 1e-6, error_if_nonfinite: bool = False, kernels=None) -> torch.Tensor:
+    """Clips the gradients of ``parameters`` (an iterable of tensors, or one) in place and returns their norm before clipping, as
+    ``torch.nn.utils.clip_grad_norm_`` does; parameters without a gradient are left out.  With
+    ``error_if_nonfinite`` the norm is read by the host first and the gradients stay as they are when it is not finite."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.zeros(())
+    if error_if_nonfinite:
+        norm = grad_norm(grads, kernels)
+        if not bool(torch.isfinite(norm)):
+            raise RuntimeError(f"clip_grad_norm_: the gradient norm is {norm.item()}")
+    return clip_grads(grads, max_norm, eps=eps, kernels=kernels)
 
 
 def l2norm_scale(e: torch.Tensor, temperature: torch.Tensor, kernels=None) -> torch.Tensor:
