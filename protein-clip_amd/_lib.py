@@ -100,7 +100,7 @@ def ptr(t):
 
 
 def stream_of(t: torch.Tensor):
-    return c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+    return c_void_p(torch._C._cuda_getCurrentRawStream(t.device.index))   # without building a Stream object: 0.4 us instead of 2
 
 
 def check(rc: int, what: str):

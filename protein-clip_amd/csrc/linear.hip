@@ -96,26 +96,30 @@ struct Tile {
         }
     }
     // chunk c of the tile whose first row is i0 and first k is k0: elements outside rows x k are zero
-    static __device__ __forceinline__ u32x4 fetch(const T* p, int ld, int i0, int rows, long long k0, long long k_end, int c) {
+    static __device__ __forceinline__ u32x4 fetch_edge(const T* p, int ld, int i0, int rows, long long k0, long long k_end, int c) {
         int row, k;
         slot(c, row, k);
         const long long kk = k0 + k;
         const int i = i0 + row;
-        long long valid;
-        const T* at;
-        if constexpr (ALONG_K) {
-            valid = i < rows ? k_end - kk : 0;
-            at = p + (long long)i * ld + kk;
-        } else {
-            valid = kk < k_end ? rows - i : 0;
-            at = p + kk * ld + i;
-        }
-        if (valid >= V) return __builtin_bit_cast(u32x4, *(const PclipPack<T, V>*)at);
+        const long long valid = ALONG_K ? (i < rows ? k_end - kk : 0) : (kk < k_end ? rows - i : 0);
+        const T* at = ALONG_K ? p + (long long)i * ld + kk : p + kk * ld + i;
         PclipPack<T, V> a;
 #pragma unroll
         for (int e = 0; e < V; e++) a.v[e] = e < valid ? at[e] : (T)0.f;
         return __builtin_bit_cast(u32x4, a);
     }
+    // Inside the matrix a chunk's address is the tile's (the same for all lanes, kept in scalar registers) plus this offset,
+    // which no step changes.  Rows behind the last one read the last one again when they lie along k: nothing of them is stored.
+    static __device__ __forceinline__ unsigned offset(int ld, int i0, int rows, int c) {
+        int row, k;
+        slot(c, row, k);
+        if (ALONG_K) row = min(row, rows - 1 - i0);
+        return (unsigned)(ALONG_K ? row * ld + k : k * ld + row) * (unsigned)sizeof(T);
+    }
+    static __device__ __forceinline__ const char* origin(const T* p, int ld, int i0, long long k0) {
+        return (const char*)(ALONG_K ? p + (long long)i0 * ld + k0 : p + k0 * ld + i0);
+    }
+    static __device__ __forceinline__ bool inside(int i0, int rows) { return ALONG_K || i0 + ROWS <= rows; }
 };
 
 // ---- activations --------------------------------------------------------------------------------
@@ -164,6 +168,31 @@ __device__ __forceinline__ float activate(float z, int act, float& slope) {
     return z;
 }
 
+// The slope is kept for the backward: as it is for f32, for 16-bit types as a whole number of steps of 1 / 28672 (slopes lie
+// between -0.13 and 1.13; half a step is a fifteenth of an f16 rounding at one), so that dz is rounded once, not twice.
+template <typename T> using SlopeOf = std::conditional_t<sizeof(T) == 4, float, short>;
+template <typename T> constexpr float SLOPE_UNIT = sizeof(T) == 4 ? 1.f : 1.f / 28672.f;
+
+// VW columns of one row in 16-byte accesses
+template <typename T, int VW>
+__device__ __forceinline__ void load_run(const T* p, int valid, float (&v)[VW]) {
+    constexpr int V = VW < PclipVec<T>::N ? VW : PclipVec<T>::N;
+#pragma unroll
+    for (int e = 0; e < VW; e += V) load_f32<T, V>(p + e, valid - e, *(float(*)[V])(v + e));
+}
+template <typename T, int VW>
+__device__ __forceinline__ void store_run(T* p, int valid, const float (&v)[VW]) {
+    constexpr int V = VW < PclipVec<T>::N ? VW : PclipVec<T>::N;
+#pragma unroll
+    for (int e = 0; e < VW; e += V) store_f32<T, V>(p + e, valid - e, *(const float(*)[V])(v + e));
+}
+template <typename T, int VW>
+__device__ __forceinline__ void store_slope(SlopeOf<T>* p, int valid, float (&v)[VW]) {
+#pragma unroll
+    for (int e = 0; e < VW; e++) v[e] = sizeof(T) == 4 ? v[e] : rintf(v[e] * 28672.f);
+    store_run<SlopeOf<T>, VW>(p, valid, v);
+}
+
 // ---- the product -----------------------------------------------------------------------------------
 enum { EPI_FORWARD, EPI_STORE, EPI_SLAB };
 
@@ -185,7 +214,7 @@ __device__ __forceinline__ int xcd_order(int b, int n) {
 }
 
 template <typename T, int BI, int BJ, int WI, int WJ, bool PK, bool QK, int EPI>
-__global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(const GemmArgs A) {
+__global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_kernel(const GemmArgs A) {
     typedef Tile<T, BI, PK> TP;
     typedef Tile<T, BJ, QK> TQ;
     typedef typename Mfma<T>::Frag Frag;
@@ -204,11 +233,30 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(const GemmArgs A) {
     const T *P = (const T*)A.P, *Q = (const T*)A.Q;
 
     u32x4 rp[NP], rq[NQ];
+    unsigned op[NP], oq[NQ];
+#pragma unroll
+    for (int n = 0; n < NP; n++) op[n] = TP::offset(A.ldp, i0, A.I, tid + n * N);
+#pragma unroll
+    for (int n = 0; n < NQ; n++) oq[n] = TQ::offset(A.ldq, j0, A.J, tid + n * N);
+    const bool p_inside = TP::inside(i0, A.I), q_inside = TQ::inside(j0, A.J);
     auto fetch = [&](long long k0) {
+        const bool whole = k0 + KSTEP<T> <= k_end;
+        if (whole && p_inside) {
+            const char* at = TP::origin(P, A.ldp, i0, k0);
 #pragma unroll
-        for (int n = 0; n < NP; n++) rp[n] = TP::fetch(P, A.ldp, i0, A.I, k0, k_end, tid + n * N);
+            for (int n = 0; n < NP; n++) rp[n] = __builtin_bit_cast(u32x4, *(const PclipPack<T, TP::V>*)(at + op[n]));
+        } else {
 #pragma unroll
-        for (int n = 0; n < NQ; n++) rq[n] = TQ::fetch(Q, A.ldq, j0, A.J, k0, k_end, tid + n * N);
+            for (int n = 0; n < NP; n++) rp[n] = TP::fetch_edge(P, A.ldp, i0, A.I, k0, k_end, tid + n * N);
+        }
+        if (whole && q_inside) {
+            const char* at = TQ::origin(Q, A.ldq, j0, k0);
+#pragma unroll
+            for (int n = 0; n < NQ; n++) rq[n] = __builtin_bit_cast(u32x4, *(const PclipPack<T, TQ::V>*)(at + oq[n]));
+        } else {
+#pragma unroll
+            for (int n = 0; n < NQ; n++) rq[n] = TQ::fetch_edge(Q, A.ldq, j0, A.J, k0, k_end, tid + n * N);
+        }
     };
     f32x4 acc[FI][FJ], ones[FI];
 #pragma unroll
@@ -252,86 +300,114 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(const GemmArgs A) {
     }
 
     // a lane holds, of every 16 x 16 tile, row i = lane % 16 and the four columns from j = 4 * (lane / 16) on
+    if constexpr (EPI == EPI_SLAB) {
 #pragma unroll
-    for (int fi = 0; fi < FI; fi++) {
-        const int i = i0 + wi + fi * 16 + (lane & 15);
-        if (i >= A.I) continue;
+        for (int fi = 0; fi < FI; fi++) {
+            const int i = i0 + wi + fi * 16 + (lane & 15);
+            if (i >= A.I) continue;
 #pragma unroll
-        for (int fj = 0; fj < FJ; fj++) {
-            const int j = j0 + wj + fj * 16 + (lane >> 4) * 4, left = A.J - j;
-            if (left <= 0) continue;
-            float v[4];
+            for (int fj = 0; fj < FJ; fj++) {
+                const int j = j0 + wj + fj * 16 + (lane >> 4) * 4;
+                float v[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = acc[fi][fj][e];
+                for (int e = 0; e < 4; e++) v[e] = acc[fi][fj][e];
+                if (j < A.J) store_f32<float, 4>(A.slab + ((size_t)split * A.I + i) * A.J + j, A.J - j, v);
+            }
+            if (sum_rows && lane < 16) A.row_sum[(size_t)split * A.I + i] = ones[fi][0];
+        }
+    } else {
+        // 16 rows at a time through LDS (a wave's own part of it), after which a lane holds VW columns of one row in a run: rows
+        // are written, and residuals read, in whole 16-byte accesses
+        constexpr int WC = FJ * 16, PITCH = WC + 4, VW = WC / 4;
+        __syncthreads();
+        float* own = (float*)lds + wave * 16 * PITCH;
+        const int j = j0 + wj + (lane & 3) * VW, left = A.J - j;
+        float bias[VW];
+        if (EPI == EPI_FORWARD) {
+#pragma unroll
+            for (int e = 0; e < VW; e++) bias[e] = 0.f;
+            if (A.bias) load_run<T, VW>((const T*)A.bias + j, left, bias);
+        }
+#pragma unroll
+        for (int fi = 0; fi < FI; fi++) {
+#pragma unroll
+            for (int fj = 0; fj < FJ; fj++) *(f32x4*)(own + (lane & 15) * PITCH + fj * 16 + (lane >> 4) * 4) = acc[fi][fj];
+            float v[VW];
+#pragma unroll
+            for (int e = 0; e < VW; e += 4) *(f32x4*)(v + e) = *(const f32x4*)(own + (lane >> 2) * PITCH + (lane & 3) * VW + e);
+            const int i = i0 + wi + fi * 16 + (lane >> 2);
+            if (i >= A.I || left <= 0) continue;
             const size_t at = (size_t)i * A.J + j;
             if constexpr (EPI == EPI_FORWARD) {
-                if (A.bias) {
-                    float bias[4];
-                    load_f32<T, 4>((const T*)A.bias + j, left, bias);
+                float slope[VW];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] += bias[e];
-                }
-                float slope[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = activate<sizeof(T) == 4>(v[e], A.act, slope[e]);
-                if (A.slope) store_f32<T, 4>((T*)A.slope + at, left, slope);
+                for (int e = 0; e < VW; e++) v[e] = activate<sizeof(T) == 4>(v[e] + bias[e], A.act, slope[e]);
+                if (A.slope) store_slope<T, VW>((SlopeOf<T>*)A.slope + at, left, slope);
                 if (A.residual) {
-                    float res[4];
-                    load_f32<T, 4>((const T*)A.residual + at, left, res);
+                    float res[VW];
+                    load_run<T, VW>((const T*)A.residual + at, left, res);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] += res[e];
+                    for (int e = 0; e < VW; e++) v[e] += res[e];
                 }
-                store_f32<T, 4>((T*)A.out + at, left, v);
-            } else if constexpr (EPI == EPI_STORE) {
-                store_f32<T, 4>((T*)A.out + at, left, v);
-            } else {
-                store_f32<float, 4>(A.slab + (size_t)split * A.I * A.J + at, left, v);
             }
+            store_run<T, VW>((T*)A.out + at, left, v);
         }
-        if (sum_rows && lane < 16) A.row_sum[(size_t)split * A.I + i] = ones[fi][0];
     }
 }
 
-// out[e] = sum over the splits' slabs, in their order, rounded once; 64 x 4 elements and four parts of the splits a workgroup
+// out[e] = sum over the splits' slabs, in their order, rounded once; blocks behind those of the weight's gradient add the row
+// sums to the bias's.  16 lanes x 4 elements and 16 parts of the splits a workgroup.
+struct SlabSum {
+    const float* slab[2];
+    void* out[2];
+    long long n[2];
+    int splits, blocks;   // blocks: of the first sum
+};
 template <typename T>
-__global__ __launch_bounds__(256) void slab_sum_kernel(const float* __restrict__ slab, int splits, long long n, T* __restrict__ out) {
-    __shared__ float lds[3][64][4];
-    const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
-    const long long e = ((long long)blockIdx.x * 64 + lane) * 4;
-    const long long left = n - e;
+__global__ __launch_bounds__(256) void slab_sum_kernel(const SlabSum A) {
+    __shared__ float lds[16][16][4];
+    const int lane = threadIdx.x & 15, part = threadIdx.x >> 4, which = (int)blockIdx.x >= A.blocks;
+    const long long n = A.n[which], e = (((long long)blockIdx.x - (which ? A.blocks : 0)) * 16 + lane) * 4, left = n - e;
     const int valid = left < 4 ? (int)left : 4;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
     if (valid > 0)
 #pragma unroll 4
-        for (int k = part; k < splits; k += 4) {
+        for (int k = part; k < A.splits; k += 16) {
             float v[4];
-            load_f32<float, 4>(slab + (size_t)k * n + e, valid, v);
+            load_f32<float, 4>(A.slab[which] + (size_t)k * n + e, valid, v);
 #pragma unroll
             for (int c = 0; c < 4; c++) s[c] += v[c];
         }
-    if (part)
 #pragma unroll
-        for (int c = 0; c < 4; c++) lds[part - 1][lane][c] = s[c];
+    for (int c = 0; c < 4; c++) lds[part][lane][c] = s[c];
     __syncthreads();
     if (part == 0 && valid > 0) {
 #pragma unroll
-        for (int c = 0; c < 4; c++) s[c] += (lds[0][lane][c] + lds[1][lane][c]) + lds[2][lane][c];
-        store_f32<T, 4>(out + e, valid, s);
+        for (int p = 1; p < 16; p++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) s[c] += lds[p][lane][c];
+        store_f32<T, 4>((T*)A.out[which] + e, valid, s);
     }
 }
 
 // dz = dy * slope, or dy where the output is positive
 template <typename T>
-__global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, const T* __restrict__ saved, int is_output, long long n, T* __restrict__ dz) {
+__global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, const void* __restrict__ saved, int is_output, long long n, T* __restrict__ dz) {
     constexpr int V = PclipVec<T>::N;
     for (long long e = ((long long)blockIdx.x * 256 + threadIdx.x) * V; e < n; e += (long long)gridDim.x * 256 * V) {
         const long long left = n - e;
         const int valid = left < V ? (int)left : V;
         float d[V], s[V];
         load_f32<T, V>(dy + e, valid, d);
-        load_f32<T, V>(saved + e, valid, s);
+        if (is_output) {
+            load_f32<T, V>((const T*)saved + e, valid, s);
 #pragma unroll
-        for (int i = 0; i < V; i++) d[i] = is_output ? (s[i] > 0.f ? d[i] : 0.f) : d[i] * s[i];
+            for (int i = 0; i < V; i++) d[i] = s[i] > 0.f ? d[i] : 0.f;
+        } else {
+            load_f32<SlopeOf<T>, V>((const SlopeOf<T>*)saved + e, valid, s);
+#pragma unroll
+            for (int i = 0; i < V; i++) d[i] *= s[i] * SLOPE_UNIT<T>;
+        }
         store_f32<T, V>(dz + e, valid, d);
     }
 }
@@ -365,7 +441,7 @@ struct RowPlan { int tile, splits; long long k_split; };
 RowPlan row_plan(int M, int K, int N, int dtype) {
     const int step = dtype == PCLIP_DT_F32 ? 32 : 64, tile = K > 64 && N > 64 ? 128 : 64;
     const long long t = tiles(N, K, tile, tile), steps = ((long long)M + step - 1) / step;
-    long long s = (512 + t - 1) / t;
+    long long s = (256 + t - 1) / t;
     if (s > (steps + 3) / 4) s = (steps + 3) / 4;   // four steps a workgroup at least
     if (s < 1) s = 1;
     const long long per = (steps + s - 1) / s;
@@ -376,7 +452,7 @@ template <typename T>
 int forward(const GemmArgs& A, hipStream_t st) { return launch_rows<T, true, true, EPI_FORWARD>(A, st); }
 
 template <typename T>
-int backward(const T* x, const T* w, const T* dy, const T* saved, int is_output, int M, int K, int N, int dtype, int act, T* dx, T* dw, T* db, char* ws,
+int backward(const T* x, const T* w, const T* dy, const void* saved, int is_output, int M, int K, int N, int dtype, int act, T* dx, T* dw, T* db, char* ws,
              hipStream_t st) {
     const T* dz = dy;
     if (act != PCLIP_ACT_NONE) {
@@ -400,8 +476,8 @@ int backward(const T* x, const T* w, const T* dy, const T* saved, int is_output,
         const int rc = p.tile == 128 ? launch_tile<T, 128, 128, 2, 2, false, false, EPI_SLAB>(A, st) : launch_tile<T, 64, 64, 2, 2, false, false, EPI_SLAB>(A, st);
         if (rc) return rc;
         const long long n = (long long)N * K;
-        if (dw) slab_sum_kernel<T><<<(int)((n + 255) / 256), 256, 0, st>>>(A.slab, p.splits, n, dw);
-        if (db) slab_sum_kernel<T><<<(N + 255) / 256, 256, 0, st>>>(A.row_sum, p.splits, N, db);
+        SlabSum S = {{A.slab, A.row_sum}, {dw, db}, {n, N}, p.splits, dw ? (int)((n + 63) / 64) : 0};
+        slab_sum_kernel<T><<<S.blocks + (db ? (N + 63) / 64 : 0), 256, 0, st>>>(S);
     }
     return PCLIP_OK;
 }
@@ -450,7 +526,7 @@ extern "C" int pclip_linear_bwd(const void* x, const void* w, const void* dy, co
     PCLIP_REQUIRE(ws_bytes >= need, "linear_bwd: workspace too small (%zu bytes, need %zu)", ws_bytes, need);
     PCLIP_REQUIRE(((uintptr_t)ws & 15) == 0, "linear_bwd: the workspace must be 16-byte aligned");
     hipStream_t st = (hipStream_t)stream;
-#define PCLIP_LINEAR_BWD(T)                                                                                                                         backward<T>((const T*)x, (const T*)w, (const T*)dy, (const T*)saved, saved_is_output, M, K, N, dtype, activation, (T*)dx, (T*)dw, (T*)db, (char*)ws, st)
+#define PCLIP_LINEAR_BWD(T)                                                                                                                         backward<T>((const T*)x, (const T*)w, (const T*)dy, saved, saved_is_output, M, K, N, dtype, activation, (T*)dx, (T*)dw, (T*)db, (char*)ws, st)
     if (dtype == PCLIP_DT_F32) rc = PCLIP_LINEAR_BWD(float);
     else if (dtype == PCLIP_DT_BF16) rc = PCLIP_LINEAR_BWD(__bf16);
     else rc = PCLIP_LINEAR_BWD(_Float16);

@@ -2,12 +2,12 @@
 workspace allocation through torch, one C call each.  No arithmetic happens here."""
 from __future__ import annotations
 
-import bisect
 import collections
 import ctypes
 import threading
 from typing import Optional, Tuple
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -257,6 +257,10 @@ def _linear_sizes(x, w):
     return M, K, N, code
 
 
+def _slope_type(dtype):
+    return F32 if dtype == F32 else torch.int16   # steps of 1 / 28672
+
+
 def linear_fwd(x, w, bias=None, residual=None, activation: str = "none", want_slope: bool = False):
     """``act(x @ w.T + bias) + residual`` for x [M,K], w [N,K], bias [N], residual [M,N] of one type.
     Returns (y [M,N], slope): slope = act'(z) [M,N] when asked for (what :func:`linear_bwd` needs), else None."""
@@ -264,7 +268,7 @@ def linear_fwd(x, w, bias=None, residual=None, activation: str = "none", want_sl
     dev = x.device
     b, r = _operand(bias, "bias", (N,), x.dtype, dev), _operand(residual, "residual", (M, N), x.dtype, dev)
     y = _empty((M, N), x.dtype, dev)
-    slope = _empty((M, N), x.dtype, dev) if want_slope else None
+    slope = _empty((M, N), _slope_type(x.dtype), dev) if want_slope else None
     with _on(dev):
         check(_lib.load().pclip_linear_fwd(x.data_ptr(), w.data_ptr(), b, r, M, K, N, code, ACTIVATIONS[activation], y.data_ptr(),
                                            slope.data_ptr() if want_slope else None, stream_of(x)), "pclip_linear_fwd")
@@ -277,7 +281,8 @@ def linear_bwd(x, w, dy, saved=None, saved_is_output: bool = False, activation: 
     ``saved_is_output`` (relu without a residual), None for activation "none"."""
     M, K, N, code = _linear_sizes(x, w)
     dev, act = x.device, ACTIVATIONS[activation]
-    g, s = _operand(dy, "dy", (M, N), x.dtype, dev), _operand(saved, "saved", (M, N), x.dtype, dev)
+    g = _operand(dy, "dy", (M, N), x.dtype, dev)
+    s = _operand(saved, "saved", (M, N), x.dtype if saved_is_output else _slope_type(x.dtype), dev)
     lib = _lib.load()
     dx = _empty((M, K), x.dtype, dev) if want_dx else None
     dw = _empty((N, K), x.dtype, dev) if want_dw else None
@@ -362,56 +367,67 @@ def _dense(t) -> bool:
     return True
 
 
+def _spans(tensors):
+    """(first byte, byte behind the last, element count, type code) of each tensor, as arrays."""
+    n = len(tensors)
+    start = np.fromiter(map(torch.Tensor.data_ptr, tensors), np.int64, n)
+    count = np.fromiter(map(torch.Tensor.numel, tensors), np.int64, n)
+    code = np.fromiter((DTYPES.get(t.dtype, -1) for t in tensors), np.int32, n)
+    return start, start + count * np.where(code == 0, 4, 2), count, code
+
+
 def _check_disjoint(src, dst):
     """No destination may share memory with another tensor of the call (its own source excepted): workgroups of
     different tensors run side by side."""
-    spans = sorted((d.data_ptr(), d.data_ptr() + d.numel() * d.element_size()) for d in dst if d.numel())
-    for (_, end), (start, _) in zip(spans, spans[1:]):
-        if start < end:
-            raise _lib.PclipError("grad_clip: two of the written tensors share memory (the same gradient twice?)")
-    starts = [s for s, _ in spans]
-    for s, d in zip(src, dst):
-        p = s.data_ptr()
-        if p == d.data_ptr() or not s.numel():
-            continue
-        k = bisect.bisect_left(starts, p + s.numel() * s.element_size()) - 1   # the last span that begins before s ends
-        if k >= 0 and spans[k][1] > p:
+    (s0, s1, count, _), (d0, d1, _, _) = src, dst
+    order = np.argsort(d0[count > 0], kind="stable")
+    first, last = d0[count > 0][order], d1[count > 0][order]
+    if (last[:-1] > first[1:]).any():
+        raise _lib.PclipError("grad_clip: two of the written tensors share memory (the same gradient twice?)")
+    other = (count > 0) & (s0 != d0)
+    if other.any():
+        k = np.searchsorted(first, s1[other]) - 1   # the last destination that begins before the source ends
+        if ((k >= 0) & (last[k] > s0[other])).any():
             raise _lib.PclipError("grad_clip: a written tensor shares memory with another tensor that is read")
+
+
+def _c_array(a, kind):
+    return a.ctypes.data_as(ctypes.POINTER(kind))
 
 
 def grad_clip(src, dst=None, max_norm: float = 0.0, eps: float = 1e-6) -> torch.Tensor:
     """Norm [1] of all elements of the tensors ``src``; with ``dst`` (tensors of the same shapes; ``src`` itself: in place)
     also ``dst = src * min(1, max_norm / (norm + eps))``.  One launch a pass for every 120 tensors."""
+    in_place = dst is src
     src = list(src)
-    if not src:
+    n = len(src)
+    if not n:
         raise _lib.PclipError("grad_clip: no tensors")
-    n, dev = len(src), src[0].device
+    dev = src[0].device
     for i, t in enumerate(src):
         if t.dtype not in DTYPES or t.device != dev or not t.is_cuda or t.layout != torch.strided:
             raise _lib.PclipError(f"grad_clip: tensor {i}: expected a dense float32, bfloat16 or float16 GPU tensor on {dev}, got {t.dtype} on {t.device}")
-        if not _dense(t):
+        if not t.is_contiguous() and not _dense(t):
             raise _lib.PclipError(f"grad_clip: tensor {i} has gaps or shared elements (strides {t.stride()} of shape {tuple(t.shape)})")
-    out, out_types = None, None
+    read = write = _spans(src)
     if dst is not None:
-        dst = list(dst)
-        if len(dst) != n:
-            raise _lib.PclipError(f"grad_clip: {len(dst)} destinations for {n} tensors")
-        for i, (s, d) in enumerate(zip(src, dst)):
-            if d is s:
-                continue
-            if d.dtype not in DTYPES or d.device != dev or d.shape != s.shape or d.layout != torch.strided or (d.stride() != s.stride() and not (
-                    d.is_contiguous() and s.is_contiguous())):
-                raise _lib.PclipError(f"grad_clip: destination {i} must have the shape, layout and device of its tensor and a supported type")
-        _check_disjoint(src, dst)
-        out = (ctypes.c_void_p * n)(*[d.data_ptr() for d in dst])
-        out_types = (ctypes.c_int * n)(*[DTYPES[d.dtype] for d in dst])
+        if not in_place:
+            dst = list(dst)
+            if len(dst) != n:
+                raise _lib.PclipError(f"grad_clip: {len(dst)} destinations for {n} tensors")
+            for i, (s, d) in enumerate(zip(src, dst)):
+                if d.dtype not in DTYPES or d.device != dev or d.shape != s.shape or d.layout != torch.strided or not (
+                        d.is_contiguous() and s.is_contiguous() or d.stride() == s.stride()):
+                    raise _lib.PclipError(f"grad_clip: destination {i} must have the shape, layout and device of its tensor and a supported type")
+            write = _spans(dst)
+        _check_disjoint(read, write)
     lib = _lib.load()
     norm = _empty((1,), F32, dev)
     ws = _empty((lib.pclip_grad_clip_workspace_bytes(n),), torch.uint8, dev)   # the call's own, see linear_bwd
+    out = (_c_array(write[0], ctypes.c_void_p), _c_array(write[3], ctypes.c_int)) if dst is not None else (None, None)
     with _on(dev):
-        check(lib.pclip_grad_clip((ctypes.c_void_p * n)(*[t.data_ptr() for t in src]), (ctypes.c_int64 * n)(*[t.numel() for t in src]),
-                                  (ctypes.c_int * n)(*[DTYPES[t.dtype] for t in src]), out, out_types, n, max_norm, eps, norm.data_ptr(), ws.data_ptr(),
-                                  ws.numel(), stream_of(norm)), "pclip_grad_clip")
+        check(lib.pclip_grad_clip(_c_array(read[0], ctypes.c_void_p), _c_array(read[2], ctypes.c_int64), _c_array(read[3], ctypes.c_int), *out, n, max_norm,
+                                  eps, norm.data_ptr(), ws.data_ptr(), ws.numel(), stream_of(norm)), "pclip_grad_clip")
     return norm
 
 

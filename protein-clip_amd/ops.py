@@ -137,15 +137,19 @@ def embedding_head(pooled: torch.Tensor, params, temperature: torch.Tensor, keep
 # --------------------------------------------------------------------------------------
 # token head: linear layers, norms around a block   (modules/models.py:54-73)
 # --------------------------------------------------------------------------------------
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """[..., d] -> contiguous [rows, d]."""
+    t = t.contiguous()
+    return t if t.dim() == 2 else t.view(math.prod(t.shape[:-1]), t.shape[-1])
+
+
 class _LinearAct(torch.autograd.Function):
+    # operands keep their leading dimensions here: views made outside would be nodes of the graph
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, K):
         product = any(ctx.needs_input_grad[:3])
         output = activation == "relu" and residual is None   # the sign of y says where the slope is one
-        if x.shape[0] == 0:
-            y, slope = x.new_empty(0, weight.shape[0]), None
-        else:
-            y, slope = K.linear_fwd(x, weight, bias, residual, activation, want_slope=product and activation != "none" and not output)
+        y, slope = _linear_rows(x, weight, bias, residual, activation, product and activation != "none" and not output, K)
         ctx.K, ctx.activation, ctx.output = K, activation, output
         ctx.save_for_backward(x, weight, y if output and product else slope)
         return y
@@ -156,11 +160,23 @@ class _LinearAct(torch.autograd.Function):
         x, weight, saved = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         dx = dw = db = None
-        if x.shape[0] == 0:
+        if x.numel() == 0:
             dx, dw, db = torch.zeros_like(x), torch.zeros_like(weight), weight.new_zeros(weight.shape[0])
         elif need_x or need_w or need_b:
-            dx, dw, db = ctx.K.linear_bwd(x, weight, dy.contiguous(), saved, ctx.output, ctx.activation, need_x, need_w, need_b)
+            dx, dw, db = ctx.K.linear_bwd(_rows(x), weight.contiguous(), _rows(dy), None if saved is None else _rows(saved), ctx.output, ctx.activation,
+                                          need_x, need_w, need_b)
+            if need_x:
+                dx = dx.view(x.shape)
         return dx if need_x else None, dw if need_w else None, db if need_b else None, dy if need_r else None, None, None
+
+
+def _linear_rows(x, weight, bias, residual, activation, want_slope, K):
+    shape = x.shape[:-1] + weight.shape[:1]
+    if x.numel() == 0:
+        return x.new_empty(shape), None
+    y, slope = K.linear_fwd(_rows(x), weight.contiguous(), None if bias is None else bias.contiguous(), None if residual is None else _rows(residual),
+                            activation, want_slope)
+    return (y, slope) if x.dim() == 2 else (y.view(shape), slope)
 
 
 def _wants_grad(*tensors) -> bool:
@@ -177,34 +193,31 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     ``activation``: "none", "relu", "gelu" (with erf) or "silu".  First derivatives only."""
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"linear_act: x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
-    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+    if weight.numel() == 0:
+        raise ValueError("linear_act: the layer has no input or no output")
+    if bias is not None and bias.shape != weight.shape[:1]:
         raise ValueError(f"linear_act: bias must have shape ({weight.shape[0]},), got {tuple(bias.shape)}")
     if activation not in _hip_kernels.ACTIVATIONS:
         raise ValueError(f"linear_act: unknown activation {activation!r}")
     K = kernels or _hip_kernels
-    shape = x.shape[:-1] + (weight.shape[0],)
-    x2 = x.reshape(-1, x.shape[-1]) if x.numel() else x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
-    x2 = x2.contiguous()
-    weight = weight.to(x.dtype).contiguous()
+    weight = weight.to(x.dtype)
     if bias is not None:
-        bias = bias.to(x.dtype).contiguous()
+        bias = bias.to(x.dtype)
     if residual is not None:
-        residual = residual.to(x.dtype).expand(shape).reshape(x2.shape[0], weight.shape[0]).contiguous()
-    if x2.shape[0] == 0 or _wants_grad(x2, weight, bias, residual):
-        y = _LinearAct.apply(x2, weight, bias, residual, activation, K)
-    else:
-        y, _ = K.linear_fwd(x2, weight, bias, residual, activation)
-    return y.reshape(shape)
+        shape = x.shape[:-1] + weight.shape[:1]
+        residual = residual.to(x.dtype)
+        if residual.shape != shape:
+            residual = residual.expand(shape)
+    if _wants_grad(x, weight, bias, residual):
+        return _LinearAct.apply(x, weight, bias, residual, activation, K)
+    return _linear_rows(x, weight, bias, residual, activation, False, K)[0]
 
 
 class _NormGate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, u, r, gate, wa, ba, wb, bb, gate_rows, scale, after, before, eps, K):
         ctx.set_materialize_grads(False)
-        if u.shape[0] == 0:
-            y, n, stats = torch.empty_like(u), torch.empty_like(u) if before else None, None
-        else:
-            y, n, stats = K.norm_gate_fwd(u, r, gate, gate_rows, scale, after, wa, ba, before, wb, bb, eps, want_stats=True)
+        y, n, stats = _norm_rows(u, r, gate, wa, ba, wb, bb, gate_rows, scale, after, before, eps, True, K)
         ctx.K, ctx.cfg = K, (gate_rows, scale, after, before, eps)
         ctx.save_for_backward(u, r, gate, wa, ba, wb, bb, stats)
         return (y, n) if before else y
@@ -217,26 +230,41 @@ class _NormGate(torch.autograd.Function):
         need = ctx.needs_input_grad[:7]
         if dy is None and dn is None:
             return (None,) * 13
-        if u.shape[0] == 0:
+        if u.numel() == 0:
             return tuple(torch.zeros_like(t) if w else None for t, w in zip((u, r, gate, wa, ba, wb, bb), need)) + (None,) * 6
-        dy = None if dy is None else dy.contiguous()
-        dn = None if dn is None else dn.contiguous()
-        grads = ctx.K.norm_gate_bwd(u, r, gate, gate_rows, scale, after, wa, ba, before, wb, bb, eps, stats, dy, dn, want=need)
-        return tuple(grads) + (None,) * 6
+        rows = lambda t: None if t is None else _rows(t)
+        flat = lambda t: None if t is None else t.contiguous()
+        grads = ctx.K.norm_gate_bwd(_rows(u), rows(r), _gate2(gate, u.shape[-1]), gate_rows, scale, after, flat(wa), flat(ba), before, flat(wb), flat(bb),
+                                    eps, stats, rows(dy), rows(dn), want=need)
+        du, dr, dg = (None if g is None else g.view(t.shape) for g, t in zip(grads[:3], (u, r, gate)))
+        return (du, dr, dg) + tuple(grads[3:]) + (None,) * 6
 
 
-def _gate_rows(gate: torch.Tensor, lead, d: int):
-    """(gate as [groups, d], rows of the operand that share a row of it), or None when its shape is no such pattern: its
-    leading dimensions must be the operand's first ones followed by ones."""
-    if gate.shape[-1] != d:
-        return None
+def _gate2(gate, d: int):
+    return None if gate is None else gate.contiguous().view(-1, d)
+
+
+def _norm_rows(u, r, gate, wa, ba, wb, bb, gate_rows, scale, after, before, eps, want_stats, K):
+    if u.numel() == 0:
+        return torch.empty_like(u), torch.empty_like(u) if before else None, None
+    flat = lambda t: None if t is None else t.contiguous()
+    y, n, stats = K.norm_gate_fwd(_rows(u), None if r is None else _rows(r), _gate2(gate, u.shape[-1]), gate_rows, scale, after, flat(wa), flat(ba), before,
+                                  flat(wb), flat(bb), eps, want_stats)
+    if u.dim() != 2:
+        y, n = y.view(u.shape), n.view(u.shape) if before else None
+    return y, n, stats
+
+
+def _gate_rows(gate: torch.Tensor, lead, d: int) -> int:
+    """Rows of the operand that share a row of the gate, or 0 when its shape is no such pattern: the gate's leading
+    dimensions must be the operand's first ones followed by ones."""
+    if gate.dim() == 0 or gate.shape[-1] != d:
+        return 0
     dims = (1,) * (len(lead) + 1 - gate.dim()) + tuple(gate.shape[:-1])
     j = 0
     while j < len(lead) and dims[j] == lead[j]:
         j += 1
-    if any(s != 1 for s in dims[j:]):
-        return None
-    return gate.reshape(-1, d), math.prod(lead[j:])
+    return 0 if any(s != 1 for s in dims[j:]) else math.prod(lead[j:])
 
 
 def norm_gate_residual(u: torch.Tensor, residual: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, scale: float = 1.0,
@@ -250,47 +278,44 @@ def norm_gate_residual(u: torch.Tensor, residual: Optional[torch.Tensor] = None,
     ``gate``: a tensor broadcastable to ``u`` (a channel's, a sequence's, an element's; with a gradient) or a bool / uint8
     dropout mask of ``u``'s shape, used with ``scale = 1 / (1 - p)``.
     Returns ``y``, or ``(y, norm(y))`` when ``before`` is given.  First derivatives only."""
-    if u.dim() < 1 or norm not in ("layer", "rms"):
+    if u.dim() < 1 or u.shape[-1] == 0 or norm not in ("layer", "rms"):
         raise ValueError("norm_gate_residual: expected u [..., d] and norm 'layer' or 'rms'")
     if isinstance(scale, torch.Tensor):
         raise ValueError("norm_gate_residual: scale is a number (a learned scale is a gate)")
     K = kernels or _hip_kernels
-    d, lead = u.shape[-1], tuple(u.shape[:-1])
-    rows = math.prod(lead)
-    u2 = u.reshape(rows, d).contiguous()
+    d = u.shape[-1]
     wa, ba = (None, None) if after is None else after
     wb, bb = (None, None) if before is None else before
-    params = [wa, ba, wb, bb]
-    for p in params:
-        if p is not None and tuple(p.shape) != (d,):
-            raise ValueError(f"norm_gate_residual: affine parameters must have shape ({d},), got {tuple(p.shape)}")
-    types = {p.dtype for p in params if p is not None}
-    if types and types not in ({torch.float32}, {u.dtype}):
-        params = [None if p is None else p.float() for p in params]
-    params = [None if p is None else p.contiguous() for p in params]
+    types = set()
+    for p in (wa, ba, wb, bb):
+        if p is not None:
+            if tuple(p.shape) != (d,):
+                raise ValueError(f"norm_gate_residual: affine parameters must have shape ({d},), got {tuple(p.shape)}")
+            types.add(p.dtype)
+    if types and types != {torch.float32} and types != {u.dtype}:
+        wa, ba, wb, bb = (None if p is None else p.float() for p in (wa, ba, wb, bb))
     gate_rows = 1
     if gate is not None:
+        if gate.dim() > u.dim():
+            raise ValueError(f"norm_gate_residual: gate {tuple(gate.shape)} does not broadcast to u {tuple(u.shape)}")
         if gate.dtype == torch.bool:
-            gate = gate.to(torch.uint8)
+            gate = gate.view(torch.uint8)
         if gate.dtype == torch.uint8:
-            gate = gate.expand(u.shape).reshape(rows, d).contiguous()
+            gate = gate.expand(u.shape)
         else:
-            if gate.dim() > u.dim():
-                raise ValueError(f"norm_gate_residual: gate {tuple(gate.shape)} does not broadcast to u {tuple(u.shape)}")
             gate = gate.to(u.dtype)
-            found = _gate_rows(gate, lead, d) if gate.dim() and rows else None
-            if found is None:   # any other broadcast is written out
-                found = gate.expand(u.shape).reshape(rows, d), 1
-            gate, gate_rows = found[0].contiguous(), found[1]
+            gate_rows = _gate_rows(gate, tuple(u.shape[:-1]), d)
+            if not gate_rows:   # any other broadcast is written out (also when there are no rows)
+                gate, gate_rows = gate.expand(u.shape), 1
     if residual is not None:
-        residual = residual.to(u.dtype).expand(u.shape).reshape(rows, d).contiguous()
-    kinds = [norm if pair is not None else None for pair in (after, before)]
-    if rows == 0 or _wants_grad(u2, residual, gate, *params):
-        out = _NormGate.apply(u2, residual, gate, *params, gate_rows, float(scale), kinds[0], kinds[1], float(eps), K)
-    else:
-        y, n, _ = K.norm_gate_fwd(u2, residual, gate, gate_rows, float(scale), kinds[0], params[0], params[1], kinds[1], params[2], params[3], float(eps))
-        out = (y, n) if kinds[1] else y
-    return tuple(o.reshape(u.shape) for o in out) if kinds[1] else out.reshape(u.shape)
+        residual = residual.to(u.dtype)
+        if residual.shape != u.shape:
+            residual = residual.expand(u.shape)
+    first, second = norm if after is not None else None, norm if before is not None else None
+    if _wants_grad(u, residual, gate, wa, ba, wb, bb):
+        return _NormGate.apply(u, residual, gate, wa, ba, wb, bb, gate_rows, float(scale), first, second, float(eps), K)
+    y, n, _ = _norm_rows(u, residual, gate, wa, ba, wb, bb, gate_rows, float(scale), first, second, float(eps), False, K)
+    return (y, n) if second else y
 
 
 # --------------------------------------------------------------------------------------
