@@ -44,6 +44,15 @@ template <> struct Mfma<float> {
 // off each other's banks.
 template <typename T> constexpr int KSTEP = 128 / (int)sizeof(T);   // k values of a tile
 
+constexpr unsigned DIRECT_RANGE = 1u << 30;   // bytes that a buffer descriptor reaches: more than a tile spans (256 rows of 65536 f32)
+// 16 bytes a lane from base + offset to lds + 16 * lane; zeros from DIRECT_RANGE on.  base and lds are the same for the wave.
+__device__ __forceinline__ void load_direct(const void* base, unsigned offset, char* lds) {
+#ifdef __HIP_DEVICE_COMPILE__   // the host pass has no descriptor type
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, DIRECT_RANGE, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)lds, 16, offset, 0, 0, 0);
+#endif
+}
+
 template <typename T, int ROWS, bool ALONG_K>
 struct Tile {
     static constexpr int V = PclipVec<T>::N;
@@ -119,6 +128,12 @@ struct Tile {
     static __device__ __forceinline__ const char* origin(const T* p, int ld, int i0, long long k0) {
         return (const char*)(ALONG_K ? p + (long long)i0 * ld + k0 : p + k0 * ld + i0);
     }
+    // Straight to LDS, 16 bytes a lane in the order of the lanes: place c of the tile takes the chunk that slot() puts there.
+    static __device__ __forceinline__ int direct_k(int c) { return ALONG_K ? ((c & 7) ^ ((c >> 3) & 7)) * V : c / ICH; }
+    static __device__ __forceinline__ unsigned direct_offset(int ld, int i0, int rows, int c) {
+        const int k = direct_k(c), row = ALONG_K ? c >> 3 : ((c % ICH) ^ swizzle_i(c / ICH)) * V;
+        return i0 + row < rows ? (unsigned)(ALONG_K ? row * ld + k : k * ld + row) * (unsigned)sizeof(T) : DIRECT_RANGE;
+    }
     static __device__ __forceinline__ bool inside(int i0, int rows) { return ALONG_K || i0 + ROWS <= rows; }
 };
 
@@ -128,13 +143,13 @@ struct Tile {
 // squares over 0 <= a <= 13: 1.9e-6 relative error, a hundredth of an f16 half step, in one exp and one reciprocal,
 // which the slope's density shares.  Far arguments are cut at 40 where only their product with a vanished density
 // enters, so an infinite z has the limit's slope.
-template <bool EXACT>
-__device__ __forceinline__ float activate(float z, int act, float& slope) {
-    if (act == PCLIP_ACT_RELU) {
+template <bool EXACT, int ACT>
+__device__ __forceinline__ float activate(float z, float& slope) {
+    if constexpr (ACT == PCLIP_ACT_RELU) {
         slope = z > 0.f ? 1.f : 0.f;
         return z > 0.f ? z : (z != z ? z : 0.f);   // NaN stays
     }
-    if (act == PCLIP_ACT_GELU) {
+    if constexpr (ACT == PCLIP_ACT_GELU) {
         const float c = fminf(fmaxf(z, -40.f), 40.f);
         float phi, density;
         if constexpr (EXACT) {
@@ -156,7 +171,7 @@ __device__ __forceinline__ float activate(float z, int act, float& slope) {
         slope = fmaf(c * 0.39894228040143268f, density, phi);
         return z * phi;
     }
-    if (act == PCLIP_ACT_SILU) {
+    if constexpr (ACT == PCLIP_ACT_SILU) {
         float s;
         if constexpr (EXACT) s = 1.f / (1.f + expf(-z));
         else s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
@@ -166,6 +181,13 @@ __device__ __forceinline__ float activate(float z, int act, float& slope) {
     }
     slope = 1.f;
     return z;
+}
+
+// the activation is chosen once for a run of values, so that their chains of dependent instructions interleave
+template <bool EXACT, int ACT, int VW>
+__device__ __forceinline__ void activate_run(float (&v)[VW], const float (&bias)[VW], float (&slope)[VW]) {
+#pragma unroll
+    for (int e = 0; e < VW; e++) v[e] = activate<EXACT, ACT>(v[e] + bias[e], slope[e]);
 }
 
 // The slope is kept for the backward: as it is for f32, for 16-bit types as a whole number of steps of 1 / 28672 (slopes lie
@@ -211,6 +233,69 @@ struct GemmArgs {
 __device__ __forceinline__ int xcd_order(int b, int n) {
     const int xcd = b & 7, q = n >> 3, r = n & 7;
     return xcd * q + min(xcd, r) + (b >> 3);
+}
+
+// What a wave does with its accumulators: rows from i0, columns from j0 on.
+template <typename T, int FI, int FJ, int EPI>
+__device__ __forceinline__ void finish(const GemmArgs& A, f32x4 (&acc)[FI][FJ], f32x4 (&ones)[FI], bool sum_rows, char* lds, int i0, int j0, int split) {
+    const int lane = threadIdx.x & 63;
+    // a lane holds, of every 16 x 16 tile, row i = lane % 16 and the four columns from j = 4 * (lane / 16) on
+    if constexpr (EPI == EPI_SLAB) {
+#pragma unroll
+        for (int fi = 0; fi < FI; fi++) {
+            const int i = i0 + fi * 16 + (lane & 15);
+            if (i >= A.I) continue;
+#pragma unroll
+            for (int fj = 0; fj < FJ; fj++) {
+                const int j = j0 + fj * 16 + (lane >> 4) * 4;
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = acc[fi][fj][e];
+                if (j < A.J) store_f32<float, 4>(A.slab + ((size_t)split * A.I + i) * A.J + j, A.J - j, v);
+            }
+            if (sum_rows && lane < 16) A.row_sum[(size_t)split * A.I + i] = ones[fi][0];
+        }
+    } else {
+        // 16 rows at a time through LDS (a wave's own part of it), after which a lane holds VW columns of one row in a run: rows
+        // are written, and residuals read, in whole 16-byte accesses
+        constexpr int WC = FJ * 16, PITCH = WC + 4, VW = WC / 4;
+        __syncthreads();
+        float* own = (float*)lds + (threadIdx.x >> 6) * 16 * PITCH;
+        const int j = j0 + (lane & 3) * VW, left = A.J - j;
+        float bias[VW];
+        if (EPI == EPI_FORWARD) {
+#pragma unroll
+            for (int e = 0; e < VW; e++) bias[e] = 0.f;
+            if (A.bias) load_run<T, VW>((const T*)A.bias + j, left, bias);
+        }
+#pragma unroll
+        for (int fi = 0; fi < FI; fi++) {
+#pragma unroll
+            for (int fj = 0; fj < FJ; fj++) *(f32x4*)(own + (lane & 15) * PITCH + fj * 16 + (lane >> 4) * 4) = acc[fi][fj];
+            float v[VW];
+#pragma unroll
+            for (int e = 0; e < VW; e += 4) *(f32x4*)(v + e) = *(const f32x4*)(own + (lane >> 2) * PITCH + (lane & 3) * VW + e);
+            const int i = i0 + fi * 16 + (lane >> 2);
+            if (i >= A.I || left <= 0) continue;
+            const size_t at = (size_t)i * A.J + j;
+            if constexpr (EPI == EPI_FORWARD) {
+                float slope[VW];
+                constexpr bool EXACT = sizeof(T) == 4;
+                if (A.act == PCLIP_ACT_NONE) activate_run<EXACT, PCLIP_ACT_NONE>(v, bias, slope);
+                else if (A.act == PCLIP_ACT_RELU) activate_run<EXACT, PCLIP_ACT_RELU>(v, bias, slope);
+                else if (A.act == PCLIP_ACT_GELU) activate_run<EXACT, PCLIP_ACT_GELU>(v, bias, slope);
+                else activate_run<EXACT, PCLIP_ACT_SILU>(v, bias, slope);
+                if (A.slope) store_slope<T, VW>((SlopeOf<T>*)A.slope + at, left, slope);
+                if (A.residual) {
+                    float res[VW];
+                    load_run<T, VW>((const T*)A.residual + at, left, res);
+#pragma unroll
+                    for (int e = 0; e < VW; e++) v[e] += res[e];
+                }
+            }
+            store_run<T, VW>((T*)A.out + at, left, v);
+        }
+    }
 }
 
 template <typename T, int BI, int BJ, int WI, int WJ, bool PK, bool QK, int EPI>
@@ -299,60 +384,90 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_kernel(const GemmArgs A)
         buf ^= 1;
     }
 
-    // a lane holds, of every 16 x 16 tile, row i = lane % 16 and the four columns from j = 4 * (lane / 16) on
-    if constexpr (EPI == EPI_SLAB) {
+    finish<T, FI, FJ, EPI>(A, acc, ones, sum_rows, lds, i0 + wi, j0 + wj, split);
+}
+
+// The same product for operands whose rows begin at multiples of 16 bytes: tiles go from memory to LDS directly.  One buffer of
+// LDS is enough, because a wave takes all its fragments of a step into registers first; the next tile is on its way while
+// the matrix cores work, and two workgroups share a compute unit.  Chunks outside the matrix are read at an offset
+// beyond the descriptor's range, which writes zeros.
+template <typename T, int BI, int BJ, int WI, int WJ, bool PK, bool QK, int EPI>
+__global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_direct_kernel(const GemmArgs A) {
+    typedef Tile<T, BI, PK> TP;
+    typedef Tile<T, BJ, QK> TQ;
+    typedef typename Mfma<T>::Frag Frag;
+    constexpr int N = 64 * WI * WJ, NP = TP::CHUNKS / N, NQ = TQ::CHUNKS / N;
+    constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int b = xcd_order(blockIdx.x, gridDim.x);
+    const int tj = b % A.tiles_j;
+    b /= A.tiles_j;
+    const int ti = b % A.tiles_i, split = b / A.tiles_i;
+    const int i0 = ti * BI, j0 = tj * BJ;
+    const int wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
+    const long long k_first = split * A.k_split, k_end = k_first + A.k_split < A.K ? k_first + A.k_split : A.K;
+    const T *P = (const T*)A.P, *Q = (const T*)A.Q;
+
+    unsigned op[NP], oq[NQ];
 #pragma unroll
-        for (int fi = 0; fi < FI; fi++) {
-            const int i = i0 + wi + fi * 16 + (lane & 15);
-            if (i >= A.I) continue;
+    for (int n = 0; n < NP; n++) op[n] = TP::direct_offset(A.ldp, i0, A.I, tid + n * N);
 #pragma unroll
-            for (int fj = 0; fj < FJ; fj++) {
-                const int j = j0 + wj + fj * 16 + (lane >> 4) * 4;
-                float v[4];
+    for (int n = 0; n < NQ; n++) oq[n] = TQ::direct_offset(A.ldq, j0, A.J, tid + n * N);
+    auto fetch = [&](long long k0) {
+        const long long left = k_end - k0;
+        const void *at_p = TP::origin(P, A.ldp, i0, k0), *at_q = TQ::origin(Q, A.ldq, j0, k0);
+        char *lp = lds + wave * 1024, *lq = lp + BI * 128;
+        if (left >= KSTEP<T>) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = acc[fi][fj][e];
-                if (j < A.J) store_f32<float, 4>(A.slab + ((size_t)split * A.I + i) * A.J + j, A.J - j, v);
-            }
-            if (sum_rows && lane < 16) A.row_sum[(size_t)split * A.I + i] = ones[fi][0];
+            for (int n = 0; n < NP; n++) load_direct(at_p, op[n], lp + n * N * 16);
+#pragma unroll
+            for (int n = 0; n < NQ; n++) load_direct(at_q, oq[n], lq + n * N * 16);
+        } else {
+#pragma unroll
+            for (int n = 0; n < NP; n++) load_direct(at_p, TP::direct_k(tid + n * N) < left ? op[n] : DIRECT_RANGE, lp + n * N * 16);
+#pragma unroll
+            for (int n = 0; n < NQ; n++) load_direct(at_q, TQ::direct_k(tid + n * N) < left ? oq[n] : DIRECT_RANGE, lq + n * N * 16);
         }
-    } else {
-        // 16 rows at a time through LDS (a wave's own part of it), after which a lane holds VW columns of one row in a run: rows
-        // are written, and residuals read, in whole 16-byte accesses
-        constexpr int WC = FJ * 16, PITCH = WC + 4, VW = WC / 4;
-        __syncthreads();
-        float* own = (float*)lds + wave * 16 * PITCH;
-        const int j = j0 + wj + (lane & 3) * VW, left = A.J - j;
-        float bias[VW];
-        if (EPI == EPI_FORWARD) {
+    };
+    f32x4 acc[FI][FJ], ones[FI];
 #pragma unroll
-            for (int e = 0; e < VW; e++) bias[e] = 0.f;
-            if (A.bias) load_run<T, VW>((const T*)A.bias + j, left, bias);
+    for (int i = 0; i < FI; i++) {
+        ones[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < FJ; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    Frag one;
+#pragma unroll
+    for (int e = 0; e < PclipVec<T>::N; e++) one[e] = (T)1.f;
+    const bool sum_rows = EPI == EPI_SLAB && A.row_sum && tj == 0 && wj == 0;
+
+    fetch(k_first);
+    for (long long k = k_first; k < k_end; k += KSTEP<T>) {
+        __syncthreads();   // every wave's part of the tile is there
+        Frag fp[2][FI], fq[2][FJ];
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+#pragma unroll
+            for (int j = 0; j < FJ; j++) fq[s][j] = TQ::frag(lds + BI * 128, wj + j * 16, s, lane);
+#pragma unroll
+            for (int i = 0; i < FI; i++) fp[s][i] = TP::frag(lds, wi + i * 16, s, lane);
         }
+        __syncthreads();   // and in every wave's registers: LDS may be written again
+        if (k + KSTEP<T> < k_end) fetch(k + KSTEP<T>);
 #pragma unroll
-        for (int fi = 0; fi < FI; fi++) {
+        for (int s = 0; s < 2; s++) {
 #pragma unroll
-            for (int fj = 0; fj < FJ; fj++) *(f32x4*)(own + (lane & 15) * PITCH + fj * 16 + (lane >> 4) * 4) = acc[fi][fj];
-            float v[VW];
+            for (int i = 0; i < FI; i++)
 #pragma unroll
-            for (int e = 0; e < VW; e += 4) *(f32x4*)(v + e) = *(const f32x4*)(own + (lane >> 2) * PITCH + (lane & 3) * VW + e);
-            const int i = i0 + wi + fi * 16 + (lane >> 2);
-            if (i >= A.I || left <= 0) continue;
-            const size_t at = (size_t)i * A.J + j;
-            if constexpr (EPI == EPI_FORWARD) {
-                float slope[VW];
+                for (int j = 0; j < FJ; j++) acc[i][j] = Mfma<T>::step(fq[s][j], fp[s][i], acc[i][j]);
+            if (sum_rows)
 #pragma unroll
-                for (int e = 0; e < VW; e++) v[e] = activate<sizeof(T) == 4>(v[e] + bias[e], A.act, slope[e]);
-                if (A.slope) store_slope<T, VW>((SlopeOf<T>*)A.slope + at, left, slope);
-                if (A.residual) {
-                    float res[VW];
-                    load_run<T, VW>((const T*)A.residual + at, left, res);
-#pragma unroll
-                    for (int e = 0; e < VW; e++) v[e] += res[e];
-                }
-            }
-            store_run<T, VW>((T*)A.out + at, left, v);
+                for (int i = 0; i < FI; i++) ones[i] = Mfma<T>::step(one, fp[s][i], ones[i]);
         }
     }
+    finish<T, FI, FJ, EPI>(A, acc, ones, sum_rows, lds, i0 + wi, j0 + wj, split);
 }
 
 // out[e] = sum over the splits' slabs, in their order, rounded once; blocks behind those of the weight's gradient add the row
@@ -413,39 +528,61 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, co
 }
 
 // ---- host side -----------------------------------------------------------------------------------------
-template <typename T, int BI, int BJ, int WI, int WJ, bool PK, bool QK, int EPI>
+template <typename T, int BI, int BJ, bool DIRECT, bool PK, bool QK, int EPI>
 int launch_tile(GemmArgs A, hipStream_t st) {
     static PclipLdsLimit limit;
-    constexpr size_t bytes = 2 * (size_t)(BI + BJ) * 128;
-    auto* fn = gemm_kernel<T, BI, BJ, WI, WJ, PK, QK, EPI>;
-    const int rc = pclip_ensure_lds(limit, (const void*)fn, bytes, "linear");
+    constexpr size_t bytes = (DIRECT ? 1 : 2) * (size_t)(BI + BJ) * 128;
+    const void* fn;
+    if constexpr (DIRECT) fn = (const void*)&gemm_direct_kernel<T, BI, BJ, 2, 2, PK, QK, EPI>;
+    else fn = (const void*)&gemm_kernel<T, BI, BJ, 2, 2, PK, QK, EPI>;
+    const int rc = pclip_ensure_lds(limit, fn, bytes, "linear");
     if (rc) return rc;
     A.tiles_i = (A.I + BI - 1) / BI;
     A.tiles_j = (A.J + BJ - 1) / BJ;
     const long long blocks = (long long)A.tiles_i * A.tiles_j * A.splits;
     PCLIP_REQUIRE(blocks <= 0x7fffffffll, "linear: too many tiles (%lld)", blocks);
-    fn<<<(int)blocks, 64 * WI * WJ, bytes, st>>>(A);
+    if constexpr (DIRECT) gemm_direct_kernel<T, BI, BJ, 2, 2, PK, QK, EPI><<<(int)blocks, 256, bytes, st>>>(A);
+    else gemm_kernel<T, BI, BJ, 2, 2, PK, QK, EPI><<<(int)blocks, 256, bytes, st>>>(A);
     return PCLIP_OK;
 }
 
 long long tiles(long long i, long long j, int bi, int bj) { return ((i + bi - 1) / bi) * ((j + bj - 1) / bj); }
 
+template <typename T, bool DIRECT, bool PK, bool QK, int EPI>
+int launch_size(const GemmArgs& A, int bi, int bj, hipStream_t st) {
+    if constexpr (DIRECT && EPI != EPI_SLAB)
+        if (bi == 256) return launch_tile<T, 256, 128, DIRECT, PK, QK, EPI>(A, st);
+    if (bi >= 128) return launch_tile<T, 128, 128, DIRECT, PK, QK, EPI>(A, st);
+    return launch_tile<T, 64, 64, DIRECT, PK, QK, EPI>(A, st);
+}
+// whether every row of both operands begins at a multiple of 16 bytes
+template <typename T>
+bool direct(const GemmArgs& A) {
+    const uintptr_t bits = (uintptr_t)A.P | (uintptr_t)A.Q | (uintptr_t)A.ldp * sizeof(T) | (uintptr_t)A.ldq * sizeof(T);
+    return (bits & 15) == 0;
+}
+template <typename T, bool PK, bool QK, int EPI>
+int launch_product(const GemmArgs& A, int bi, int bj, hipStream_t st) {
+    return direct<T>(A) ? launch_size<T, true, PK, QK, EPI>(A, bi, bj, st) : launch_size<T, false, PK, QK, EPI>(A, bi, bj, st);
+}
+
+// forward and dx: the largest tile that still gives every compute unit work
 template <typename T, bool PK, bool QK, int EPI>
 int launch_rows(const GemmArgs& A, hipStream_t st) {
-    if (tiles(A.I, A.J, 128, 128) >= 256) return launch_tile<T, 128, 128, 2, 2, PK, QK, EPI>(A, st);
-    return launch_tile<T, 64, 64, 2, 2, PK, QK, EPI>(A, st);
+    const int bi = tiles(A.I, A.J, 256, 128) >= 512 ? 256 : tiles(A.I, A.J, 128, 128) >= 256 ? 128 : 64;
+    return launch_product<T, PK, QK, EPI>(A, bi, bi == 64 ? 64 : 128, st);
 }
 
 // the product over the rows (dW): tile size and the number of splits
-struct RowPlan { int tile, splits; long long k_split; };
+struct RowPlan { int bi, bj, splits; long long k_split; };
 RowPlan row_plan(int M, int K, int N, int dtype) {
-    const int step = dtype == PCLIP_DT_F32 ? 32 : 64, tile = K > 64 && N > 64 ? 128 : 64;
-    const long long t = tiles(N, K, tile, tile), steps = ((long long)M + step - 1) / step;
-    long long s = (256 + t - 1) / t;
+    const int step = dtype == PCLIP_DT_F32 ? 32 : 64, bj = K > 64 && N > 64 ? 128 : 64, bi = bj;
+    const long long t = tiles(N, K, bi, bj), steps = ((long long)M + step - 1) / step;
+    long long s = 512 / t;                          // two workgroups a compute unit, in one round
     if (s > (steps + 3) / 4) s = (steps + 3) / 4;   // four steps a workgroup at least
     if (s < 1) s = 1;
     const long long per = (steps + s - 1) / s;
-    return {tile, (int)((steps + per - 1) / per), per * step};
+    return {bi, bj, (int)((steps + per - 1) / per), per * step};
 }
 
 template <typename T>
@@ -473,7 +610,7 @@ int backward(const T* x, const T* w, const T* dy, const void* saved, int is_outp
         A.P = dz, A.Q = x, A.ldp = N, A.ldq = K, A.I = N, A.J = K, A.K = M, A.k_split = p.k_split, A.splits = p.splits;
         A.slab = (float*)ws;
         A.row_sum = db ? A.slab + (size_t)p.splits * N * K : nullptr;
-        const int rc = p.tile == 128 ? launch_tile<T, 128, 128, 2, 2, false, false, EPI_SLAB>(A, st) : launch_tile<T, 64, 64, 2, 2, false, false, EPI_SLAB>(A, st);
+        const int rc = launch_product<T, false, false, EPI_SLAB>(A, p.bi, p.bj, st);
         if (rc) return rc;
         const long long n = (long long)N * K;
         SlabSum S = {{A.slab, A.row_sum}, {dw, db}, {n, N}, p.splits, dw ? (int)((n + 63) / 64) : 0};
