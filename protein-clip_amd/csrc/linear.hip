@@ -141,91 +141,83 @@ struct Tile {
 // act(z) and its slope.  f32 results use the library's erf and exp.  For 16-bit results the Gaussian tail is
 // Phi(-a) = exp(-a^2 / 2) * P(1 / (1 + 0.3 a)), P a polynomial fitted to erfcx(a / sqrt 2) / 2 by reweighted least
 // squares over 0 <= a <= 13: 1.9e-6 relative error, a hundredth of an f16 half step, in one exp and one reciprocal,
-// which the slope's density shares.  Far arguments are cut at 40 where only their product with a vanished density
-// enters, so an infinite z has the limit's slope.
+// and z Phi(z) = max(z, 0) - a Phi(-a), Phi(z) + z phi(z) = exp(-a^2 / 2) (P - a / sqrt(2 pi)) or one minus that.
+// Arguments are cut off where only their product with a factor that has vanished remains, so that an infinite z has the
+// limits of value and slope; a NaN passes through the factor.
 template <bool EXACT, int ACT>
 __device__ __forceinline__ float activate(float z, float& slope) {
     if constexpr (ACT == PCLIP_ACT_RELU) {
         slope = z > 0.f ? 1.f : 0.f;
         return z > 0.f ? z : (z != z ? z : 0.f);   // NaN stays
-    }
-    if constexpr (ACT == PCLIP_ACT_GELU) {
-        const float c = fminf(fmaxf(z, -40.f), 40.f);
-        float phi, density;
-        if constexpr (EXACT) {
-            density = expf(-0.5f * c * c);
-            phi = 0.5f * erfcf(z * -0.70710678118654752f);
-        } else {
-            const float t = __builtin_amdgcn_rcpf(fmaf(0.3f, fabsf(c), 1.f));
-            density = __builtin_amdgcn_exp2f(c * c * -0.72134752044448170f);
-            float g = -0.0845887363f;
-            g = fmaf(g, t, 0.240555853f);
-            g = fmaf(g, t, -0.0486187227f);
-            g = fmaf(g, t, 0.164744467f);
-            g = fmaf(g, t, 0.106712937f);
-            g = fmaf(g, t, 0.121272907f);
-            g = fmaf(g, t, -7.96368695e-05f);
-            g *= density;
-            phi = c < 0.f ? g : 1.f - g;
-        }
-        slope = fmaf(c * 0.39894228040143268f, density, phi);
-        return z * phi;
-    }
-    if constexpr (ACT == PCLIP_ACT_SILU) {
+    } else if constexpr (ACT == PCLIP_ACT_GELU && EXACT) {
+        const float phi = 0.5f * erfcf(z * -0.70710678118654752f);
+        slope = fmaf(fminf(fmaxf(z, -40.f), 40.f) * 0.39894228040143268f, expf(-0.5f * z * z), phi);
+        return fmaxf(z, -40.f) * phi;
+    } else if constexpr (ACT == PCLIP_ACT_GELU) {
+        const float a = fminf(fabsf(z), 40.f), t = __builtin_amdgcn_rcpf(fmaf(0.3f, a, 1.f));
+        const float e = __builtin_amdgcn_exp2f(z * -0.72134752044448170f * z);
+        float p = -0.0845887363f;
+        p = fmaf(p, t, 0.240555853f);
+        p = fmaf(p, t, -0.0486187227f);
+        p = fmaf(p, t, 0.164744467f);
+        p = fmaf(p, t, 0.106712937f);
+        p = fmaf(p, t, 0.121272907f);
+        p = fmaf(p, t, -7.96368695e-05f);
+        const float w = e * fmaf(-0.39894228040143268f, a, p);
+        slope = z < 0.f ? w : 1.f - w;
+        return fmaf(-a, p * e, fmaxf(z, 0.f));
+    } else if constexpr (ACT == PCLIP_ACT_SILU) {
         float s;
         if constexpr (EXACT) s = 1.f / (1.f + expf(-z));
         else s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
-        const float c = fminf(fmaxf(z, -100.f), 100.f);
-        slope = s * fmaf(c, 1.f - s, 1.f);
-        return z * s;
+        const float y = fmaxf(z, -100.f) * s;
+        slope = fmaf(fminf(y, 100.f), 1.f - s, s);
+        return y;
+    } else {
+        slope = 1.f;
+        return z;
     }
-    slope = 1.f;
-    return z;
 }
 
-// the activation is chosen once for a run of values, so that their chains of dependent instructions interleave
-template <bool EXACT, int ACT, int VW>
-__device__ __forceinline__ void activate_run(float (&v)[VW], const float (&bias)[VW], float (&slope)[VW]) {
-#pragma unroll
-    for (int e = 0; e < VW; e++) v[e] = activate<EXACT, ACT>(v[e] + bias[e], slope[e]);
-}
-
-// The slope is kept for the backward: as it is for f32, for 16-bit types as a whole number of steps of 1 / 28672 (slopes lie
-// between -0.13 and 1.13; half a step is a fifteenth of an f16 rounding at one), so that dz is rounded once, not twice.
+// The slope is kept for the backward: as it is for f32, for 16-bit types as 16-bit whole numbers in steps of
+// 1 / (0.875 * 32767) (slopes lie between -0.13 and 1.13; half a step is a fourteenth of an f16 rounding at one, and the
+// hardware packs two such numbers in one instruction), so that dz is rounded once, not twice.
 template <typename T> using SlopeOf = std::conditional_t<sizeof(T) == 4, float, short>;
-template <typename T> constexpr float SLOPE_UNIT = sizeof(T) == 4 ? 1.f : 1.f / 28672.f;
+template <typename T> constexpr float SLOPE_UNIT = sizeof(T) == 4 ? 1.f : 1.f / (0.875f * 32767.f);
 
-// VW columns of one row in 16-byte accesses
-template <typename T, int VW>
-__device__ __forceinline__ void load_run(const T* p, int valid, float (&v)[VW]) {
-    constexpr int V = VW < PclipVec<T>::N ? VW : PclipVec<T>::N;
+template <typename T, int V>
+__device__ __forceinline__ void store_slope(SlopeOf<T>* p, int valid, const float (&v)[V]) {
+    if constexpr (sizeof(T) == 4) {
+        store_f32<T, V>(p, valid, v);
+    } else {
+        PclipPack<short, V> a;
 #pragma unroll
-    for (int e = 0; e < VW; e += V) load_f32<T, V>(p + e, valid - e, *(float(*)[V])(v + e));
-}
-template <typename T, int VW>
-__device__ __forceinline__ void store_run(T* p, int valid, const float (&v)[VW]) {
-    constexpr int V = VW < PclipVec<T>::N ? VW : PclipVec<T>::N;
+        for (int i = 0; i < V; i += 2) {
+            const auto two = __builtin_amdgcn_cvt_pknorm_i16(0.875f * v[i], 0.875f * v[i + 1]);
+            a.v[i] = two[0];
+            a.v[i + 1] = two[1];
+        }
+        if (valid >= V) {
+            *(PclipPack<short, V>*)p = a;
+        } else {
 #pragma unroll
-    for (int e = 0; e < VW; e += V) store_f32<T, V>(p + e, valid - e, *(const float(*)[V])(v + e));
-}
-template <typename T, int VW>
-__device__ __forceinline__ void store_slope(SlopeOf<T>* p, int valid, float (&v)[VW]) {
-#pragma unroll
-    for (int e = 0; e < VW; e++) v[e] = sizeof(T) == 4 ? v[e] : rintf(v[e] * 28672.f);
-    store_run<SlopeOf<T>, VW>(p, valid, v);
+            for (int i = 0; i < V; i++)
+                if (i < valid) p[i] = a.v[i];
+        }
+    }
 }
 
 // ---- the product -----------------------------------------------------------------------------------
-enum { EPI_FORWARD, EPI_STORE, EPI_SLAB };
+// what becomes of the sums: below EPI_STORE the forward's epilogue with that activation
+enum { EPI_STORE = PCLIP_ACT_SILU + 1, EPI_SLAB };
 
 struct GemmArgs {
     const void *P, *Q;
     int ldp, ldq, I, J;
     long long K, k_split;           // contraction length, and the part of one workgroup (a multiple of KSTEP)
     int tiles_i, tiles_j, splits;
-    const void *bias, *residual;    // EPI_FORWARD
+    const void *bias, *residual;    // forward
     void *out, *slope;
-    int act;
     float *slab, *row_sum;          // EPI_SLAB: [splits][I][J], [splits][I] or NULL
 };
 
@@ -256,44 +248,44 @@ __device__ __forceinline__ void finish(const GemmArgs& A, f32x4 (&acc)[FI][FJ], 
             if (sum_rows && lane < 16) A.row_sum[(size_t)split * A.I + i] = ones[fi][0];
         }
     } else {
-        // 16 rows at a time through LDS (a wave's own part of it), after which a lane holds VW columns of one row in a run: rows
-        // are written, and residuals read, in whole 16-byte accesses
-        constexpr int WC = FJ * 16, PITCH = WC + 4, VW = WC / 4;
+        // 16 rows at a time through LDS (a wave's own part of it), after which a lane holds the V columns of one 16-byte access and
+        // neighbouring lanes neighbouring ones: whole lines are written, and read of the residual
+        constexpr int V = PclipVec<T>::N, WC = FJ * 16, PITCH = WC + 4, LANES = WC / V, ROWS = 64 / LANES;
         __syncthreads();
         float* own = (float*)lds + (threadIdx.x >> 6) * 16 * PITCH;
-        const int j = j0 + (lane & 3) * VW, left = A.J - j;
-        float bias[VW];
-        if (EPI == EPI_FORWARD) {
+        const int c = (lane % LANES) * V, j = j0 + c, left = A.J - j;
+        float bias[V];
+        if (EPI < EPI_STORE) {
 #pragma unroll
-            for (int e = 0; e < VW; e++) bias[e] = 0.f;
-            if (A.bias) load_run<T, VW>((const T*)A.bias + j, left, bias);
+            for (int e = 0; e < V; e++) bias[e] = 0.f;
+            if (A.bias) load_f32<T, V>((const T*)A.bias + j, left, bias);
         }
 #pragma unroll
         for (int fi = 0; fi < FI; fi++) {
 #pragma unroll
             for (int fj = 0; fj < FJ; fj++) *(f32x4*)(own + (lane & 15) * PITCH + fj * 16 + (lane >> 4) * 4) = acc[fi][fj];
-            float v[VW];
 #pragma unroll
-            for (int e = 0; e < VW; e += 4) *(f32x4*)(v + e) = *(const f32x4*)(own + (lane >> 2) * PITCH + (lane & 3) * VW + e);
-            const int i = i0 + fi * 16 + (lane >> 2);
-            if (i >= A.I || left <= 0) continue;
-            const size_t at = (size_t)i * A.J + j;
-            if constexpr (EPI == EPI_FORWARD) {
-                float slope[VW];
-                constexpr bool EXACT = sizeof(T) == 4;
-                if (A.act == PCLIP_ACT_NONE) activate_run<EXACT, PCLIP_ACT_NONE>(v, bias, slope);
-                else if (A.act == PCLIP_ACT_RELU) activate_run<EXACT, PCLIP_ACT_RELU>(v, bias, slope);
-                else if (A.act == PCLIP_ACT_GELU) activate_run<EXACT, PCLIP_ACT_GELU>(v, bias, slope);
-                else activate_run<EXACT, PCLIP_ACT_SILU>(v, bias, slope);
-                if (A.slope) store_slope<T, VW>((SlopeOf<T>*)A.slope + at, left, slope);
-                if (A.residual) {
-                    float res[VW];
-                    load_run<T, VW>((const T*)A.residual + at, left, res);
+            for (int first = 0; first < 16; first += ROWS) {
+                const int row = first + lane / LANES, i = i0 + fi * 16 + row;
+                float v[V];
 #pragma unroll
-                    for (int e = 0; e < VW; e++) v[e] += res[e];
+                for (int e = 0; e < V; e += 4) *(f32x4*)(v + e) = *(const f32x4*)(own + row * PITCH + c + e);
+                if (i >= A.I || left <= 0) continue;
+                const size_t at = (size_t)i * A.J + j;
+                if constexpr (EPI < EPI_STORE) {
+                    float slope[V];
+#pragma unroll
+                    for (int e = 0; e < V; e++) v[e] = activate<sizeof(T) == 4, EPI>(v[e] + bias[e], slope[e]);
+                    if (A.slope) store_slope<T, V>((SlopeOf<T>*)A.slope + at, left, slope);
+                    if (A.residual) {
+                        float res[V];
+                        load_f32<T, V>((const T*)A.residual + at, left, res);
+#pragma unroll
+                        for (int e = 0; e < V; e++) v[e] += res[e];
+                    }
                 }
+                store_f32<T, V>((T*)A.out + at, left, v);
             }
-            store_run<T, VW>((T*)A.out + at, left, v);
         }
     }
 }
@@ -401,6 +393,9 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_direct_kernel(const Gemm
     extern __shared__ __attribute__((aligned(16))) char lds[];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#ifdef STAGGER
+    if (gridDim.x > 1024 && blockIdx.x >= 256 && blockIdx.x < 512) for (int q = 0; q < STAGGER; q++) __builtin_amdgcn_s_sleep(127);
+#endif
     int b = xcd_order(blockIdx.x, gridDim.x);
     const int tj = b % A.tiles_j;
     b /= A.tiles_j;
@@ -569,7 +564,12 @@ int launch_product(const GemmArgs& A, int bi, int bj, hipStream_t st) {
 // forward and dx: the largest tile that still gives every compute unit work
 template <typename T, bool PK, bool QK, int EPI>
 int launch_rows(const GemmArgs& A, hipStream_t st) {
-    const int bi = tiles(A.I, A.J, 256, 128) >= 512 ? 256 : tiles(A.I, A.J, 128, 128) >= 256 ? 128 : 64;
+#ifdef NO256
+    const int bi =
+#else
+    const int bi = tiles(A.I, A.J, 256, 128) >= 512 ? 256 :
+#endif
+        tiles(A.I, A.J, 128, 128) >= 256 ? 128 : 64;
     return launch_product<T, PK, QK, EPI>(A, bi, bi == 64 ? 64 : 128, st);
 }
 
@@ -586,7 +586,12 @@ RowPlan row_plan(int M, int K, int N, int dtype) {
 }
 
 template <typename T>
-int forward(const GemmArgs& A, hipStream_t st) { return launch_rows<T, true, true, EPI_FORWARD>(A, st); }
+int forward(const GemmArgs& A, int act, hipStream_t st) {
+    if (act == PCLIP_ACT_NONE) return launch_rows<T, true, true, PCLIP_ACT_NONE>(A, st);
+    if (act == PCLIP_ACT_RELU) return launch_rows<T, true, true, PCLIP_ACT_RELU>(A, st);
+    if (act == PCLIP_ACT_GELU) return launch_rows<T, true, true, PCLIP_ACT_GELU>(A, st);
+    return launch_rows<T, true, true, PCLIP_ACT_SILU>(A, st);
+}
 
 template <typename T>
 int backward(const T* x, const T* w, const T* dy, const void* saved, int is_output, int M, int K, int N, int dtype, int act, T* dx, T* dw, T* db, char* ws,
@@ -636,11 +641,11 @@ extern "C" int pclip_linear_fwd(const void* x, const void* w, const void* bias, 
     PCLIP_REQUIRE(x && w && y, "linear_fwd: null pointer");
     GemmArgs A = {};
     A.P = x, A.Q = w, A.ldp = K, A.ldq = K, A.I = M, A.J = N, A.K = K, A.k_split = (K + 63) / 64 * 64, A.splits = 1;
-    A.bias = bias, A.residual = residual, A.out = y, A.slope = slope, A.act = activation;
+    A.bias = bias, A.residual = residual, A.out = y, A.slope = slope;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == PCLIP_DT_F32) rc = forward<float>(A, st);
-    else if (dtype == PCLIP_DT_BF16) rc = forward<__bf16>(A, st);
-    else rc = forward<_Float16>(A, st);
+    if (dtype == PCLIP_DT_F32) rc = forward<float>(A, activation, st);
+    else if (dtype == PCLIP_DT_BF16) rc = forward<__bf16>(A, activation, st);
+    else rc = forward<_Float16>(A, activation, st);
     return rc ? rc : pclip_check_launch("linear_fwd");
 }
 

@@ -258,7 +258,7 @@ def _linear_sizes(x, w):
 
 
 def _slope_type(dtype):
-    return F32 if dtype == F32 else torch.int16   # steps of 1 / 28672
+    return F32 if dtype == F32 else torch.int16   # whole steps, see pclip.h
 
 
 def linear_fwd(x, w, bias=None, residual=None, activation: str = "none", want_slope: bool = False):
