@@ -35,6 +35,26 @@ __device__ __forceinline__ void store_f32(T* p, int valid, const float (&v)[V]) 
             if (i < valid) p[i] = (T)v[i];
     }
 }
+// 16 bytes past the L2 (results that nobody reads back soon: they would push out what the kernel still reads)
+template <typename P>
+__device__ __forceinline__ void store_past_l2(void* p, const P& a) {
+    static_assert(sizeof(P) == 16, "one access");
+    typedef unsigned __attribute__((ext_vector_type(4), aligned(1))) u32x4_any;
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4_any, a), (u32x4_any*)p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void stream_f32(T* p, int valid, const float (&v)[V]) {
+    if (valid >= V) {
+        PclipPack<T, V> a;
+#pragma unroll
+        for (int i = 0; i < V; i++) a.v[i] = (T)v[i];
+        store_past_l2(p, a);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (i < valid) p[i] = (T)v[i];
+    }
+}
 
 inline int pclip_dtype_size(int dtype) { return dtype == PCLIP_DT_F32 ? 4 : 2; }
 inline bool pclip_dtype_ok(int dtype) { return dtype == PCLIP_DT_F32 || dtype == PCLIP_DT_BF16 || dtype == PCLIP_DT_F16; }

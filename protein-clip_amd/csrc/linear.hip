@@ -188,7 +188,7 @@ template <typename T> constexpr float SLOPE_UNIT = sizeof(T) == 4 ? 1.f : 1.f / 
 template <typename T, int V>
 __device__ __forceinline__ void store_slope(SlopeOf<T>* p, int valid, const float (&v)[V]) {
     if constexpr (sizeof(T) == 4) {
-        store_f32<T, V>(p, valid, v);
+        stream_f32<T, V>(p, valid, v);
     } else {
         PclipPack<short, V> a;
 #pragma unroll
@@ -198,7 +198,7 @@ __device__ __forceinline__ void store_slope(SlopeOf<T>* p, int valid, const floa
             a.v[i + 1] = two[1];
         }
         if (valid >= V) {
-            *(PclipPack<short, V>*)p = a;
+            store_past_l2(p, a);
         } else {
 #pragma unroll
             for (int i = 0; i < V; i++)
@@ -221,6 +221,19 @@ struct GemmArgs {
     float *slab, *row_sum;          // EPI_SLAB: [splits][I][J], [splits][I] or NULL
 };
 
+// The rows' sums as one more column of the product, of ones: the first half of a wave's rows, or the second.  (`first` comes
+// from a scalar: matrix instructions run whatever the lanes' mask says, so no branch around them may be the lanes' own.)
+template <typename T, int FI>
+__device__ __forceinline__ void add_rows(const typename Mfma<T>::Frag (&fp)[FI], typename Mfma<T>::Frag one, bool first, f32x4 (&ones)[FI / 2]) {
+    if (first) {
+#pragma unroll
+        for (int i = 0; i < FI / 2; i++) ones[i] = Mfma<T>::step(one, fp[i], ones[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < FI / 2; i++) ones[i] = Mfma<T>::step(one, fp[FI / 2 + i], ones[i]);
+    }
+}
+
 // Workgroups go to the eight XCDs in turn; give each XCD a run of neighbouring tiles, which share rows of P or Q in its L2.
 __device__ __forceinline__ int xcd_order(int b, int n) {
     const int xcd = b & 7, q = n >> 3, r = n & 7;
@@ -229,7 +242,7 @@ __device__ __forceinline__ int xcd_order(int b, int n) {
 
 // What a wave does with its accumulators: rows from i0, columns from j0 on.
 template <typename T, int FI, int FJ, int EPI>
-__device__ __forceinline__ void finish(const GemmArgs& A, f32x4 (&acc)[FI][FJ], f32x4 (&ones)[FI], bool sum_rows, char* lds, int i0, int j0, int split) {
+__device__ __forceinline__ void finish(const GemmArgs& A, f32x4 (&acc)[FI][FJ], f32x4 (&ones)[FI / 2], bool sum_rows, char* lds, int i0, int j0, int split) {
     const int lane = threadIdx.x & 63;
     // a lane holds, of every 16 x 16 tile, row i = lane % 16 and the four columns from j = 4 * (lane / 16) on
     if constexpr (EPI == EPI_SLAB) {
@@ -245,7 +258,8 @@ __device__ __forceinline__ void finish(const GemmArgs& A, f32x4 (&acc)[FI][FJ], 
                 for (int e = 0; e < 4; e++) v[e] = acc[fi][fj][e];
                 if (j < A.J) store_f32<float, 4>(A.slab + ((size_t)split * A.I + i) * A.J + j, A.J - j, v);
             }
-            if (sum_rows && lane < 16) A.row_sum[(size_t)split * A.I + i] = ones[fi][0];
+            const bool first = (threadIdx.x >> 6 & 1) == 0;   // the column of waves, see add_rows
+            if (sum_rows && lane < 16 && first == (fi < FI / 2)) A.row_sum[(size_t)split * A.I + i] = ones[fi % (FI / 2)][0];
         }
     } else {
         // 16 rows at a time through LDS (a wave's own part of it), after which a lane holds the V columns of one 16-byte access and
@@ -284,7 +298,7 @@ __device__ __forceinline__ void finish(const GemmArgs& A, f32x4 (&acc)[FI][FJ], 
                         for (int e = 0; e < V; e++) v[e] += res[e];
                     }
                 }
-                store_f32<T, V>((T*)A.out + at, left, v);
+                stream_f32<T, V>((T*)A.out + at, left, v);
             }
         }
     }
@@ -299,7 +313,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_kernel(const GemmArgs A)
     constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16, BYTES = (BI + BJ) * 128;
     extern __shared__ __attribute__((aligned(16))) char lds[];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int b = xcd_order(blockIdx.x, gridDim.x);
     const int tj = b % A.tiles_j;
     b /= A.tiles_j;
@@ -335,17 +349,17 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_kernel(const GemmArgs A)
             for (int n = 0; n < NQ; n++) rq[n] = TQ::fetch_edge(Q, A.ldq, j0, A.J, k0, k_end, tid + n * N);
         }
     };
-    f32x4 acc[FI][FJ], ones[FI];
+    f32x4 acc[FI][FJ], ones[FI / 2];
 #pragma unroll
     for (int i = 0; i < FI; i++) {
-        ones[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        ones[i / 2] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < FJ; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     Frag one;
 #pragma unroll
     for (int e = 0; e < PclipVec<T>::N; e++) one[e] = (T)1.f;
-    const bool sum_rows = EPI == EPI_SLAB && A.row_sum && tj == 0 && wj == 0;
+    const bool sum_rows = EPI == EPI_SLAB && A.row_sum && tj == 0;   // each column of waves half of its rows
 
     fetch(k_first);
     int buf = 0;
@@ -369,9 +383,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_kernel(const GemmArgs A)
             for (int i = 0; i < FI; i++)
 #pragma unroll
                 for (int j = 0; j < FJ; j++) acc[i][j] = Mfma<T>::step(fq[j], fp[i], acc[i][j]);
-            if (sum_rows)
-#pragma unroll
-                for (int i = 0; i < FI; i++) ones[i] = Mfma<T>::step(one, fp[i], ones[i]);
+            if (sum_rows) add_rows<T, FI>(fp, one, wj == 0, ones);
         }
         buf ^= 1;
     }
@@ -393,9 +405,6 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_direct_kernel(const Gemm
     extern __shared__ __attribute__((aligned(16))) char lds[];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-#ifdef STAGGER
-    if (gridDim.x > 1024 && blockIdx.x >= 256 && blockIdx.x < 512) for (int q = 0; q < STAGGER; q++) __builtin_amdgcn_s_sleep(127);
-#endif
     int b = xcd_order(blockIdx.x, gridDim.x);
     const int tj = b % A.tiles_j;
     b /= A.tiles_j;
@@ -426,17 +435,17 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_direct_kernel(const Gemm
             for (int n = 0; n < NQ; n++) load_direct(at_q, TQ::direct_k(tid + n * N) < left ? oq[n] : DIRECT_RANGE, lq + n * N * 16);
         }
     };
-    f32x4 acc[FI][FJ], ones[FI];
+    f32x4 acc[FI][FJ], ones[FI / 2];
 #pragma unroll
     for (int i = 0; i < FI; i++) {
-        ones[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        ones[i / 2] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < FJ; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     Frag one;
 #pragma unroll
     for (int e = 0; e < PclipVec<T>::N; e++) one[e] = (T)1.f;
-    const bool sum_rows = EPI == EPI_SLAB && A.row_sum && tj == 0 && wj == 0;
+    const bool sum_rows = EPI == EPI_SLAB && A.row_sum && tj == 0;   // each column of waves half of its rows
 
     fetch(k_first);
     for (long long k = k_first; k < k_end; k += KSTEP<T>) {
@@ -457,9 +466,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_direct_kernel(const Gemm
             for (int i = 0; i < FI; i++)
 #pragma unroll
                 for (int j = 0; j < FJ; j++) acc[i][j] = Mfma<T>::step(fq[s][j], fp[s][i], acc[i][j]);
-            if (sum_rows)
-#pragma unroll
-                for (int i = 0; i < FI; i++) ones[i] = Mfma<T>::step(one, fp[s][i], ones[i]);
+            if (sum_rows) add_rows<T, FI>(fp[s], one, wj == 0, ones);
         }
     }
     finish<T, FI, FJ, EPI>(A, acc, ones, sum_rows, lds, i0 + wi, j0 + wj, split);
@@ -564,12 +571,7 @@ int launch_product(const GemmArgs& A, int bi, int bj, hipStream_t st) {
 // forward and dx: the largest tile that still gives every compute unit work
 template <typename T, bool PK, bool QK, int EPI>
 int launch_rows(const GemmArgs& A, hipStream_t st) {
-#ifdef NO256
-    const int bi =
-#else
-    const int bi = tiles(A.I, A.J, 256, 128) >= 512 ? 256 :
-#endif
-        tiles(A.I, A.J, 128, 128) >= 256 ? 128 : 64;
+    const int bi = tiles(A.I, A.J, 256, 128) >= 512 ? 256 : tiles(A.I, A.J, 128, 128) >= 256 ? 128 : 64;
     return launch_product<T, PK, QK, EPI>(A, bi, bi == 64 ? 64 : 128, st);
 }
 
