@@ -35,12 +35,12 @@ __device__ __forceinline__ void store_f32(T* p, int valid, const float (&v)[V]) 
             if (i < valid) p[i] = (T)v[i];
     }
 }
-// 16 bytes past the L2 (results that nobody reads back soon: they would push out what the kernel still reads)
+// 8 or 16 bytes past the L2 (results that nobody reads back soon: they would push out what the kernel still reads)
 template <typename P>
 __device__ __forceinline__ void store_past_l2(void* p, const P& a) {
-    static_assert(sizeof(P) == 16, "one access");
-    typedef unsigned __attribute__((ext_vector_type(4), aligned(1))) u32x4_any;
-    __builtin_nontemporal_store(__builtin_bit_cast(u32x4_any, a), (u32x4_any*)p);
+    static_assert(sizeof(P) == 16 || sizeof(P) == 8, "one access");
+    typedef unsigned __attribute__((ext_vector_type(sizeof(P) / 4), aligned(1))) Any;
+    __builtin_nontemporal_store(__builtin_bit_cast(Any, a), (Any*)p);
 }
 template <typename T, int V>
 __device__ __forceinline__ void stream_f32(T* p, int valid, const float (&v)[V]) {

@@ -20,6 +20,10 @@ namespace {
 
 constexpr int THREADS = 256;
 constexpr int MAX_D = PCLIP_NORM_MAX_D;
+#ifndef FB
+#define FB 1024
+#endif
+constexpr int FWD_BLOCKS = FB;   // four workgroups a compute unit, which then take row after row
 
 struct NormGateArgs {
     const void *u, *r, *gate;
@@ -38,6 +42,8 @@ struct NormGateArgs {
     int sum_gate;                     // the gate's gradient is a sum over the rows of a group
     int wanted;                       // which affine gradients: bit 0 dwa, 1 dba, 2 dwb, 3 dbb
 };
+
+__host__ __device__ __forceinline__ int padded(int d) { return (d + 3) & ~3; }
 
 // sums of two values over the G lanes that hold a row (16, 64, or the whole workgroup), in every lane
 template <int G>
@@ -69,9 +75,34 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float (*lds)[2]) {
 }
 
 // The elements of one lane: NV vectors of V, vector k at column (k * G + lane) * V.
-template <typename T, int G, int NV>
+template <typename T, int G, int NV, int V>
 struct Row {
-    static constexpr int V = PclipVec<T>::N, E = NV * V, NG = THREADS / G;
+    static constexpr int E = NV * V, NG = THREADS / G;
+    // whether a row is loaded while the one before it is worked on: two waves a SIMD do not cover the memory's latency by
+    // themselves; rows of many f32 would not fit the registers
+    static constexpr bool AHEAD = E * sizeof(T) <= 32;
+    struct Raw { PclipPack<T, V> v[NV]; };
+    static __device__ __forceinline__ void load_raw(const void* base, size_t at, int d, Raw& r) {
+        const T* p = (const T*)base + at;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int valid = d - col(k);
+            if (valid >= V) {
+                r.v[k] = *(const PclipPack<T, V>*)(p + col(k));
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; i++) r.v[k].v[i] = i < valid ? p[col(k) + i] : (T)0.f;
+            }
+        }
+    }
+    static __device__ __forceinline__ void widen(const Raw& r, float (&x)[E]) {
+#pragma unroll
+        for (int i = 0; i < E; i++) x[i] = (float)r.v[i / V].v[i % V];
+    }
+    static __device__ __forceinline__ void fill(float (&x)[E], float v) {
+#pragma unroll
+        for (int i = 0; i < E; i++) x[i] = v;
+    }
     static __device__ __forceinline__ int col(int k) { return (k * G + (int)(threadIdx.x % G)) * V; }
     template <typename S>
     static __device__ __forceinline__ void load(const S* p, int d, float (&x)[E]) {
@@ -81,25 +112,81 @@ struct Row {
     template <typename S>
     static __device__ __forceinline__ void store(S* p, int d, const float (&x)[E]) {
 #pragma unroll
-        for (int k = 0; k < NV; k++) store_f32<S, V>(p + col(k), d - col(k), *(const float(*)[V])(x + k * V));
+        for (int k = 0; k < NV; k++) stream_f32<S, V>(p + col(k), d - col(k), *(const float(*)[V])(x + k * V));
     }
-    static __device__ __forceinline__ void load_param(const void* p, bool f32, int d, float other, float (&x)[E]) {
-        if (!p) {
+    // Affine parameters.  Lanes that take row after row of one place keep theirs in registers when each has a place of its own
+    // (G = 256); waves that share the places read them from LDS, as f32 padded to whole vectors, again for each row: in
+    // registers they would take a quarter of a lane's, which the column sums need.
+    struct Param {
+        static constexpr bool OWN = G == 256;
+        float own[OWN ? E : 1];
+        const float* lds;
+        __device__ __forceinline__ void stage(const void* p, bool f32, int d, float other, float* to) {
+            if constexpr (OWN) {
 #pragma unroll
-            for (int i = 0; i < E; i++) x[i] = other;
-        } else if (f32) {
-            load((const float*)p, d, x);
-        } else {
-            load((const T*)p, d, x);
+                for (int k = 0; k < NV; k++)
+#pragma unroll
+                    for (int i = 0; i < V; i++) own[k * V + i] = at(p, f32, d, other, col(k) + i);
+            } else {
+                for (int c = threadIdx.x; c < padded(d); c += THREADS) to[c] = at(p, f32, d, other, c);
+                lds = to;
+            }
+        }
+        static __device__ __forceinline__ float at(const void* p, bool f32, int d, float other, int c) {
+            return !p || c >= d ? other : f32 ? ((const float*)p)[c] : (float)((const T*)p)[c];
+        }
+        __device__ __forceinline__ void get(int k, int d, float (&x)[V]) const {
+#pragma unroll
+            for (int i = 0; i < V; i += 4) {
+                if constexpr (OWN) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) x[i + j] = own[k * V + i + j];
+                } else {
+                    const int c = col(k) + i;
+                    const f32x4 v = *(const f32x4*)(lds + (c < d ? c : 0));   // lanes behind the row use any
+#pragma unroll
+                    for (int j = 0; j < 4; j++) x[i + j] = v[j];
+                }
+            }
+        }
+    };
+    // a row of the gate: values of T, or bytes (nonzero = 1)
+    struct RawGate { Raw t; PclipPack<uint8_t, V> b[NV]; };
+    static __device__ __forceinline__ void load_gate(const NormGateArgs& A, int row, RawGate& r) {
+        if (A.gate_kind == PCLIP_GATE_BYTES) {
+            const uint8_t* p = (const uint8_t*)A.gate + (size_t)row * A.d;
+#pragma unroll
+            for (int k = 0; k < NV; k++) {
+                const int valid = A.d - col(k);
+                if (valid >= V) {
+                    r.b[k] = *(const PclipPack<uint8_t, V>*)(p + col(k));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; i++) r.b[k].v[i] = i < valid ? p[col(k) + i] : 0;
+                }
+            }
+        } else if (A.gate_kind == PCLIP_GATE_ROWS) {
+            load_raw(A.gate, (size_t)((unsigned)row / (unsigned)A.gate_rows) * A.d, A.d, r.t);
         }
     }
-    static __device__ __forceinline__ void load_gate(const NormGateArgs& A, int row, float (&g)[E]) {
+    static __device__ __forceinline__ void widen_gate(const NormGateArgs& A, const RawGate& r, float (&g)[E]) {
         if (A.gate_kind == PCLIP_GATE_BYTES) {
-            load((const uint8_t*)A.gate + (size_t)row * A.d, A.d, g);
 #pragma unroll
-            for (int i = 0; i < E; i++) g[i] = g[i] != 0.f ? 1.f : 0.f;
+            for (int i = 0; i < E; i++) g[i] = r.b[i / V].v[i % V] ? 1.f : 0.f;
+        } else if (A.gate_kind == PCLIP_GATE_ROWS) {
+            widen(r.t, g);
         } else {
-            load((const T*)A.gate + (size_t)((unsigned)row / (unsigned)A.gate_rows) * A.d, A.d, g);
+            fill(g, 1.f);
+        }
+    }
+    static __device__ __forceinline__ void affine(float (&x)[E], float mean, float rstd, const Param& w, const Param& b, int d) {
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            float wk[V], bk[V];
+            w.get(k, d, wk);
+            b.get(k, d, bk);
+#pragma unroll
+            for (int i = 0; i < V; i++) x[k * V + i] = fmaf((x[k * V + i] - mean) * rstd, wk[i], bk[i]);
         }
     }
     // mean (zero for rms) and 1 / sqrt(mean square of the centred values + eps)
@@ -128,48 +215,54 @@ struct Row {
     }
 };
 
-template <typename T, int G, int NV>
+template <typename T, int G, int NV, int V>
 __global__ __launch_bounds__(THREADS) void norm_gate_fwd_kernel(const NormGateArgs A) {
-    using R = Row<T, G, NV>;
+    using R = Row<T, G, NV, V>;
     constexpr int E = R::E;
     __shared__ float lds[4][2];
     const int d = A.d;
-    for (int row = blockIdx.x * R::NG + (int)threadIdx.x / G; row < A.rows; row += gridDim.x * R::NG) {
+    extern __shared__ __attribute__((aligned(16))) float params[];
+    typename R::Param wa, ba, wb, bb;
+    wa.stage(A.wa, A.param_f32, d, 1.f, params);
+    ba.stage(A.ba, A.param_f32, d, 0.f, params + padded(d));
+    wb.stage(A.wb, A.param_f32, d, 1.f, params + 2 * padded(d));
+    bb.stage(A.bb, A.param_f32, d, 0.f, params + 3 * padded(d));
+    __syncthreads();
+    struct { typename R::Raw u, r; typename R::RawGate g; } in;
+    auto load = [&](int row) {
+        R::load_raw(A.u, (size_t)row * d, d, in.u);
+        if (A.r) R::load_raw(A.r, (size_t)row * d, d, in.r);
+        R::load_gate(A, row, in.g);
+    };
+    const int stride = gridDim.x * R::NG;
+    int row = blockIdx.x * R::NG + (int)threadIdx.x / G;
+    if (R::AHEAD && row < A.rows) load(row);
+    for (; row < A.rows; row += stride) {
+        asm volatile("" ::: "memory");   // parameters in LDS are read again for each row
         const size_t at = (size_t)row * d;
-        float u[E], y[E];
-        R::load((const T*)A.u + at, d, u);
-        if (A.r) R::load((const T*)A.r + at, d, y);
-        else {
-#pragma unroll
-            for (int i = 0; i < E; i++) y[i] = 0.f;
-        }
+        float u[E], y[E], g[E];
+        if (!R::AHEAD) load(row);
+        R::widen(in.u, u);
+        if (A.r) R::widen(in.r, y);
+        else R::fill(y, 0.f);
+        R::widen_gate(A, in.g, g);
+        if (R::AHEAD && A.rows - row > stride) load(row + stride);
         float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
         if (A.after) {
-            float w[E], b[E];
-            R::load_param(A.wa, A.param_f32, d, 1.f, w);
-            R::load_param(A.ba, A.param_f32, d, 0.f, b);
             R::stats(u, A.after, d, A.eps, st.x, st.y, lds);
-#pragma unroll
-            for (int i = 0; i < E; i++) u[i] = fmaf((u[i] - st.x) * st.y, w[i], b[i]);
-        }
-        if (A.gate_kind) {
-            float g[E];
-            R::load_gate(A, row, g);
-#pragma unroll
-            for (int i = 0; i < E; i++) u[i] *= g[i];
+            R::affine(u, st.x, st.y, wa, ba, d);
         }
 #pragma unroll
         for (int k = 0; k < NV; k++)
 #pragma unroll
-            for (int i = 0; i < R::V; i++) y[k * R::V + i] = R::col(k) + i < d ? fmaf(A.scale, u[k * R::V + i], y[k * R::V + i]) : 0.f;
+            for (int j = 0; j < V; j++) {
+                const int i = k * V + j;
+                y[i] = R::col(k) + j < d ? fmaf(A.scale, u[i] * g[i], y[i]) : 0.f;
+            }
         R::store((T*)A.y + at, d, y);
         if (A.before) {
-            float w[E], b[E];
-            R::load_param(A.wb, A.param_f32, d, 1.f, w);
-            R::load_param(A.bb, A.param_f32, d, 0.f, b);
             R::stats(y, A.before, d, A.eps, st.z, st.w, lds);
-#pragma unroll
-            for (int i = 0; i < E; i++) y[i] = fmaf((y[i] - st.z) * st.w, w[i], b[i]);
+            R::affine(y, st.z, st.w, wb, bb, d);
             R::store((T*)A.n + at, d, y);
         }
         if (A.stats && threadIdx.x % G == 0) A.stats[row] = st;
@@ -178,17 +271,17 @@ __global__ __launch_bounds__(THREADS) void norm_gate_fwd_kernel(const NormGateAr
 
 // Adds the accumulators of a workgroup's row slots (`buf`: one row of E * G floats a wave) and hands each column's sum
 // to `put(column, value)`.  Every thread of the workgroup calls it.
-template <typename T, int G, int NV, typename Put>
-__device__ __forceinline__ void flush_columns(float (&acc)[NV * PclipVec<T>::N], float* buf, int d, Put put) {
-    using R = Row<T, G, NV>;
+template <typename T, int G, int NV, int V, int E, typename Put>
+__device__ __forceinline__ void flush_columns(float (&acc)[E], float* buf, int d, Put put) {
+    using R = Row<T, G, NV, V>;
     if constexpr (G == 256) {   // one row at a time: every column has one owner
 #pragma unroll
         for (int k = 0; k < NV; k++)
 #pragma unroll
-            for (int i = 0; i < R::V; i++)
-                if (R::col(k) + i < d) put(R::col(k) + i, acc[k * R::V + i]);
+            for (int i = 0; i < V; i++)
+                if (R::col(k) + i < d) put(R::col(k) + i, acc[k * V + i]);
     } else {
-        constexpr int W = G * NV * R::V;   // columns of a wave's row of buf
+        constexpr int W = G * E;   // columns of a wave's row of buf
         if constexpr (G == 16) {
 #pragma unroll
             for (int i = 0; i < R::E; i++) {
@@ -201,7 +294,7 @@ __device__ __forceinline__ void flush_columns(float (&acc)[NV * PclipVec<T>::N],
 #pragma unroll
             for (int k = 0; k < NV; k++)
 #pragma unroll
-                for (int i = 0; i < R::V; i++) buf[(threadIdx.x >> 6) * W + R::col(k) + i] = acc[k * R::V + i];
+                for (int i = 0; i < V; i++) buf[(threadIdx.x >> 6) * W + R::col(k) + i] = acc[k * V + i];
         __syncthreads();
         for (int c = threadIdx.x; c < d; c += THREADS) put(c, (buf[c] + buf[W + c]) + (buf[2 * W + c] + buf[3 * W + c]));
     }
@@ -209,9 +302,9 @@ __device__ __forceinline__ void flush_columns(float (&acc)[NV * PclipVec<T>::N],
     for (int i = 0; i < R::E; i++) acc[i] = 0.f;
 }
 
-template <typename T, int G, int NV>
-__global__ __launch_bounds__(THREADS) void norm_gate_bwd_kernel(const NormGateArgs A) {
-    using R = Row<T, G, NV>;
+template <typename T, int G, int NV, int V>
+__global__ __launch_bounds__(THREADS, NV * V > 12 ? 1 : 2) void norm_gate_bwd_kernel(const NormGateArgs A) {
+    using R = Row<T, G, NV, V>;
     constexpr int E = R::E;
     __shared__ float lds[4][2];
     __shared__ float buf[G == 256 ? 1 : 4 * G * E];
@@ -220,6 +313,24 @@ __global__ __launch_bounds__(THREADS) void norm_gate_bwd_kernel(const NormGateAr
     float swa[E], sba[E], swb[E], sbb[E], sg[E];
 #pragma unroll
     for (int i = 0; i < E; i++) swa[i] = sba[i] = swb[i] = sbb[i] = sg[i] = 0.f;
+    extern __shared__ __attribute__((aligned(16))) float params[];
+    typename R::Param wa, ba, wb;
+    wa.stage(A.wa, A.param_f32, d, 1.f, params);
+    ba.stage(A.ba, A.param_f32, d, 0.f, params + padded(d));
+    wb.stage(A.wb, A.param_f32, d, 1.f, params + 2 * padded(d));
+    __syncthreads();
+    const bool before = A.before && A.dn;
+    struct { typename R::Raw u, r, dy, dn; typename R::RawGate g; float4 st; } in;
+    in.st = make_float4(0.f, 1.f, 0.f, 1.f);
+    auto load = [&](int row) {
+        const size_t at = (size_t)row * d;
+        if (A.stats) in.st = A.stats[row];
+        R::load_raw(A.u, at, d, in.u);
+        if (A.dy) R::load_raw(A.dy, at, d, in.dy);
+        if (before) R::load_raw(A.dn, at, d, in.dn);
+        if (before && A.r) R::load_raw(A.r, at, d, in.r);
+        R::load_gate(A, row, in.g);
+    };
     const int g0 = A.chunks > 1 ? (int)blockIdx.x / A.chunks : (int)blockIdx.x * A.groups_per_block;
     const int g1 = A.chunks > 1 ? g0 + 1 : min(g0 + A.groups_per_block, A.groups);
     for (int grp = g0; grp < g1; grp++) {
@@ -230,56 +341,55 @@ __global__ __launch_bounds__(THREADS) void norm_gate_bwd_kernel(const NormGateAr
             first = (int)min(from, (long long)last);
             last = (int)min(from + A.chunk_rows, (long long)last);
         }
+        if (R::AHEAD && first + slot < last) load(first + slot);
         for (int row = first + slot; row < last; row += R::NG) {
+            asm volatile("" ::: "memory");   // parameters in LDS are read again for each row
             const size_t at = (size_t)row * d;
-            float u[E], t[E], g[E];
-            R::load((const T*)A.u + at, d, u);
-            const float4 st = A.stats ? A.stats[row] : make_float4(0.f, 1.f, 0.f, 1.f);
-            if (A.dy) R::load((const T*)A.dy + at, d, t);
-            else {
-#pragma unroll
-                for (int i = 0; i < E; i++) t[i] = 0.f;
-            }
-            if (A.gate_kind) R::load_gate(A, row, g);
-            else {
-#pragma unroll
-                for (int i = 0; i < E; i++) g[i] = 1.f;
-            }
-            float w[E], v[E];   // w: weight of the norm in hand; v: the value that the gate multiplies
+            float u[E], t[E], g[E], h[E], q[E];
+            if (!R::AHEAD) load(row);
+            const float4 st = in.st;
+            R::widen(in.u, u);
+            if (A.dy) R::widen(in.dy, t);
+            else R::fill(t, 0.f);
+            if (before) R::widen(in.dn, q);
+            if (before && A.r) R::widen(in.r, h);
+            else R::fill(h, 0.f);
+            R::widen_gate(A, in.g, g);
+            if (R::AHEAD && last - row > R::NG) load(row + R::NG);
+            float v[E];   // the value that the gate multiplies
             if (A.after) {
-                float b[E];
-                R::load_param(A.wa, A.param_f32, d, 1.f, w);
-                R::load_param(A.ba, A.param_f32, d, 0.f, b);
 #pragma unroll
-                for (int i = 0; i < E; i++) {
-                    u[i] = (u[i] - st.x) * st.y;   // from here on the normalised value
-                    v[i] = fmaf(u[i], w[i], b[i]);
+                for (int k = 0; k < NV; k++) {
+                    float wk[V], bk[V];
+                    wa.get(k, d, wk);
+                    ba.get(k, d, bk);
+#pragma unroll
+                    for (int j = 0; j < V; j++) {
+                        const int i = k * V + j;
+                        u[i] = (u[i] - st.x) * st.y;   // from here on the normalised value
+                        v[i] = fmaf(u[i], wk[j], bk[j]);
+                    }
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < E; i++) {
-                    w[i] = 1.f;
-                    v[i] = u[i];
-                }
+                for (int i = 0; i < E; i++) v[i] = u[i];
             }
-            if (A.before && A.dn) {
-                float h[E], q[E], wb[E];
-                if (A.r) R::load((const T*)A.r + at, d, h);
-                else {
-#pragma unroll
-                    for (int i = 0; i < E; i++) h[i] = 0.f;
-                }
-                R::load((const T*)A.dn + at, d, q);
-                R::load_param(A.wb, A.param_f32, d, 1.f, wb);
+            if (before) {
                 float m1 = 0.f, m2 = 0.f;
 #pragma unroll
-                for (int i = 0; i < E; i++) {
-                    h[i] = (fmaf(A.scale, g[i] * v[i], h[i]) - st.z) * st.w;
-                    swb[i] = fmaf(q[i], h[i], swb[i]);   // q is zero behind the row
-                    sbb[i] += q[i];
-                    q[i] *= wb[i];
-                    m1 += q[i];
-                    m2 = fmaf(q[i], h[i], m2);
+                for (int k = 0; k < NV; k++) {
+                    float wk[V];
+                    wb.get(k, d, wk);
+#pragma unroll
+                    for (int j = 0; j < V; j++) {
+                        const int i = k * V + j;
+                        h[i] = (fmaf(A.scale, g[i] * v[i], h[i]) - st.z) * st.w;
+                        swb[i] = fmaf(q[i], h[i], swb[i]);   // q is zero behind the row
+                        sbb[i] += q[i];
+                        q[i] *= wk[j];
+                        m1 += q[i];
+                        m2 = fmaf(q[i], h[i], m2);
+                    }
                 }
                 row_sum2<G>(m1, m2, lds);
                 m1 = A.before == PCLIP_NORM_LAYER ? m1 * inv : 0.f;
@@ -296,19 +406,22 @@ __global__ __launch_bounds__(THREADS) void norm_gate_bwd_kernel(const NormGateAr
             }
             float m1 = 0.f, m2 = 0.f;
 #pragma unroll
-            for (int k = 0; k < NV; k++)
+            for (int k = 0; k < NV; k++) {
+                float wk[V];
+                wa.get(k, d, wk);
 #pragma unroll
-                for (int j = 0; j < R::V; j++) {
-                    const int i = k * R::V + j;
+                for (int j = 0; j < V; j++) {
+                    const int i = k * V + j;
                     const float in = R::col(k) + j < d ? A.scale * t[i] : 0.f;   // nothing behind the row enters the sums
                     sg[i] = fmaf(v[i], in, sg[i]);
                     t[i] = g[i] * in;                                            // dv
                     swa[i] = fmaf(t[i], u[i], swa[i]);
                     sba[i] += t[i];
-                    t[i] *= w[i];
+                    t[i] *= wk[j];
                     m1 += t[i];
                     m2 = fmaf(t[i], u[i], m2);
                 }
+            }
             if (A.after) {
                 row_sum2<G>(m1, m2, lds);
                 m1 = A.after == PCLIP_NORM_LAYER ? m1 * inv : 0.f;
@@ -321,7 +434,7 @@ __global__ __launch_bounds__(THREADS) void norm_gate_bwd_kernel(const NormGateAr
         if (A.sum_gate) {
             float* to = A.part_g + ((size_t)grp * A.chunks + (A.chunks > 1 ? (int)blockIdx.x % A.chunks : 0)) * d;
             T* out = (T*)A.dg + (size_t)grp * d;
-            flush_columns<T, G, NV>(sg, buf, d, [&](int c, float s) {
+            flush_columns<T, G, NV, V>(sg, buf, d, [&](int c, float s) {
                 if (A.chunks > 1) to[c] = s;
                 else out[c] = (T)s;
             });
@@ -329,10 +442,10 @@ __global__ __launch_bounds__(THREADS) void norm_gate_bwd_kernel(const NormGateAr
     }
     if (A.part_w) {
         float* to = A.part_w + (size_t)blockIdx.x * 4 * d;
-        if (A.wanted & 1) flush_columns<T, G, NV>(swa, buf, d, [&](int c, float s) { to[c] = s; });
-        if (A.wanted & 2) flush_columns<T, G, NV>(sba, buf, d, [&](int c, float s) { to[d + c] = s; });
-        if (A.wanted & 4) flush_columns<T, G, NV>(swb, buf, d, [&](int c, float s) { to[2 * d + c] = s; });
-        if (A.wanted & 8) flush_columns<T, G, NV>(sbb, buf, d, [&](int c, float s) { to[3 * d + c] = s; });
+        if (A.wanted & 1) flush_columns<T, G, NV, V>(swa, buf, d, [&](int c, float s) { to[c] = s; });
+        if (A.wanted & 2) flush_columns<T, G, NV, V>(sba, buf, d, [&](int c, float s) { to[d + c] = s; });
+        if (A.wanted & 4) flush_columns<T, G, NV, V>(swb, buf, d, [&](int c, float s) { to[2 * d + c] = s; });
+        if (A.wanted & 8) flush_columns<T, G, NV, V>(sbb, buf, d, [&](int c, float s) { to[3 * d + c] = s; });
     }
 }
 
@@ -358,8 +471,16 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(const ColumnSumArgs A)
     const size_t stride = gate ? (size_t)d : (size_t)4 * d;
     const int count = gate ? A.chunks : A.blocks;
     float s = 0.f;
-    if (c < d)
-        for (int i = part; i < count; i += 16) s += p[i * stride + c];
+    if (c < d) {
+        float more[8] = {};
+        int i = part;
+        for (; i + 7 * 16 < count; i += 8 * 16)   // eight loads under way
+#pragma unroll
+            for (int q = 0; q < 8; q++) more[q] += p[(i + q * 16) * stride + c];
+        for (; i < count; i += 16) s += p[i * stride + c];
+#pragma unroll
+        for (int q = 0; q < 8; q++) s += more[q];
+    }
     lds[part][lane] = s;
     __syncthreads();
     if (part == 0 && c < d) {
@@ -371,15 +492,20 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(const ColumnSumArgs A)
     }
 }
 
-// Lanes and vectors of a row: the fewest lanes whose vectors hold it with at most 16 elements a lane (the backward keeps
-// five column sums of that many registers).
-struct Shape { int lanes, vectors; };
+// Lanes, vectors and their width for a row: the fewest lanes that hold it with at most 12 elements each (the backward keeps five
+// column sums of that many registers; 16 only beyond 2048, where nothing smaller holds a row), in 16-byte accesses where that
+// wastes less than half of them.
+struct Shape { int lanes, vectors, width; };
 Shape shape_of(int d, int dtype) {
-    const int V = dtype == PCLIP_DT_F32 ? 4 : 8, most = 16 / V, vecs = (d + V - 1) / V;
-    for (int lanes : {16, 64, 256})
-        for (int nv = 1; nv <= most; nv *= 2)
-            if (vecs <= lanes * nv) return {lanes, nv};
-    return {256, most};
+    const bool wide = dtype != PCLIP_DT_F32;   // 16 bytes are eight elements
+    if (d <= 64) return {16, 1, 4};
+    if (d <= 128) return wide ? Shape{16, 1, 8} : Shape{16, 2, 4};
+    if (d <= 256) return {64, 1, 4};
+    if (d <= 512) return wide ? Shape{64, 1, 8} : Shape{64, 2, 4};
+    if (d <= 768) return {64, 3, 4};
+    if (d <= 1024) return {256, 1, 4};
+    if (d <= 2048) return wide ? Shape{256, 1, 8} : Shape{256, 2, 4};
+    return wide ? Shape{256, 2, 8} : Shape{256, 4, 4};
 }
 
 // How the backward divides the rows over workgroups (see NormGateArgs).  512 workgroups, two a compute unit, are aimed
@@ -403,32 +529,30 @@ void plan(NormGateArgs& A, int dtype, bool sums, int& blocks) {
     blocks = A.chunks > 1 ? A.groups * A.chunks : (A.groups + A.groups_per_block - 1) / A.groups_per_block;
 }
 
-template <typename T, int G, int NV>
-void launch(const NormGateArgs& A, bool fwd, int blocks, hipStream_t st) {
-    if (fwd) norm_gate_fwd_kernel<T, G, NV><<<blocks, THREADS, 0, st>>>(A);
-    else norm_gate_bwd_kernel<T, G, NV><<<blocks, THREADS, 0, st>>>(A);
+template <typename T, int G, int NV, int V>
+int launch(const NormGateArgs& A, bool fwd, int blocks, hipStream_t st) {
+    static PclipLdsLimit limit[2];
+    const size_t bytes = (size_t)(fwd ? 4 : 3) * padded(A.d) * sizeof(float);
+    const int rc = pclip_ensure_lds(limit[fwd], fwd ? (const void*)&norm_gate_fwd_kernel<T, G, NV, V> : (const void*)&norm_gate_bwd_kernel<T, G, NV, V>, bytes, "norm_gate");
+    if (rc) return rc;
+    if (fwd) norm_gate_fwd_kernel<T, G, NV, V><<<blocks, THREADS, bytes, st>>>(A);
+    else norm_gate_bwd_kernel<T, G, NV, V><<<blocks, THREADS, bytes, st>>>(A);
+    return PCLIP_OK;
 }
 template <typename T>
-void launch_shape(const NormGateArgs& A, Shape s, bool fwd, int blocks, hipStream_t st) {
-    constexpr int MOST = 16 / PclipVec<T>::N;
-    const int key = s.lanes * 8 + s.vectors;
-    switch (key) {
-        case 16 * 8 + 1: launch<T, 16, 1>(A, fwd, blocks, st); break;
-        case 16 * 8 + 2: launch<T, 16, 2>(A, fwd, blocks, st); break;
-        case 64 * 8 + 1: launch<T, 64, 1>(A, fwd, blocks, st); break;
-        case 64 * 8 + 2: launch<T, 64, 2>(A, fwd, blocks, st); break;
-        case 256 * 8 + 1: launch<T, 256, 1>(A, fwd, blocks, st); break;
-        case 256 * 8 + 2: launch<T, 256, 2>(A, fwd, blocks, st); break;
-        case 16 * 8 + 4: launch<T, 16, MOST>(A, fwd, blocks, st); break;     // f32 only
-        case 64 * 8 + 4: launch<T, 64, MOST>(A, fwd, blocks, st); break;
-        case 256 * 8 + 4: launch<T, 256, MOST>(A, fwd, blocks, st); break;
-    }
-}
-void launch_type(const NormGateArgs& A, int dtype, bool fwd, int blocks, hipStream_t st) {
+int launch_type(const NormGateArgs& A, int dtype, bool fwd, int blocks, hipStream_t st) {
+    constexpr int W = PclipVec<T>::N, H = W == 8 ? 1 : 2;   // eight elements in one access or in two
     const Shape s = shape_of(A.d, dtype);
-    if (dtype == PCLIP_DT_F32) launch_shape<float>(A, s, fwd, blocks, st);
-    else if (dtype == PCLIP_DT_BF16) launch_shape<__bf16>(A, s, fwd, blocks, st);
-    else launch_shape<_Float16>(A, s, fwd, blocks, st);
+    const int each = s.vectors * s.width;
+    if (s.lanes == 16) return each == 4 ? launch<T, 16, 1, 4>(A, fwd, blocks, st) : launch<T, 16, H, W>(A, fwd, blocks, st);
+    if (s.lanes == 64)
+        return each == 4 ? launch<T, 64, 1, 4>(A, fwd, blocks, st) : each == 8 ? launch<T, 64, H, W>(A, fwd, blocks, st) : launch<T, 64, 3, 4>(A, fwd, blocks, st);
+    return each == 4 ? launch<T, 256, 1, 4>(A, fwd, blocks, st) : each == 8 ? launch<T, 256, H, W>(A, fwd, blocks, st) : launch<T, 256, 2 * H, W>(A, fwd, blocks, st);
+}
+int launch_kernel(const NormGateArgs& A, int dtype, bool fwd, int blocks, hipStream_t st) {
+    if (dtype == PCLIP_DT_F32) return launch_type<float>(A, dtype, fwd, blocks, st);
+    if (dtype == PCLIP_DT_BF16) return launch_type<__bf16>(A, dtype, fwd, blocks, st);
+    return launch_type<_Float16>(A, dtype, fwd, blocks, st);
 }
 
 int check_common(const char* who, int rows, int d, int dtype, int param_type, const void* gate, int gate_kind, int gate_rows, int after, int before,
@@ -458,8 +582,8 @@ extern "C" int pclip_norm_gate_fwd(const void* u, const void* r, const void* gat
     A.param_f32 = param_type == PCLIP_DT_F32, A.scale = scale, A.eps = eps;
     const int slots = THREADS / shape_of(d, dtype).lanes;
     const long long want = ((long long)rows + slots - 1) / slots;
-    launch_type(A, dtype, true, want < 4096 ? (int)want : 4096, (hipStream_t)stream);
-    return pclip_check_launch("norm_gate_fwd");
+    rc = launch_kernel(A, dtype, true, want < FWD_BLOCKS ? (int)want : FWD_BLOCKS, (hipStream_t)stream);
+    return rc ? rc : pclip_check_launch("norm_gate_fwd");
 }
 
 extern "C" size_t pclip_norm_gate_bwd_workspace_bytes(int rows, int d, int dtype, int gate_rows) {
@@ -495,7 +619,8 @@ extern "C" int pclip_norm_gate_bwd(const void* u, const void* r, const void* gat
     PCLIP_REQUIRE(need == 0 || (ws && ws_bytes >= need), "norm_gate_bwd: workspace too small (%zu bytes, need %zu)", ws_bytes, need);
     A.part_w = affine ? (float*)ws : nullptr;
     A.part_g = gate_parts ? (float*)ws + w_floats : nullptr;
-    launch_type(A, dtype, false, blocks, (hipStream_t)stream);
+    rc = launch_kernel(A, dtype, false, blocks, (hipStream_t)stream);
+    if (rc) return rc;
     if (affine || gate_parts) {
         ColumnSumArgs S = {};
         S.part_w = A.part_w, S.part_g = A.part_g, S.out[0] = dwa, S.out[1] = dba, S.out[2] = dwb, S.out[3] = dbb, S.dg = dgate;
