@@ -29,10 +29,10 @@ def main():
     scaler = GradScaler("cuda", enabled=False)  # the loss kernels are f32: nothing to scale
 
     def build():
-        return models.ExtendedCLIP(input_dim, embedding_dim, h1, h2, dropout, esm_model)
+        return models.ExtendedCLIP(input_dim, embedding_dim, h1, h2, dropout, esm_model, entry.TOKEN_DTYPES[args.token_dtype])
 
     def train_epoch(model, loader, optimizer):
-        return training_utils.train_gc(model, loader, tokenizer, optimizer, scaler, device, args.accumulated_batches)
+        return training_utils.train_gc(model, loader, tokenizer, optimizer, scaler, device, args.accumulated_batches, max_grad_norm=args.max_grad_norm)
 
     def evaluate(model, loader):
         return training_utils.evaluate(model, loader, tokenizer, device)

@@ -28,10 +28,10 @@ def main():
     loaders = entry.make_loaders(args, rank, pep_len=(50, args.max_len))   # both chains are proteins
 
     def build():
-        return models.ExtendedFILIP(input_dim, embedding_dim, h1, h2, dropout, esm_model)
+        return models.ExtendedFILIP(input_dim, embedding_dim, h1, h2, dropout, esm_model, entry.TOKEN_DTYPES[args.token_dtype])
 
     def train_epoch(model, loader, optimizer):
-        return training_utils_filip.train(model, loader, optimizer, tokenizer, device)
+        return training_utils_filip.train(model, loader, optimizer, tokenizer, device, max_grad_norm=args.max_grad_norm)
 
     def evaluate(model, loader):
         return training_utils_filip.evaluate(model, loader, tokenizer, device)

@@ -26,6 +26,7 @@ from . import synthetic
 from .modules import seed as seed_mod
 
 ESM_NAME = "facebook/esm2_t30_150M_UR50D"
+TOKEN_DTYPES = {"modules": None, "f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 
 
 def parse_args(defaults):
@@ -38,6 +39,9 @@ def parse_args(defaults):
     ap.add_argument("--eval-pairs", type=int, default=64, help="synthetic mode: validation / test pairs each")
     ap.add_argument("--trunk-layers", type=int, default=30, help="synthetic mode: depth of the random trunk")
     ap.add_argument("--max-len", type=int, default=254, help="synthetic mode: longest receptor")
+    ap.add_argument("--token-dtype", choices=sorted(TOKEN_DTYPES), default="modules",
+                    help="projection and per-residue network: PyTorch modules in float32, or the fused operators in a type")
+    ap.add_argument("--max-grad-norm", type=float, default=None, help="clip the global gradient norm to this before each optimizer step")
     return ap.parse_args()
 
 

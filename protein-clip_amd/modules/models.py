@@ -1,6 +1,6 @@
 """Projection heads and dual encoders with the reference's API (modules/models.py).
 
-Everything up to the head output is ordinary PyTorch-ROCm (frozen ESM trunk, Linear /
+Everything up to the head output is ordinary PyTorch-ROCm by default (frozen ESM trunk, Linear /
 LayerNorm / ReLU / Dropout).  The lines of the reference that sit on the contrastive hot path
 are replaced by HIP operators:
 
@@ -8,6 +8,8 @@ are replaced by HIP operators:
 * ``Encoder.forward`` tail, ``embedding_ffn`` and ``F.normalize(e) * exp(t/2)`` (models.py:49-51)
   -> :func:`protein_clip_amd.ops.embedding_head` (one launch; the layers stay ordinary
   ``nn.Linear`` / ``nn.LayerNorm`` modules that own the parameters);
+* with ``token_dtype=``, the projection and ``amino_acid_ffn`` (models.py:32-52, 54-73) ->
+  :func:`protein_clip_amd.ops.linear_act` and :func:`protein_clip_amd.ops.norm_gate_residual`;
 * ``ExtendedFILIP.forward`` token normalisation + ``_filip_similarity_score``
   (models.py:237-243, 292-356) -> :func:`protein_clip_amd.ops.filip_similarity`.
 
@@ -35,7 +37,30 @@ def _feed_forward(width: int, depth: int, dropout_rate: float) -> nn.Sequential:
 
 def _token_features(tower, seq):
     hidden = tower.esm_model(input_ids=seq["input_ids"], attention_mask=seq["attention_mask"]).last_hidden_state
-    return tower.amino_acid_ffn(tower.projection(hidden))
+    if tower.token_dtype is None:
+        return tower.amino_acid_ffn(tower.projection(hidden))
+    return _token_head(tower, hidden.to(tower.token_dtype)).float()
+
+
+def _token_head(tower, hidden):
+    """The projection and the per-residue network on the token-head operators, in ``hidden``'s type: bias and ReLU in the
+    products' epilogue, LayerNorm and Dropout in one pass."""
+    x = ops.linear_act(hidden, tower.projection.weight, tower.projection.bias)
+    for linear, _, norm, dropout in list(tower.amino_acid_ffn)[:-1]:
+        x = ops.linear_act(x, linear.weight, linear.bias, activation="relu")
+        keep, scale = None, 1.0
+        if tower.training and dropout.p > 0.0:   # drawn from torch's generator of this device, as in Encoder.forward
+            keep = torch.rand(x.shape, device=x.device) >= dropout.p
+            scale = 1.0 / (1.0 - dropout.p) if dropout.p < 1.0 else 0.0
+        x = ops.norm_gate_residual(x, gate=keep, scale=scale, after=(norm.weight, norm.bias), eps=norm.eps)
+    last = tower.amino_acid_ffn[-1]
+    return ops.linear_act(x, last.weight, last.bias)
+
+
+def _check_token_dtype(dtype):
+    if dtype not in (None, torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"token_dtype must be None, float32, bfloat16 or float16, got {dtype}")
+    return dtype
 
 
 def _head_layout(ffn: nn.Sequential):
@@ -67,10 +92,15 @@ def _head_layout(ffn: nn.Sequential):
 
 class Encoder(nn.Module):
     """One CLIP tower: trunk -> projection -> per-residue FFN -> masked mean -> FFN ->
-    unit-norm embedding scaled by exp(temperature / 2)."""
+    unit-norm embedding scaled by exp(temperature / 2).
 
-    def __init__(self, input_dim, embedding_dim, h1, h2, dropout_rate, esm_model):
+    ``token_dtype``: None runs projection and per-residue FFN as PyTorch modules (float32, the reference's
+    arithmetic); a type runs them on the token-head operators in that type (sums in float32, parameters and
+    their gradients stay float32)."""
+
+    def __init__(self, input_dim, embedding_dim, h1, h2, dropout_rate, esm_model, token_dtype=None):
         super().__init__()
+        self.token_dtype = _check_token_dtype(token_dtype)
         self.projection = nn.Linear(input_dim, embedding_dim)
         self.amino_acid_ffn = _feed_forward(embedding_dim, h1, dropout_rate)
         self.embedding_ffn = _feed_forward(embedding_dim, h2, dropout_rate)
@@ -100,10 +130,10 @@ class Encoder(nn.Module):
 
 
 class ExtendedCLIP(nn.Module):
-    def __init__(self, input_dim, embedding_dim, h1, h2, dropout, esm_model):
+    def __init__(self, input_dim, embedding_dim, h1, h2, dropout, esm_model, token_dtype=None):
         super().__init__()
-        self.pep_encoder = Encoder(input_dim, embedding_dim, h1, h2, dropout, esm_model)
-        self.rec_encoder = Encoder(input_dim, embedding_dim, h1, h2, dropout, esm_model)
+        self.pep_encoder = Encoder(input_dim, embedding_dim, h1, h2, dropout, esm_model, token_dtype)
+        self.rec_encoder = Encoder(input_dim, embedding_dim, h1, h2, dropout, esm_model, token_dtype)
         self.temperature = nn.Parameter(torch.tensor(1.0))
 
     def forward(self, pep_seq, rec_seq):
@@ -116,10 +146,11 @@ class ExtendedCLIP(nn.Module):
 
 class FILIPEncoder(nn.Module):
     """One FILIP tower: per-residue embeddings and the attention mask (``embedding_ffn`` is
-    built but unused, as in the reference, so checkpoints keep their keys)."""
+    built but unused, as in the reference, so checkpoints keep their keys).  ``token_dtype``: see :class:`Encoder`."""
 
-    def __init__(self, input_dim, embedding_dim, h1, h2, dropout_rate, esm_model):
+    def __init__(self, input_dim, embedding_dim, h1, h2, dropout_rate, esm_model, token_dtype=None):
         super().__init__()
+        self.token_dtype = _check_token_dtype(token_dtype)
         self.projection = nn.Linear(input_dim, embedding_dim)
         self.amino_acid_ffn = _feed_forward(embedding_dim, h1, dropout_rate)
         self.embedding_ffn = _feed_forward(embedding_dim, h2, dropout_rate)
@@ -132,10 +163,10 @@ class FILIPEncoder(nn.Module):
 
 
 class ExtendedFILIP(nn.Module):
-    def __init__(self, input_dim, embedding_dim, h1, h2, dropout, esm_model):
+    def __init__(self, input_dim, embedding_dim, h1, h2, dropout, esm_model, token_dtype=None):
         super().__init__()
-        self.pep_encoder = FILIPEncoder(input_dim, embedding_dim, h1, h2, dropout, esm_model)
-        self.rec_encoder = FILIPEncoder(input_dim, embedding_dim, h1, h2, dropout, esm_model)
+        self.pep_encoder = FILIPEncoder(input_dim, embedding_dim, h1, h2, dropout, esm_model, token_dtype)
+        self.rec_encoder = FILIPEncoder(input_dim, embedding_dim, h1, h2, dropout, esm_model, token_dtype)
         self.temperature = nn.Parameter(torch.tensor(1.0))
 
     def forward(self, pep_seq, rec_seq, group=None):

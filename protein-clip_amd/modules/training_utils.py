@@ -60,18 +60,27 @@ def _distributed() -> bool:
     return dist.is_available() and dist.is_initialized() and dist.get_world_size() > 1
 
 
-def train(model, data_loader, optimizer, tokenizer, device):
+def _finish_grads(model, max_grad_norm=None):
+    """What lies between the backward and the optimizer's step: the sum over the ranks and, when asked for, the
+    clipping of the global gradient norm (of the sum, so that every rank scales by the same factor)."""
+    if _distributed():
+        _sum_head_grads(model, max_grad_norm=max_grad_norm)
+    elif max_grad_norm is not None:
+        ops.clip_grad_norm_(model.parameters(), max_grad_norm)
+
+
+def train(model, data_loader, optimizer, tokenizer, device, max_grad_norm=None):
     """One epoch, one optimizer step per batch; returns the mean batch loss.  Under
     ``torch.distributed`` the loss of a batch spans the batches of all ranks (all-gather inside
     the loss) and every rank back-propagates its own rows, so the head gradients are summed over
-    the ranks before the step."""
+    the ranks before the step.  ``max_grad_norm``: clip the global gradient norm to this (None: no clipping,
+    as in the reference)."""
     model.train()
     running = 0.0
     for batch in data_loader:
         optimizer.zero_grad()
         running += _process_batch(model, batch, tokenizer, device, compute_grad=True)
-        if _distributed():
-            _sum_head_grads(model)
+        _finish_grads(model, max_grad_norm)
         optimizer.step()
     return running / len(data_loader)
 
@@ -122,24 +131,29 @@ def _replay(encoder, inputs, snap, rep):
     torch.autograd.backward(again, grad_tensors=rep.grad)
 
 
-def _sum_head_grads(model, group=None):
+def _sum_head_grads(model, group=None, max_grad_norm=None):
     """Every rank back-propagated the global loss through its own rows only, so the gradient
-    of a shared parameter is the SUM over ranks (one flat all-reduce)."""
+    of a shared parameter is the SUM over ranks (one flat all-reduce).  With ``max_grad_norm`` the way back from the
+    flat buffer clips as well."""
     grads = [p.grad for p in model.parameters() if p.requires_grad and p.grad is not None]
     if not grads:
         return
     flat = torch.cat([g.reshape(-1) for g in grads])
     dist.all_reduce(flat, group=group)
+    if max_grad_norm is not None:
+        ops.clip_grads([v.view(g.shape) for v, g in zip(flat.split([g.numel() for g in grads]), grads)], max_grad_norm, out=grads)
+        return
     offset = 0
     for g in grads:
         g.copy_(flat[offset:offset + g.numel()].view_as(g))
         offset += g.numel()
 
 
-def train_gc(model, data_loader, tokenizer, optimizer, scaler, device, accumulated_batches=1, group=None):
+def train_gc(model, data_loader, tokenizer, optimizer, scaler, device, accumulated_batches=1, group=None, max_grad_norm=None):
     """Big-batch epoch (training_utils.py:92-155): every ``accumulated_batches`` sub-batches
     form one contrastive batch and one optimizer step.  Trailing sub-batches that do not fill
-    a batch are encoded and dropped, as in the reference.  Returns the mean big-batch loss."""
+    a batch are encoded and dropped, as in the reference.  ``max_grad_norm``: as in :func:`train`, applied to
+    the unscaled gradients.  Returns the mean big-batch loss."""
     model.train()
     distributed = _distributed()
     total, big_batches = 0.0, 0
@@ -165,6 +179,9 @@ def train_gc(model, data_loader, tokenizer, optimizer, scaler, device, accumulat
         pending = []
         if distributed:
             _sum_head_grads(model, group)
+        if max_grad_norm is not None:
+            scaler.unscale_(optimizer)
+            ops.clip_grad_norm_(model.parameters(), max_grad_norm)
         scaler.step(optimizer)
         scaler.update()
         optimizer.zero_grad()

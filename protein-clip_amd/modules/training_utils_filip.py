@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 
 from .. import ops
-from .training_utils import _distributed, _sum_head_grads
+from .training_utils import _finish_grads
 
 
 def _contrastive_loss(logits: torch.Tensor, use_dcl: bool = False) -> torch.Tensor:
@@ -36,18 +36,18 @@ def _process_batch(model, batch_data, tokenizer, device, compute_grad=False):
     return loss.item()
 
 
-def train(model, data_loader, optimizer, tokenier, device):
+def train(model, data_loader, optimizer, tokenier, device, max_grad_norm=None):
     """One epoch, one optimizer step per batch; returns the mean batch loss.  (The fourth
     parameter keeps the reference's spelling so keyword calls stay valid.)  Under
     ``torch.distributed`` every rank back-propagates the global loss through its own rows, so the
-    head and temperature gradients are summed over the ranks before the step."""
+    head and temperature gradients are summed over the ranks before the step.  ``max_grad_norm``: clip the
+    global gradient norm to this (None: no clipping, as in the reference)."""
     model.train()
     running = 0.0
     for batch in data_loader:
         optimizer.zero_grad()
         running += _process_batch(model, batch, tokenier, device, compute_grad=True)
-        if _distributed():
-            _sum_head_grads(model)
+        _finish_grads(model, max_grad_norm)
         optimizer.step()
     return running / len(data_loader)
 

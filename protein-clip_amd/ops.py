@@ -137,6 +137,9 @@ def embedding_head(pooled: torch.Tensor, params, temperature: torch.Tensor, keep
 # --------------------------------------------------------------------------------------
 # token head: linear layers, norms around a block   (modules/models.py:54-73)
 # --------------------------------------------------------------------------------------
+ACTIVATIONS = tuple(_hip_kernels.ACTIVATIONS)
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """[..., d] -> contiguous [rows, d]."""
     t = t.contiguous()
@@ -197,7 +200,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
         raise ValueError("linear_act: the layer has no input or no output")
     if bias is not None and bias.shape != weight.shape[:1]:
         raise ValueError(f"linear_act: bias must have shape ({weight.shape[0]},), got {tuple(bias.shape)}")
-    if activation not in _hip_kernels.ACTIVATIONS:
+    if activation not in ACTIVATIONS:
         raise ValueError(f"linear_act: unknown activation {activation!r}")
     K = kernels or _hip_kernels
     weight = weight.to(x.dtype)
