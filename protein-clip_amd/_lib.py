@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_size_t, c_void_p
 
 import torch
 
@@ -63,7 +63,7 @@ _SIGNATURES = {
     "pclip_norm_gate_bwd": (c_int, [_P, _P, _P, c_int, c_int, c_float, c_int, _P, _P, c_int, _P, _P, c_int, c_float, c_int, c_int, c_int, _P, _P, _P,
                                     _P, _P, _P, _P, _P, _P, _P, _P, c_size_t, _P]),
     "pclip_grad_clip_workspace_bytes": (c_size_t, [c_int]),
-    "pclip_grad_clip": (c_int, [_P, POINTER(c_int64), POINTER(c_int), _P, POINTER(c_int), c_int, c_float, c_float, _P, _P, c_size_t, _P]),
+    "pclip_grad_clip": (c_int, [_P, _P, _P, _P, _P, c_int, c_float, c_float, _P, _P, c_size_t, _P]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -201,42 +201,36 @@ NORM_MAX_D = 4096
 MAX_ROWS = 2**31 - 2**16
 
 
-class _on:
-    """Makes ``device`` the current one for a call into the library when it is not (a launch needs the device
-    of its stream to be current)."""
-
-    def __init__(self, device):
-        self.device, self.other = device, None
-
-    def __enter__(self):
-        if torch.cuda.current_device() != self.device.index:
-            self.other = torch.cuda.device(self.device)
-            self.other.__enter__()
-
-    def __exit__(self, *exc):
-        if self.other is not None:
-            self.other.__exit__(*exc)
-        return False
+def _launch(device, entry, what: str, *args):
+    """One call into the library with ``device`` current (a launch needs the device of its stream to be)."""
+    if torch.cuda.current_device() == device.index:
+        rc = entry(*args)
+    else:
+        with torch.cuda.device(device):
+            rc = entry(*args)
+    if rc:
+        check(rc, what)
 
 
 def _operand(t, name: str, shape, dtype, device):
     """A contiguous GPU tensor of this shape, type and device (or None) -> its pointer."""
     if t is None:
         return None
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         require_gpu_tensor(t, dtype, name)
         raise _lib.PclipError(f"{name}: expected shape {tuple(shape)} on {device}, got {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _typed(t, name: str, dim: int):
-    """Element type code of a contiguous GPU tensor with ``dim`` dimensions."""
+def _typed(t, name: str):
+    """Element type code of a contiguous GPU tensor of at least one dimension."""
     code = DTYPES.get(t.dtype)
     if code is None:
         raise _lib.PclipError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
-    require_gpu_tensor(t, t.dtype, name)
-    if t.dim() != dim:
-        raise _lib.PclipError(f"{name}: expected {dim} dimensions, got shape {tuple(t.shape)}")
+    if not (t.is_cuda and t.is_contiguous()):
+        require_gpu_tensor(t, t.dtype, name)
+    if t.dim() < 1:
+        raise _lib.PclipError(f"{name}: expected at least one dimension")
     return code
 
 
@@ -246,14 +240,15 @@ def _check_rows(rows: int, what: str):
 
 
 def _linear_sizes(x, w):
-    code = _typed(x, "x", 2)
-    _typed(w, "weight", 2)
-    (M, K), N = x.shape, w.shape[0]
-    if w.dtype != x.dtype or w.shape[1] != K or w.device != x.device:
-        raise _lib.PclipError(f"linear: weight {tuple(w.shape)} {w.dtype} on {w.device} does not fit x {tuple(x.shape)} {x.dtype} on {x.device}")
-    _check_rows(M, "linear")
+    code = _typed(x, "x")
+    if w.dtype != x.dtype or w.dim() != 2 or w.shape[1] != x.shape[-1] or w.device != x.device or not w.is_contiguous():
+        raise _lib.PclipError(f"linear: weight {tuple(w.shape)} {w.dtype} on {w.device} does not fit x {tuple(x.shape)} {x.dtype} on {x.device}, "
+                              "or is not contiguous")
+    N, K = w.shape
     if not (1 <= K <= LINEAR_MAX_DIM and 1 <= N <= LINEAR_MAX_DIM):
         raise _lib.PclipError(f"linear: widths {K} -> {N} (1 to {LINEAR_MAX_DIM})")
+    M = x.numel() // K
+    _check_rows(M, "linear")
     return M, K, N, code
 
 
@@ -262,16 +257,16 @@ def _slope_type(dtype):
 
 
 def linear_fwd(x, w, bias=None, residual=None, activation: str = "none", want_slope: bool = False):
-    """``act(x @ w.T + bias) + residual`` for x [M,K], w [N,K], bias [N], residual [M,N] of one type.
-    Returns (y [M,N], slope): slope = act'(z) [M,N] when asked for (what :func:`linear_bwd` needs), else None."""
+    """``act(x @ w.T + bias) + residual`` for x [...,K], w [N,K], bias [N], residual [...,N], contiguous and of one type.
+    Returns (y [...,N], slope): slope = act'(z), shaped like y, when asked for (what :func:`linear_bwd` needs), else None."""
     M, K, N, code = _linear_sizes(x, w)
-    dev = x.device
-    b, r = _operand(bias, "bias", (N,), x.dtype, dev), _operand(residual, "residual", (M, N), x.dtype, dev)
-    y = _empty((M, N), x.dtype, dev)
-    slope = _empty((M, N), _slope_type(x.dtype), dev) if want_slope else None
-    with _on(dev):
-        check(_lib.load().pclip_linear_fwd(x.data_ptr(), w.data_ptr(), b, r, M, K, N, code, ACTIVATIONS[activation], y.data_ptr(),
-                                           slope.data_ptr() if want_slope else None, stream_of(x)), "pclip_linear_fwd")
+    dev, dtype = x.device, x.dtype
+    shape = x.shape[:-1] + (N,)
+    b, r = _operand(bias, "bias", w.shape[:1], dtype, dev), _operand(residual, "residual", shape, dtype, dev)
+    y = _empty(shape, dtype, dev)
+    slope = _empty(shape, _slope_type(dtype), dev) if want_slope else None
+    _launch(dev, _lib.load().pclip_linear_fwd, "pclip_linear_fwd", x.data_ptr(), w.data_ptr(), b, r, M, K, N, code, ACTIVATIONS[activation], y.data_ptr(),
+            slope.data_ptr() if want_slope else None, stream_of(x))
     return y, slope
 
 
@@ -280,79 +275,86 @@ def linear_bwd(x, w, dy, saved=None, saved_is_output: bool = False, activation: 
     """Returns (dx, dw, db), None where not wanted.  ``saved``: the forward's slope, or its output with
     ``saved_is_output`` (relu without a residual), None for activation "none"."""
     M, K, N, code = _linear_sizes(x, w)
-    dev, act = x.device, ACTIVATIONS[activation]
-    g = _operand(dy, "dy", (M, N), x.dtype, dev)
-    s = _operand(saved, "saved", (M, N), x.dtype if saved_is_output else _slope_type(x.dtype), dev)
+    dev, dtype, act = x.device, x.dtype, ACTIVATIONS[activation]
+    shape = x.shape[:-1] + (N,)
+    g = _operand(dy, "dy", shape, dtype, dev)
+    s = _operand(saved, "saved", shape, dtype if saved_is_output else _slope_type(dtype), dev)
     lib = _lib.load()
-    dx = _empty((M, K), x.dtype, dev) if want_dx else None
-    dw = _empty((N, K), x.dtype, dev) if want_dw else None
-    db = _empty((N,), x.dtype, dev) if want_db else None
+    dx = _empty(x.shape, dtype, dev) if want_dx else None
+    dw = _empty(w.shape, dtype, dev) if want_dw else None
+    db = _empty(w.shape[:1], dtype, dev) if want_db else None
     # scratch of the call's own (not the stream's shared buffer): a captured graph keeps it for its replays
-    ws = _empty((lib.pclip_linear_bwd_workspace_bytes(M, K, N, code, act),), torch.uint8, dev)
-    with _on(dev):
-        check(lib.pclip_linear_bwd(x.data_ptr(), w.data_ptr(), g, s, int(saved_is_output), M, K, N, code, act, ptr(dx), ptr(dw), ptr(db),
-                                   ws.data_ptr(), ws.numel(), stream_of(x)), "pclip_linear_bwd")
+    nbytes = lib.pclip_linear_bwd_workspace_bytes(M, K, N, code, act)
+    ws = _empty((nbytes,), torch.uint8, dev)
+    _launch(dev, lib.pclip_linear_bwd, "pclip_linear_bwd", x.data_ptr(), w.data_ptr(), g, s, int(saved_is_output), M, K, N, code, act, ptr(dx), ptr(dw), ptr(db),
+            ws.data_ptr(), nbytes, stream_of(x))
     return dx, dw, db
 
 
-def _norm_gate_args(u, r, gate, gate_rows, after, wa, ba, before, wb, bb):
-    code = _typed(u, "u", 2)
-    rows, d = u.shape
-    dev = u.device
-    _check_rows(rows, "norm_gate")
+def _norm_gate_args(u, r, gate, gate_rows, wa, ba, wb, bb):
+    code = _typed(u, "u")
+    dev, dtype, shape = u.device, u.dtype, u.shape
+    d = shape[-1]
     if not 1 <= d <= NORM_MAX_D:
         raise _lib.PclipError(f"norm_gate: row width {d} (1 to {NORM_MAX_D})")
-    params = [p for p in (wa, ba, wb, bb) if p is not None]
-    ptype = params[0].dtype if params else torch.float32
-    if ptype not in (torch.float32, u.dtype):
-        raise _lib.PclipError(f"norm_gate: affine parameters must be float32 or {u.dtype}, got {ptype}")
+    rows = u.numel() // d
+    _check_rows(rows, "norm_gate")
+    ptype, pw = None, []
+    for p in (wa, ba, wb, bb):
+        if p is not None:
+            if ptype is None:
+                ptype = p.dtype
+                if ptype != F32 and ptype != dtype:
+                    raise _lib.PclipError(f"norm_gate: affine parameters must be float32 or {dtype}, got {ptype}")
+            pw.append(_operand(p, "affine parameter", shape[-1:], ptype, dev))
+        else:
+            pw.append(None)
     kind = GATE_NONE
     if gate is not None:
-        kind = GATE_BYTES if gate.dtype == torch.uint8 else GATE_ROWS
-        if kind == GATE_BYTES:
-            _operand(gate, "gate", (rows, d), torch.uint8, dev)
+        if gate.dtype == torch.uint8:
+            kind = GATE_BYTES
+            _operand(gate, "gate", shape, torch.uint8, dev)
         else:
-            if gate_rows < 1 or rows % gate_rows:
-                raise _lib.PclipError(f"norm_gate: gate_rows={gate_rows} does not divide {rows} rows")
-            _operand(gate, "gate", (rows // gate_rows, d), u.dtype, dev)
-    ops = [_operand(p, n, (d,), ptype, dev) for p, n in ((wa, "wa"), (ba, "ba"), (wb, "wb"), (bb, "bb"))]
-    return (rows, d, code, kind, DTYPES[ptype], ptype, u.data_ptr(), _operand(r, "residual", (rows, d), u.dtype, dev), ptr(gate)) + tuple(ops)
+            kind = GATE_ROWS
+            if gate_rows < 1 or gate.numel() * gate_rows != rows * d or gate.shape[-1] != d:
+                raise _lib.PclipError(f"norm_gate: a gate of shape {tuple(gate.shape)} with {gate_rows} rows to each of its rows does not fit u {tuple(shape)}")
+            _operand(gate, "gate", gate.shape, dtype, dev)
+    return rows, d, code, kind, F32 if ptype is None else ptype, pw, u.data_ptr(), _operand(r, "residual", shape, dtype, dev), ptr(gate)
 
 
 def norm_gate_fwd(u, r=None, gate=None, gate_rows: int = 1, scale: float = 1.0, after=None, wa=None, ba=None, before=None, wb=None, bb=None,
                   eps: float = 1e-5, want_stats: bool = False):
-    """``y = r + scale * gate * norm_after(u)`` and ``n = norm_before(y)`` for u, r [rows,d]; gate [rows / gate_rows, d] of u's
-    type or a byte mask [rows,d]; ``after`` / ``before``: None, "layer" or "rms" with their affine vectors [d].
-    Returns (y, n or None, stats or None); ``stats`` is what :func:`norm_gate_bwd` needs."""
-    rows, d, code, kind, pcode, _, pu, pr, pg, pwa, pba, pwb, pbb = _norm_gate_args(u, r, gate, gate_rows, after, wa, ba, before, wb, bb)
+    """``y = r + scale * gate * norm_after(u)`` and ``n = norm_before(y)`` for contiguous u, r [...,d]; gate [...,d] of u's type with
+    one row for every ``gate_rows`` rows of u, or a byte mask of u's shape; ``after`` / ``before``: None, "layer" or "rms" with
+    their affine vectors [d].  Returns (y, n or None, stats or None); ``stats`` is what :func:`norm_gate_bwd` needs."""
+    rows, d, code, kind, ptype, (pwa, pba, pwb, pbb), pu, pr, pg = _norm_gate_args(u, r, gate, gate_rows, wa, ba, wb, bb)
     dev = u.device
-    y = _empty((rows, d), u.dtype, dev)
-    n = _empty((rows, d), u.dtype, dev) if before else None
+    y = _empty(u.shape, u.dtype, dev)
+    n = _empty(u.shape, u.dtype, dev) if before else None
     stats = _empty((rows, 4), F32, dev) if want_stats and (after or before) else None
-    with _on(dev):
-        check(_lib.load().pclip_norm_gate_fwd(pu, pr, pg, kind, gate_rows, scale, NORMS[after], pwa, pba, NORMS[before], pwb, pbb, pcode, eps, rows, d,
-                                              code, y.data_ptr(), ptr(n), ptr(stats), stream_of(u)), "pclip_norm_gate_fwd")
+    _launch(dev, _lib.load().pclip_norm_gate_fwd, "pclip_norm_gate_fwd", pu, pr, pg, kind, gate_rows, scale, NORMS[after], pwa, pba, NORMS[before], pwb, pbb,
+            DTYPES[ptype], eps, rows, d, code, y.data_ptr(), ptr(n), ptr(stats), stream_of(u))
     return y, n, stats
 
 
 def norm_gate_bwd(u, r, gate, gate_rows, scale, after, wa, ba, before, wb, bb, eps, stats, dy, dn, want=(True,) * 7):
     """Gradients (du, dr, dgate, dwa, dba, dwb, dbb) of :func:`norm_gate_fwd`, None where ``want`` says so or the operand is
     absent.  ``dy`` / ``dn`` may be None (zero), not both."""
-    rows, d, code, kind, pcode, ptype, pu, pr, pg, pwa, pba, pwb, pbb = _norm_gate_args(u, r, gate, gate_rows, after, wa, ba, before, wb, bb)
-    dev = u.device
-    pdy, pdn = _operand(dy, "dy", (rows, d), u.dtype, dev), _operand(dn, "dn", (rows, d), u.dtype, dev)
-    pst = _operand(stats, "stats", (rows, 4), F32, dev)
-    outs = [_empty(shape, dt, dev) if w and there else None
-            for w, there, shape, dt in zip(want, (True, r is not None, kind == GATE_ROWS, wa is not None, ba is not None, wb is not None, bb is not None),
-                                           ((rows, d), (rows, d), (rows // gate_rows, d)) + ((d,),) * 4, (u.dtype,) * 3 + (ptype,) * 4)]
+    rows, d, code, kind, ptype, (pwa, pba, pwb, pbb), pu, pr, pg = _norm_gate_args(u, r, gate, gate_rows, wa, ba, wb, bb)
+    dev, dtype, shape = u.device, u.dtype, u.shape
+    pdy, pdn = _operand(dy, "dy", shape, dtype, dev), _operand(dn, "dn", shape, dtype, dev)
+    pst = None if stats is None else _operand(stats, "stats", (rows, 4), F32, dev)
+    du = _empty(shape, dtype, dev) if want[0] else None
+    dr = _empty(shape, dtype, dev) if want[1] and r is not None else None
+    dg = _empty(gate.shape, dtype, dev) if want[2] and kind == GATE_ROWS else None
+    affine = [_empty((d,), ptype, dev) if w and p is not None else None for w, p in zip(want[3:], (pwa, pba, pwb, pbb))]
     lib = _lib.load()
-    sum_rows = gate_rows if outs[2] is not None else 0
-    nbytes = lib.pclip_norm_gate_bwd_workspace_bytes(rows, d, code, sum_rows) if sum_rows > 1 or any(o is not None for o in outs[3:]) else 0
+    sum_rows = gate_rows if dg is not None else 0
+    nbytes = lib.pclip_norm_gate_bwd_workspace_bytes(rows, d, code, sum_rows) if sum_rows > 1 or affine != [None] * 4 else 0
     ws = _empty((nbytes,), torch.uint8, dev) if nbytes else None   # the call's own, see linear_bwd
-    with _on(dev):
-        check(lib.pclip_norm_gate_bwd(pu, pr, pg, kind, gate_rows, scale, NORMS[after], pwa, pba, NORMS[before], pwb, pbb, pcode, eps, rows, d, code, pst,
-                                      pdy, pdn, *[ptr(o) for o in outs], ptr(ws), nbytes, stream_of(u)), "pclip_norm_gate_bwd")
-    return tuple(outs)
+    _launch(dev, lib.pclip_norm_gate_bwd, "pclip_norm_gate_bwd", pu, pr, pg, kind, gate_rows, scale, NORMS[after], pwa, pba, NORMS[before], pwb, pbb,
+            DTYPES[ptype], eps, rows, d, code, pst, pdy, pdn, ptr(du), ptr(dr), ptr(dg), *[ptr(o) for o in affine], ptr(ws), nbytes, stream_of(u))
+    return (du, dr, dg, *affine)
 
 
 def _dense(t) -> bool:
@@ -367,12 +369,20 @@ def _dense(t) -> bool:
     return True
 
 
-def _spans(tensors):
-    """(first byte, byte behind the last, element count, type code) of each tensor, as arrays."""
+def _spans(tensors, what: str, device):
+    """(first byte, byte behind the last, element count, type code) of each tensor, as arrays; refuses what the kernel cannot address."""
     n = len(tensors)
+    code = np.fromiter((DTYPES.get(t.dtype, -1) for t in tensors), np.int32, n)
+    if (code < 0).any() or not device.type == "cuda" or any(map(device.__ne__, (t.device for t in tensors))) or any(t.layout != torch.strided for t in tensors):
+        for i, t in enumerate(tensors):
+            if t.dtype not in DTYPES or t.device != device or not t.is_cuda or t.layout != torch.strided:
+                raise _lib.PclipError(f"grad_clip: {what} {i}: expected a dense float32, bfloat16 or float16 GPU tensor on {device}, got {t.dtype} on {t.device}")
+    if not all(map(torch.Tensor.is_contiguous, tensors)):
+        for i, t in enumerate(tensors):
+            if not _dense(t):
+                raise _lib.PclipError(f"grad_clip: {what} {i} has gaps or shared elements (strides {t.stride()} of shape {tuple(t.shape)})")
     start = np.fromiter(map(torch.Tensor.data_ptr, tensors), np.int64, n)
     count = np.fromiter(map(torch.Tensor.numel, tensors), np.int64, n)
-    code = np.fromiter((DTYPES.get(t.dtype, -1) for t in tensors), np.int32, n)
     return start, start + count * np.where(code == 0, 4, 2), count, code
 
 
@@ -391,10 +401,6 @@ def _check_disjoint(src, dst):
             raise _lib.PclipError("grad_clip: a written tensor shares memory with another tensor that is read")
 
 
-def _c_array(a, kind):
-    return a.ctypes.data_as(ctypes.POINTER(kind))
-
-
 def grad_clip(src, dst=None, max_norm: float = 0.0, eps: float = 1e-6) -> torch.Tensor:
     """Norm [1] of all elements of the tensors ``src``; with ``dst`` (tensors of the same shapes; ``src`` itself: in place)
     also ``dst = src * min(1, max_norm / (norm + eps))``.  One launch a pass for every 120 tensors."""
@@ -404,30 +410,26 @@ def grad_clip(src, dst=None, max_norm: float = 0.0, eps: float = 1e-6) -> torch.
     if not n:
         raise _lib.PclipError("grad_clip: no tensors")
     dev = src[0].device
-    for i, t in enumerate(src):
-        if t.dtype not in DTYPES or t.device != dev or not t.is_cuda or t.layout != torch.strided:
-            raise _lib.PclipError(f"grad_clip: tensor {i}: expected a dense float32, bfloat16 or float16 GPU tensor on {dev}, got {t.dtype} on {t.device}")
-        if not t.is_contiguous() and not _dense(t):
-            raise _lib.PclipError(f"grad_clip: tensor {i} has gaps or shared elements (strides {t.stride()} of shape {tuple(t.shape)})")
-    read = write = _spans(src)
+    read = write = _spans(src, "tensor", dev)
     if dst is not None:
         if not in_place:
             dst = list(dst)
             if len(dst) != n:
                 raise _lib.PclipError(f"grad_clip: {len(dst)} destinations for {n} tensors")
-            for i, (s, d) in enumerate(zip(src, dst)):
-                if d.dtype not in DTYPES or d.device != dev or d.shape != s.shape or d.layout != torch.strided or not (
-                        d.is_contiguous() and s.is_contiguous() or d.stride() == s.stride()):
-                    raise _lib.PclipError(f"grad_clip: destination {i} must have the shape, layout and device of its tensor and a supported type")
-            write = _spans(dst)
+            write = _spans(dst, "destination", dev)
+            shape, stride = torch.Tensor.size, torch.Tensor.stride
+            if any(map(torch.Size.__ne__, map(shape, src), map(shape, dst))) or any(map(tuple.__ne__, map(stride, src), map(stride, dst))):
+                for i, (s, d) in enumerate(zip(src, dst)):   # strides of dimensions of one element say nothing: contiguous tensors are alike
+                    if d.shape != s.shape or not (d.stride() == s.stride() or d.is_contiguous() and s.is_contiguous()):
+                        raise _lib.PclipError(f"grad_clip: destination {i} must have the shape and layout of its tensor")
         _check_disjoint(read, write)
     lib = _lib.load()
     norm = _empty((1,), F32, dev)
-    ws = _empty((lib.pclip_grad_clip_workspace_bytes(n),), torch.uint8, dev)   # the call's own, see linear_bwd
-    out = (_c_array(write[0], ctypes.c_void_p), _c_array(write[3], ctypes.c_int)) if dst is not None else (None, None)
-    with _on(dev):
-        check(lib.pclip_grad_clip(_c_array(read[0], ctypes.c_void_p), _c_array(read[2], ctypes.c_int64), _c_array(read[3], ctypes.c_int), *out, n, max_norm,
-                                  eps, norm.data_ptr(), ws.data_ptr(), ws.numel(), stream_of(norm)), "pclip_grad_clip")
+    nbytes = lib.pclip_grad_clip_workspace_bytes(n)
+    ws = _empty((nbytes,), torch.uint8, dev)   # the call's own, see linear_bwd
+    out = (write[0].ctypes.data, write[3].ctypes.data) if dst is not None else (None, None)
+    _launch(dev, lib.pclip_grad_clip, "pclip_grad_clip", read[0].ctypes.data, read[2].ctypes.data, read[3].ctypes.data, *out, n, max_norm, eps,
+            norm.data_ptr(), ws.data_ptr(), nbytes, stream_of(norm))
     return norm
 
 

@@ -140,19 +140,13 @@ def embedding_head(pooled: torch.Tensor, params, temperature: torch.Tensor, keep
 ACTIVATIONS = tuple(_hip_kernels.ACTIVATIONS)
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """[..., d] -> contiguous [rows, d]."""
-    t = t.contiguous()
-    return t if t.dim() == 2 else t.view(math.prod(t.shape[:-1]), t.shape[-1])
-
-
 class _LinearAct(torch.autograd.Function):
-    # operands keep their leading dimensions here: views made outside would be nodes of the graph
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, K):
         product = any(ctx.needs_input_grad[:3])
         output = activation == "relu" and residual is None   # the sign of y says where the slope is one
-        y, slope = _linear_rows(x, weight, bias, residual, activation, product and activation != "none" and not output, K)
+        x, weight = x.contiguous(), weight.contiguous()
+        y, slope = _linear_fwd(x, weight, bias, residual, activation, product and activation != "none" and not output, K)
         ctx.K, ctx.activation, ctx.output = K, activation, output
         ctx.save_for_backward(x, weight, y if output and product else slope)
         return y
@@ -166,20 +160,18 @@ class _LinearAct(torch.autograd.Function):
         if x.numel() == 0:
             dx, dw, db = torch.zeros_like(x), torch.zeros_like(weight), weight.new_zeros(weight.shape[0])
         elif need_x or need_w or need_b:
-            dx, dw, db = ctx.K.linear_bwd(_rows(x), weight.contiguous(), _rows(dy), None if saved is None else _rows(saved), ctx.output, ctx.activation,
-                                          need_x, need_w, need_b)
-            if need_x:
-                dx = dx.view(x.shape)
+            dx, dw, db = ctx.K.linear_bwd(x, weight, dy.contiguous(), saved, ctx.output, ctx.activation, need_x, need_w, need_b)
         return dx if need_x else None, dw if need_w else None, db if need_b else None, dy if need_r else None, None, None
 
 
-def _linear_rows(x, weight, bias, residual, activation, want_slope, K):
-    shape = x.shape[:-1] + weight.shape[:1]
+def _contiguous(t):
+    return None if t is None else t.contiguous()
+
+
+def _linear_fwd(x, weight, bias, residual, activation, want_slope, K):
     if x.numel() == 0:
-        return x.new_empty(shape), None
-    y, slope = K.linear_fwd(_rows(x), weight.contiguous(), None if bias is None else bias.contiguous(), None if residual is None else _rows(residual),
-                            activation, want_slope)
-    return (y, slope) if x.dim() == 2 else (y.view(shape), slope)
+        return x.new_empty(x.shape[:-1] + weight.shape[:1]), None
+    return K.linear_fwd(x.contiguous(), weight.contiguous(), _contiguous(bias), _contiguous(residual), activation, want_slope)
 
 
 def _wants_grad(*tensors) -> bool:
@@ -213,49 +205,38 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
             residual = residual.expand(shape)
     if _wants_grad(x, weight, bias, residual):
         return _LinearAct.apply(x, weight, bias, residual, activation, K)
-    return _linear_rows(x, weight, bias, residual, activation, False, K)[0]
+    return _linear_fwd(x, weight, bias, residual, activation, False, K)[0]
 
 
 class _NormGate(torch.autograd.Function):
+    # cfg: (gate_rows, scale, after, before, eps, K)
     @staticmethod
-    def forward(ctx, u, r, gate, wa, ba, wb, bb, gate_rows, scale, after, before, eps, K):
+    def forward(ctx, u, r, gate, wa, ba, wb, bb, cfg):
         ctx.set_materialize_grads(False)
-        y, n, stats = _norm_rows(u, r, gate, wa, ba, wb, bb, gate_rows, scale, after, before, eps, True, K)
-        ctx.K, ctx.cfg = K, (gate_rows, scale, after, before, eps)
+        u, r, gate, wa, ba, wb, bb = map(_contiguous, (u, r, gate, wa, ba, wb, bb))
+        y, n, stats = _norm_fwd(u, r, gate, wa, ba, wb, bb, cfg, True)
+        ctx.cfg = cfg
         ctx.save_for_backward(u, r, gate, wa, ba, wb, bb, stats)
-        return (y, n) if before else y
+        return y if n is None else (y, n)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dn=None):
         u, r, gate, wa, ba, wb, bb, stats = ctx.saved_tensors
-        gate_rows, scale, after, before, eps = ctx.cfg
+        gate_rows, scale, after, before, eps, K = ctx.cfg
         need = ctx.needs_input_grad[:7]
         if dy is None and dn is None:
-            return (None,) * 13
+            return (None,) * 8
         if u.numel() == 0:
-            return tuple(torch.zeros_like(t) if w else None for t, w in zip((u, r, gate, wa, ba, wb, bb), need)) + (None,) * 6
-        rows = lambda t: None if t is None else _rows(t)
-        flat = lambda t: None if t is None else t.contiguous()
-        grads = ctx.K.norm_gate_bwd(_rows(u), rows(r), _gate2(gate, u.shape[-1]), gate_rows, scale, after, flat(wa), flat(ba), before, flat(wb), flat(bb),
-                                    eps, stats, rows(dy), rows(dn), want=need)
-        du, dr, dg = (None if g is None else g.view(t.shape) for g, t in zip(grads[:3], (u, r, gate)))
-        return (du, dr, dg) + tuple(grads[3:]) + (None,) * 6
+            return tuple(torch.zeros_like(t) if w else None for t, w in zip((u, r, gate, wa, ba, wb, bb), need)) + (None,)
+        return K.norm_gate_bwd(u, r, gate, gate_rows, scale, after, wa, ba, before, wb, bb, eps, stats, _contiguous(dy), _contiguous(dn), need) + (None,)
 
 
-def _gate2(gate, d: int):
-    return None if gate is None else gate.contiguous().view(-1, d)
-
-
-def _norm_rows(u, r, gate, wa, ba, wb, bb, gate_rows, scale, after, before, eps, want_stats, K):
+def _norm_fwd(u, r, gate, wa, ba, wb, bb, cfg, want_stats):
+    gate_rows, scale, after, before, eps, K = cfg
     if u.numel() == 0:
         return torch.empty_like(u), torch.empty_like(u) if before else None, None
-    flat = lambda t: None if t is None else t.contiguous()
-    y, n, stats = K.norm_gate_fwd(_rows(u), None if r is None else _rows(r), _gate2(gate, u.shape[-1]), gate_rows, scale, after, flat(wa), flat(ba), before,
-                                  flat(wb), flat(bb), eps, want_stats)
-    if u.dim() != 2:
-        y, n = y.view(u.shape), n.view(u.shape) if before else None
-    return y, n, stats
+    return K.norm_gate_fwd(u, r, gate, gate_rows, scale, after, wa, ba, before, wb, bb, eps, want_stats)
 
 
 def _gate_rows(gate: torch.Tensor, lead, d: int) -> int:
@@ -314,11 +295,11 @@ def norm_gate_residual(u: torch.Tensor, residual: Optional[torch.Tensor] = None,
         residual = residual.to(u.dtype)
         if residual.shape != u.shape:
             residual = residual.expand(u.shape)
-    first, second = norm if after is not None else None, norm if before is not None else None
+    cfg = (gate_rows, float(scale), norm if after is not None else None, norm if before is not None else None, float(eps), K)
     if _wants_grad(u, residual, gate, wa, ba, wb, bb):
-        return _NormGate.apply(u, residual, gate, wa, ba, wb, bb, gate_rows, float(scale), first, second, float(eps), K)
-    y, n, _ = _norm_rows(u, residual, gate, wa, ba, wb, bb, gate_rows, float(scale), first, second, float(eps), False, K)
-    return (y, n) if second else y
+        return _NormGate.apply(u, residual, gate, wa, ba, wb, bb, cfg)
+    y, n, _ = _norm_fwd(*map(_contiguous, (u, residual, gate, wa, ba, wb, bb)), cfg, False)
+    return y if n is None else (y, n)
 
 
 # --------------------------------------------------------------------------------------

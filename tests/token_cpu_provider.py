@@ -12,12 +12,13 @@ def linear_fwd(x, w, bias=None, residual=None, activation="none", want_slope=Fal
 
 
 def linear_bwd(x, w, dy, saved=None, saved_is_output=False, activation="none", want_dx=True, want_dw=True, want_db=True):
+    flat = lambda t: t.reshape(-1, t.shape[-1])
     dz = dy if saved is None else dy * ((saved > 0).to(dy.dtype) if saved_is_output else saved)
-    return (dz @ w if want_dx else None), (dz.t() @ x if want_dw else None), (dz.sum(0) if want_db else None)
+    return (dz @ w if want_dx else None), (flat(dz).t() @ flat(x) if want_dw else None), (flat(dz).sum(0) if want_db else None)
 
 
 def _norm_gate(u, r, gate, gate_rows, scale, after, wa, ba, before, wb, bb, eps):
-    g = None if gate is None else gate.to(u.dtype).repeat_interleave(gate_rows, 0)
+    g = None if gate is None else gate.to(u.dtype).reshape(-1, u.shape[-1]).repeat_interleave(gate_rows, 0).reshape(u.shape)
     return R.norm_gate(u, r, g, scale, (wa, ba) if after else None, (wb, bb) if before else None, after or before, eps)
 
 
