@@ -83,6 +83,13 @@ def _empty(shape, dtype, device) -> torch.Tensor:
     return torch.empty(tuple(shape), dtype=dtype, device=device)
 
 
+def _empty_like(t: torch.Tensor) -> torch.Tensor:
+    """``_empty`` of a tensor's shape, type and device: half the host time of naming them."""
+    if getattr(BufferArena._tls, "cur", None) is not None:
+        return _empty(t.shape, t.dtype, t.device)
+    return torch.empty_like(t, memory_format=torch.contiguous_format) if not t.is_contiguous() else torch.empty_like(t)
+
+
 def _zeros(shape, dtype, device) -> torch.Tensor:
     return _empty(shape, dtype, device).zero_()
 
@@ -203,7 +210,7 @@ MAX_ROWS = 2**31 - 2**16
 
 def _launch(device, entry, what: str, *args):
     """One call into the library with ``device`` current (a launch needs the device of its stream to be)."""
-    if torch.cuda.current_device() == device.index:
+    if torch._C._cuda_getDevice() == device.index:
         rc = entry(*args)
     else:
         with torch.cuda.device(device):
@@ -280,8 +287,8 @@ def linear_bwd(x, w, dy, saved=None, saved_is_output: bool = False, activation: 
     g = _operand(dy, "dy", shape, dtype, dev)
     s = _operand(saved, "saved", shape, dtype if saved_is_output else _slope_type(dtype), dev)
     lib = _lib.load()
-    dx = _empty(x.shape, dtype, dev) if want_dx else None
-    dw = _empty(w.shape, dtype, dev) if want_dw else None
+    dx = _empty_like(x) if want_dx else None
+    dw = _empty_like(w) if want_dw else None
     db = _empty(w.shape[:1], dtype, dev) if want_db else None
     # scratch of the call's own (not the stream's shared buffer): a captured graph keeps it for its replays
     nbytes = lib.pclip_linear_bwd_workspace_bytes(M, K, N, code, act)
@@ -329,8 +336,8 @@ def norm_gate_fwd(u, r=None, gate=None, gate_rows: int = 1, scale: float = 1.0, 
     their affine vectors [d].  Returns (y, n or None, stats or None); ``stats`` is what :func:`norm_gate_bwd` needs."""
     rows, d, code, kind, ptype, (pwa, pba, pwb, pbb), pu, pr, pg = _norm_gate_args(u, r, gate, gate_rows, wa, ba, wb, bb)
     dev = u.device
-    y = _empty(u.shape, u.dtype, dev)
-    n = _empty(u.shape, u.dtype, dev) if before else None
+    y = _empty_like(u)
+    n = _empty_like(u) if before else None
     stats = _empty((rows, 4), F32, dev) if want_stats and (after or before) else None
     _launch(dev, _lib.load().pclip_norm_gate_fwd, "pclip_norm_gate_fwd", pu, pr, pg, kind, gate_rows, scale, NORMS[after], pwa, pba, NORMS[before], pwb, pbb,
             DTYPES[ptype], eps, rows, d, code, y.data_ptr(), ptr(n), ptr(stats), stream_of(u))
@@ -344,10 +351,10 @@ def norm_gate_bwd(u, r, gate, gate_rows, scale, after, wa, ba, before, wb, bb, e
     dev, dtype, shape = u.device, u.dtype, u.shape
     pdy, pdn = _operand(dy, "dy", shape, dtype, dev), _operand(dn, "dn", shape, dtype, dev)
     pst = None if stats is None else _operand(stats, "stats", (rows, 4), F32, dev)
-    du = _empty(shape, dtype, dev) if want[0] else None
-    dr = _empty(shape, dtype, dev) if want[1] and r is not None else None
-    dg = _empty(gate.shape, dtype, dev) if want[2] and kind == GATE_ROWS else None
-    affine = [_empty((d,), ptype, dev) if w and p is not None else None for w, p in zip(want[3:], (pwa, pba, pwb, pbb))]
+    du = _empty_like(u) if want[0] else None
+    dr = _empty_like(u) if want[1] and r is not None else None
+    dg = _empty_like(gate) if want[2] and kind == GATE_ROWS else None
+    affine = [_empty_like(p) if w and p is not None else None for w, p in zip(want[3:], (wa, ba, wb, bb))]
     lib = _lib.load()
     sum_rows = gate_rows if dg is not None else 0
     nbytes = lib.pclip_norm_gate_bwd_workspace_bytes(rows, d, code, sum_rows) if sum_rows > 1 or affine != [None] * 4 else 0

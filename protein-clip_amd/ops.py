@@ -145,7 +145,7 @@ class _LinearAct(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, activation, K):
         product = any(ctx.needs_input_grad[:3])
         output = activation == "relu" and residual is None   # the sign of y says where the slope is one
-        x, weight = x.contiguous(), weight.contiguous()
+        x, weight = _contiguous(x), _contiguous(weight)
         y, slope = _linear_fwd(x, weight, bias, residual, activation, product and activation != "none" and not output, K)
         ctx.K, ctx.activation, ctx.output = K, activation, output
         ctx.save_for_backward(x, weight, y if output and product else slope)
@@ -160,22 +160,26 @@ class _LinearAct(torch.autograd.Function):
         if x.numel() == 0:
             dx, dw, db = torch.zeros_like(x), torch.zeros_like(weight), weight.new_zeros(weight.shape[0])
         elif need_x or need_w or need_b:
-            dx, dw, db = ctx.K.linear_bwd(x, weight, dy.contiguous(), saved, ctx.output, ctx.activation, need_x, need_w, need_b)
+            dx, dw, db = ctx.K.linear_bwd(x, weight, _contiguous(dy), saved, ctx.output, ctx.activation, need_x, need_w, need_b)
         return dx if need_x else None, dw if need_w else None, db if need_b else None, dy if need_r else None, None, None
 
 
 def _contiguous(t):
-    return None if t is None else t.contiguous()
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def _linear_fwd(x, weight, bias, residual, activation, want_slope, K):
     if x.numel() == 0:
         return x.new_empty(x.shape[:-1] + weight.shape[:1]), None
-    return K.linear_fwd(x.contiguous(), weight.contiguous(), _contiguous(bias), _contiguous(residual), activation, want_slope)
+    return K.linear_fwd(_contiguous(x), _contiguous(weight), _contiguous(bias), _contiguous(residual), activation, want_slope)
 
 
 def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
@@ -195,12 +199,14 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     if activation not in ACTIVATIONS:
         raise ValueError(f"linear_act: unknown activation {activation!r}")
     K = kernels or _hip_kernels
-    weight = weight.to(x.dtype)
-    if bias is not None:
+    if weight.dtype != x.dtype:
+        weight = weight.to(x.dtype)
+    if bias is not None and bias.dtype != x.dtype:
         bias = bias.to(x.dtype)
     if residual is not None:
         shape = x.shape[:-1] + weight.shape[:1]
-        residual = residual.to(x.dtype)
+        if residual.dtype != x.dtype:
+            residual = residual.to(x.dtype)
         if residual.shape != shape:
             residual = residual.expand(shape)
     if _wants_grad(x, weight, bias, residual):
@@ -244,6 +250,8 @@ def _gate_rows(gate: torch.Tensor, lead, d: int) -> int:
     dimensions must be the operand's first ones followed by ones."""
     if gate.dim() == 0 or gate.shape[-1] != d:
         return 0
+    if gate.dim() == 1:
+        return math.prod(lead)
     dims = (1,) * (len(lead) + 1 - gate.dim()) + tuple(gate.shape[:-1])
     j = 0
     while j < len(lead) and dims[j] == lead[j]:
@@ -262,7 +270,7 @@ def norm_gate_residual(u: torch.Tensor, residual: Optional[torch.Tensor] = None,
     ``gate``: a tensor broadcastable to ``u`` (a channel's, a sequence's, an element's; with a gradient) or a bool / uint8
     dropout mask of ``u``'s shape, used with ``scale = 1 / (1 - p)``.
     Returns ``y``, or ``(y, norm(y))`` when ``before`` is given.  First derivatives only."""
-    if u.dim() < 1 or u.shape[-1] == 0 or norm not in ("layer", "rms"):
+    if u.dim() < 1 or u.shape[-1] < 1 or norm not in ("layer", "rms"):
         raise ValueError("norm_gate_residual: expected u [..., d] and norm 'layer' or 'rms'")
     if isinstance(scale, torch.Tensor):
         raise ValueError("norm_gate_residual: scale is a number (a learned scale is a gate)")
@@ -270,13 +278,16 @@ def norm_gate_residual(u: torch.Tensor, residual: Optional[torch.Tensor] = None,
     d = u.shape[-1]
     wa, ba = (None, None) if after is None else after
     wb, bb = (None, None) if before is None else before
-    types = set()
+    first = None
     for p in (wa, ba, wb, bb):
         if p is not None:
-            if tuple(p.shape) != (d,):
+            if p.shape != (d,):
                 raise ValueError(f"norm_gate_residual: affine parameters must have shape ({d},), got {tuple(p.shape)}")
-            types.add(p.dtype)
-    if types and types != {torch.float32} and types != {u.dtype}:
+            if first is None:
+                first = p.dtype
+            elif p.dtype != first:
+                first = torch.float64   # two types: all to float32
+    if first is not None and first != torch.float32 and first != u.dtype:
         wa, ba, wb, bb = (None if p is None else p.float() for p in (wa, ba, wb, bb))
     gate_rows = 1
     if gate is not None:
@@ -287,12 +298,14 @@ def norm_gate_residual(u: torch.Tensor, residual: Optional[torch.Tensor] = None,
         if gate.dtype == torch.uint8:
             gate = gate.expand(u.shape)
         else:
-            gate = gate.to(u.dtype)
-            gate_rows = _gate_rows(gate, tuple(u.shape[:-1]), d)
+            if gate.dtype != u.dtype:
+                gate = gate.to(u.dtype)
+            gate_rows = _gate_rows(gate, u.shape[:-1], d)
             if not gate_rows:   # any other broadcast is written out (also when there are no rows)
                 gate, gate_rows = gate.expand(u.shape), 1
     if residual is not None:
-        residual = residual.to(u.dtype)
+        if residual.dtype != u.dtype:
+            residual = residual.to(u.dtype)
         if residual.shape != u.shape:
             residual = residual.expand(u.shape)
     cfg = (gate_rows, float(scale), norm if after is not None else None, norm if before is not None else None, float(eps), K)
