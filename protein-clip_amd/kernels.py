@@ -376,27 +376,29 @@ def _dense(t) -> bool:
     return True
 
 
-def _spans(tensors, what: str, device):
-    """(first byte, byte behind the last, element count, type code) of each tensor, as arrays; refuses what the kernel cannot address."""
+def _spans(tensors, what: str, device, count=None):
+    """(first byte, byte behind the last, element count, type code) of each tensor, as arrays; refuses what the kernel cannot address.
+    Hundreds of tensors pass through here between a backward and its step: one C-level call a tensor and property."""
     n = len(tensors)
-    code = np.fromiter((DTYPES.get(t.dtype, -1) for t in tensors), np.int32, n)
-    if (code < 0).any() or not device.type == "cuda" or any(map(device.__ne__, (t.device for t in tensors))) or any(t.layout != torch.strided for t in tensors):
+    types = [t.dtype for t in tensors]
+    alike = all(map(torch.Tensor.is_contiguous, tensors))
+    if not (set(types) <= DTYPES.keys() and set(map(torch.Tensor.get_device, tensors)) == {device.index} and device.type == "cuda" and alike):
         for i, t in enumerate(tensors):
             if t.dtype not in DTYPES or t.device != device or not t.is_cuda or t.layout != torch.strided:
                 raise _lib.PclipError(f"grad_clip: {what} {i}: expected a dense float32, bfloat16 or float16 GPU tensor on {device}, got {t.dtype} on {t.device}")
-    if not all(map(torch.Tensor.is_contiguous, tensors)):
-        for i, t in enumerate(tensors):
             if not _dense(t):
                 raise _lib.PclipError(f"grad_clip: {what} {i} has gaps or shared elements (strides {t.stride()} of shape {tuple(t.shape)})")
+    code = np.fromiter(map(DTYPES.__getitem__, types), np.int32, n)
     start = np.fromiter(map(torch.Tensor.data_ptr, tensors), np.int64, n)
-    count = np.fromiter(map(torch.Tensor.numel, tensors), np.int64, n)
-    return start, start + count * np.where(code == 0, 4, 2), count, code
+    if count is None:
+        count = np.fromiter(map(torch.Tensor.numel, tensors), np.int64, n)
+    return start, start + count * np.where(code == 0, 4, 2), count, code, alike
 
 
 def _check_disjoint(src, dst):
     """No destination may share memory with another tensor of the call (its own source excepted): workgroups of
     different tensors run side by side."""
-    (s0, s1, count, _), (d0, d1, _, _) = src, dst
+    (s0, s1, count, *_), (d0, d1, *_) = src, dst
     order = np.argsort(d0[count > 0], kind="stable")
     first, last = d0[count > 0][order], d1[count > 0][order]
     if (last[:-1] > first[1:]).any():
@@ -423,12 +425,13 @@ def grad_clip(src, dst=None, max_norm: float = 0.0, eps: float = 1e-6) -> torch.
             dst = list(dst)
             if len(dst) != n:
                 raise _lib.PclipError(f"grad_clip: {len(dst)} destinations for {n} tensors")
-            write = _spans(dst, "destination", dev)
-            shape, stride = torch.Tensor.size, torch.Tensor.stride
-            if any(map(torch.Size.__ne__, map(shape, src), map(shape, dst))) or any(map(tuple.__ne__, map(stride, src), map(stride, dst))):
+            if [t.shape for t in src] != [t.shape for t in dst]:
+                raise _lib.PclipError("grad_clip: the destinations must have the shapes of the tensors")
+            write = _spans(dst, "destination", dev, read[2])
+            if not (read[4] and write[4]):
                 for i, (s, d) in enumerate(zip(src, dst)):   # strides of dimensions of one element say nothing: contiguous tensors are alike
-                    if d.shape != s.shape or not (d.stride() == s.stride() or d.is_contiguous() and s.is_contiguous()):
-                        raise _lib.PclipError(f"grad_clip: destination {i} must have the shape and layout of its tensor")
+                    if not (d.stride() == s.stride() or d.is_contiguous() and s.is_contiguous()):
+                        raise _lib.PclipError(f"grad_clip: destination {i} must have the layout of its tensor")
         _check_disjoint(read, write)
     lib = _lib.load()
     norm = _empty((1,), F32, dev)

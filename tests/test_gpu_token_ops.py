@@ -366,8 +366,14 @@ def test_clip_refusals(ops):
         ops.clip_grads([a[:32]], 1.0, out=[a[16:48]])
     with pytest.raises(PclipError, match="destinations"):
         ops.clip_grads([a], 1.0, out=[])
-    with pytest.raises(PclipError, match="destination 0"):
+    with pytest.raises(PclipError, match="shapes"):
         ops.clip_grads([a], 1.0, out=[torch.ones(63, device="cuda")])
+    with pytest.raises(PclipError, match="destination 0"):
+        ops.clip_grads([a.view(8, 8)], 1.0, out=[torch.ones(8, 8, device="cuda").t()])
+    with pytest.raises(PclipError, match="destination 0"):
+        ops.clip_grads([a], 1.0, out=[torch.ones(64, device="cuda").double()])
+    with pytest.raises(PclipError, match="tensor 0"):
+        ops.clip_grads([torch.eye(3, device="cuda").to_sparse()], 1.0)
     for limit in (-1.0, float("nan")):
         with pytest.raises(ValueError, match="max_norm"):
             ops.clip_grads([a], limit)
