@@ -218,7 +218,8 @@ struct GemmArgs {
     int tiles_i, tiles_j, splits;
     const void *bias, *residual;    // forward
     void *out, *slope;
-    float *slab, *row_sum;          // EPI_SLAB: [splits][I][J], [splits][I] or NULL
+    float *slab, *row_sum;          // EPI_SLAB: [splits][I][J], [splits][I]; slab NULL (one split): straight into out and slope
+    bool sum_rows;                  // EPI_SLAB: the sums over P's rows are wanted, too
 };
 
 // The rows' sums as one more column of the product, of ones: the first half of a wave's rows, or the second.  (`first` comes
@@ -256,10 +257,15 @@ __device__ __forceinline__ void finish(const GemmArgs& A, f32x4 (&acc)[FI][FJ], 
                 float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) v[e] = acc[fi][fj][e];
-                if (j < A.J) store_f32<float, 4>(A.slab + ((size_t)split * A.I + i) * A.J + j, A.J - j, v);
+                if (j >= A.J) continue;
+                if (A.slab) store_f32<float, 4>(A.slab + ((size_t)split * A.I + i) * A.J + j, A.J - j, v);
+                else if (A.out) store_f32<T, 4>((T*)A.out + (size_t)i * A.J + j, A.J - j, v);
             }
             const bool first = (threadIdx.x >> 6 & 1) == 0;   // the column of waves, see add_rows
-            if (sum_rows && lane < 16 && first == (fi < FI / 2)) A.row_sum[(size_t)split * A.I + i] = ones[fi % (FI / 2)][0];
+            if (sum_rows && lane < 16 && first == (fi < FI / 2)) {
+                if (A.slab) A.row_sum[(size_t)split * A.I + i] = ones[fi % (FI / 2)][0];
+                else ((T*)A.slope)[i] = (T)ones[fi % (FI / 2)][0];
+            }
         }
     } else {
         // 16 rows at a time through LDS (a wave's own part of it), after which a lane holds the V columns of one 16-byte access and
@@ -359,7 +365,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_kernel(const GemmArgs A)
     Frag one;
 #pragma unroll
     for (int e = 0; e < PclipVec<T>::N; e++) one[e] = (T)1.f;
-    const bool sum_rows = EPI == EPI_SLAB && A.row_sum && tj == 0;   // each column of waves half of its rows
+    const bool sum_rows = EPI == EPI_SLAB && A.sum_rows && tj == 0;   // each column of waves half of its rows
 
     fetch(k_first);
     int buf = 0;
@@ -445,7 +451,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_direct_kernel(const Gemm
     Frag one;
 #pragma unroll
     for (int e = 0; e < PclipVec<T>::N; e++) one[e] = (T)1.f;
-    const bool sum_rows = EPI == EPI_SLAB && A.row_sum && tj == 0;   // each column of waves half of its rows
+    const bool sum_rows = EPI == EPI_SLAB && A.sum_rows && tj == 0;   // each column of waves half of its rows
 
     fetch(k_first);
     for (long long k = k_first; k < k_end; k += KSTEP<T>) {
@@ -565,7 +571,7 @@ long long tiles(long long i, long long j, int bi, int bj) { return ((i + bi - 1)
 
 template <typename T, bool DIRECT, bool PK, bool QK, int EPI>
 int launch_size(const GemmArgs& A, int bi, int bj, hipStream_t st) {
-    if constexpr (DIRECT && EPI != EPI_SLAB)
+    if constexpr (DIRECT && EPI != EPI_SLAB && sizeof(T) == 2)
         if (bi == 256) return launch_tile<T, 256, 128, DIRECT, PK, QK, EPI>(A, st);
     if (bi >= 128) return launch_tile<T, 128, 128, DIRECT, PK, QK, EPI>(A, st);
     return launch_tile<T, 64, 64, DIRECT, PK, QK, EPI>(A, st);
@@ -581,23 +587,39 @@ int launch_product(const GemmArgs& A, int bi, int bj, hipStream_t st) {
     return direct<T>(A) ? launch_size<T, true, PK, QK, EPI>(A, bi, bj, st) : launch_size<T, false, PK, QK, EPI>(A, bi, bj, st);
 }
 
-// forward and dx: the largest tile that still gives every compute unit work
+// Forward and dx: the tile whose workgroups are done first.  A compute unit's share is its number of workgroups times the tile's
+// area, over what the tile reaches of the matrix cores when several share a unit (16-bit: 256 x 128 a little more than
+// 128 x 128, 64 x 64 0.62 of it: 232, 241 and 371 us for 65,536 x 640 -> 2560) and 0.6 of that for one alone, which waits for its own
+// loads (4096 x 2560 -> 640: 39 us with one 128 x 128 tile on some units, 31 with three of 64 x 64).  16,384 x 1280 -> 1280: 3 * 256 x 128
+// tiles a unit 63 us, 5 * 128 x 128 56 us.  f32 products wait for the matrix cores whatever the tile, so the smallest,
+// which divides most evenly, always wins (8192 x 640 -> 640: 61 us; 128 x 128 85).
 template <typename T, bool PK, bool QK, int EPI>
 int launch_rows(const GemmArgs& A, hipStream_t st) {
-    const int bi = tiles(A.I, A.J, 256, 128) >= 512 ? 256 : tiles(A.I, A.J, 128, 128) >= 256 ? 128 : 64;
-    return launch_product<T, PK, QK, EPI>(A, bi, bi == 64 ? 64 : 128, st);
+    if (sizeof(T) == 4) return launch_product<T, PK, QK, EPI>(A, 64, 64, st);
+    int best = 64;
+    double least = 0.0;
+    for (int bi : {64, 128, 256}) {
+        const int bj = bi == 64 ? 64 : 128;
+        const double each = (double)((tiles(A.I, A.J, bi, bj) + 255) / 256), reach = (bi == 64 ? 0.62 : bi == 128 ? 1.0 : 1.03) * (each == 1.0 ? 0.6 : 1.0);
+        const double cost = each * bi * bj / reach;
+        if (bi == 64 || cost < least) best = bi, least = cost;
+    }
+    return launch_product<T, PK, QK, EPI>(A, best, best == 64 ? 64 : 128, st);
 }
 
-// the product over the rows (dW): tile size and the number of splits
-struct RowPlan { int bi, bj, splits; long long k_split; };
+// The product over the rows (dW): tile size, the number of splits and their length.  The tile is 128 x 128, or 64 x 64 where a side is
+// no longer, and for f32 with few tiles: 16 waves then share a compute unit instead of 8 (4096 x 640 -> 128: 22 us instead
+// of 28; 16,384 x 1280 -> 1280, a hundred tiles: 658 instead of 492).
+struct RowPlan { int tile, splits; long long k_split; };
 RowPlan row_plan(int M, int K, int N, int dtype) {
-    const int step = dtype == PCLIP_DT_F32 ? 32 : 64, bj = K > 64 && N > 64 ? 128 : 64, bi = bj;
-    const long long t = tiles(N, K, bi, bj), steps = ((long long)M + step - 1) / step;
+    const bool f32 = dtype == PCLIP_DT_F32;
+    const int step = f32 ? 32 : 64, tile = K > 64 && N > 64 && !(f32 && tiles(N, K, 128, 128) <= 16) ? 128 : 64;
+    const long long t = tiles(N, K, tile, tile), steps = ((long long)M + step - 1) / step;
     long long s = 512 / t;                          // two workgroups a compute unit, in one round
     if (s > (steps + 3) / 4) s = (steps + 3) / 4;   // four steps a workgroup at least
     if (s < 1) s = 1;
     const long long per = (steps + s - 1) / s;
-    return {bi, bj, (int)((steps + per - 1) / per), per * step};
+    return {tile, (int)((steps + per - 1) / per), per * step};
 }
 
 template <typename T>
@@ -628,10 +650,15 @@ int backward(const T* x, const T* w, const T* dy, const void* saved, int is_outp
         const RowPlan p = row_plan(M, K, N, dtype);
         GemmArgs A = {};
         A.P = dz, A.Q = x, A.ldp = N, A.ldq = K, A.I = N, A.J = K, A.K = M, A.k_split = p.k_split, A.splits = p.splits;
-        A.slab = (float*)ws;
-        A.row_sum = db ? A.slab + (size_t)p.splits * N * K : nullptr;
-        const int rc = launch_product<T, false, false, EPI_SLAB>(A, p.bi, p.bj, st);
-        if (rc) return rc;
+        A.sum_rows = db != nullptr;
+        if (p.splits == 1) {
+            A.out = dw, A.slope = db;
+        } else {
+            A.slab = (float*)ws;
+            A.row_sum = A.slab + (size_t)p.splits * N * K;
+        }
+        const int rc = launch_product<T, false, false, EPI_SLAB>(A, p.tile, p.tile, st);
+        if (rc || p.splits == 1) return rc;
         const long long n = (long long)N * K;
         SlabSum S = {{A.slab, A.row_sum}, {dw, db}, {n, N}, p.splits, dw ? (int)((n + 63) / 64) : 0};
         slab_sum_kernel<T><<<S.blocks + (db ? (N + 63) / 64 : 0), 256, 0, st>>>(S);
@@ -668,19 +695,19 @@ extern "C" size_t pclip_linear_bwd_workspace_bytes(int M, int K, int N, int dtyp
     if (check_sizes("linear_bwd", M, K, N, dtype, activation)) return 0;
     const RowPlan p = row_plan(M, K, N, dtype);
     const size_t dz = activation == PCLIP_ACT_NONE ? 0 : pclip_align_up((size_t)M * N * pclip_dtype_size(dtype), 256);
-    return dz + (size_t)p.splits * N * ((size_t)K + 1) * sizeof(float);
+    return dz + (p.splits > 1 ? (size_t)p.splits * N * ((size_t)K + 1) * sizeof(float) : 0);
 }
 
 extern "C" int pclip_linear_bwd(const void* x, const void* w, const void* dy, const void* saved, int saved_is_output, int M, int K, int N, int dtype,
                                 int activation, void* dx, void* dw, void* db, void* ws, size_t ws_bytes, void* stream) {
     int rc = check_sizes("linear_bwd", M, K, N, dtype, activation);
     if (rc) return rc;
-    PCLIP_REQUIRE(dy && ws && (!dx || w) && (!dw || x), "linear_bwd: null pointer");
+    PCLIP_REQUIRE(dy && (!dx || w) && (!dw || x), "linear_bwd: null pointer");
     PCLIP_REQUIRE(x || !db, "linear_bwd: the bias gradient runs with the weight's product and needs x");
     PCLIP_REQUIRE(activation == PCLIP_ACT_NONE || saved, "linear_bwd: what the forward saved is needed");
     PCLIP_REQUIRE(!saved_is_output || activation == PCLIP_ACT_RELU, "linear_bwd: only relu's slope can be read from the output");
     const size_t need = pclip_linear_bwd_workspace_bytes(M, K, N, dtype, activation);
-    PCLIP_REQUIRE(ws_bytes >= need, "linear_bwd: workspace too small (%zu bytes, need %zu)", ws_bytes, need);
+    PCLIP_REQUIRE(need == 0 || (ws && ws_bytes >= need), "linear_bwd: workspace too small (%zu bytes, need %zu)", ws_bytes, need);
     PCLIP_REQUIRE(((uintptr_t)ws & 15) == 0, "linear_bwd: the workspace must be 16-byte aligned");
     hipStream_t st = (hipStream_t)stream;
 #define PCLIP_LINEAR_BWD(T)                                                                                                                         backward<T>((const T*)x, (const T*)w, (const T*)dy, saved, saved_is_output, M, K, N, dtype, activation, (T*)dx, (T*)dw, (T*)db, (char*)ws, st)

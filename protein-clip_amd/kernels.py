@@ -292,9 +292,9 @@ def linear_bwd(x, w, dy, saved=None, saved_is_output: bool = False, activation: 
     db = _empty(w.shape[:1], dtype, dev) if want_db else None
     # scratch of the call's own (not the stream's shared buffer): a captured graph keeps it for its replays
     nbytes = lib.pclip_linear_bwd_workspace_bytes(M, K, N, code, act)
-    ws = _empty((nbytes,), torch.uint8, dev)
+    ws = _empty((nbytes,), torch.uint8, dev) if nbytes else None
     _launch(dev, lib.pclip_linear_bwd, "pclip_linear_bwd", x.data_ptr(), w.data_ptr(), g, s, int(saved_is_output), M, K, N, code, act, ptr(dx), ptr(dw), ptr(db),
-            ws.data_ptr(), nbytes, stream_of(x))
+            ptr(ws), nbytes, stream_of(x))
     return dx, dw, db
 
 

@@ -45,11 +45,13 @@ def test_c_entry_points_reject_before_launch():
     def linear_bwd(x=one, w=one, dy=one, saved=None, is_out=0, act=0, dx=one, dw=one, db=one, ws=one, n=1 << 30):
         return lib.pclip_linear_bwd(x, w, dy, saved, is_out, 4, 8, 8, 1, act, dx, dw, db, ws, n, None)
 
-    for bad, what in ((dict(dy=None), "null pointer"), (dict(ws=None), "null pointer"), (dict(w=None), "null pointer"), (dict(x=None), "null pointer"),
+    for bad, what in ((dict(dy=None), "null pointer"), (dict(w=None), "null pointer"), (dict(x=None), "null pointer"),
                       (dict(x=None, dw=None), "needs x"), (dict(act=2), "saved is needed"), (dict(act=2, saved=one, is_out=1), "only relu"),
-                      (dict(n=16), "workspace too small"), (dict(ws=ctypes.c_void_p(72)), "16-byte aligned")):
+                      (dict(act=2, saved=one, n=16), "workspace too small"), (dict(act=2, saved=one, ws=None), "workspace too small"),
+                      (dict(ws=ctypes.c_void_p(72)), "16-byte aligned")):
         assert linear_bwd(**bad) == -1 and what in err(), bad
-    assert lib.pclip_linear_bwd_workspace_bytes(0, 8, 8, 1, 0) == 0 and lib.pclip_linear_bwd_workspace_bytes(4, 8, 8, 1, 2) > 8 * 9 * 4
+    assert lib.pclip_linear_bwd_workspace_bytes(0, 8, 8, 1, 0) == 0 and lib.pclip_linear_bwd_workspace_bytes(4, 8, 8, 1, 0) == 0
+    assert lib.pclip_linear_bwd_workspace_bytes(4, 8, 8, 1, 2) >= 4 * 8 * 2 and lib.pclip_linear_bwd_workspace_bytes(4096, 8, 8, 1, 0) > 8 * 9 * 4
 
     def norm_fwd(u=one, gate=None, kind=0, gate_rows=1, after=1, before=0, ptype=0, eps=1e-5, rows=6, d=8, dtype=1, y=one, n=None, stats=None):
         return lib.pclip_norm_gate_fwd(u, None, gate, kind, gate_rows, 1.0, after, None, None, before, None, None, ptype, eps, rows, d, dtype, y, n, stats, None)
