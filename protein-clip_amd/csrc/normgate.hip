@@ -10,8 +10,8 @@
 //   dr = dt;  dg = scale v dt;  dv = scale g dt;  du = norm_after'(dv);  dw = sum_rows d ^;  db = sum_rows d
 //
 // Bound: HBM.  Every operand is read once and every result written once; a row lives in the registers of the lanes
-// that read it (16 lanes up to 128 16-bit elements, a wave up to 1024, a workgroup up to 4096), y is made again in
-// the backward from u and r instead of being read.  Statistics, sums and y are f32; n is taken from the f32 y, not
+// that read it (16 lanes up to 128 elements, a wave up to 768, a workgroup up to 4096), y is made again in the
+// backward from u and r instead of being read.  Statistics, sums and y are f32; n is taken from the f32 y, not
 // from its rounded copy.  Column sums (affine and broadcast-gate gradients) stay in registers over a workgroup's
 // rows, then go to the workspace, one row a workgroup, and are added by a second kernel in a fixed order: no atomics.
 #include "elem.h"
@@ -90,45 +90,122 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float (*lds)[2]) {
     }
 }
 
-// The elements of one lane: NV vectors of V, vector k at column (k * G + lane) * V.
+// A row of a wave's operands as the buffer instructions see it: the first byte of the wave's first row, and how far it reaches.
+// An operand that is absent reaches nowhere: its loads give zeros and its stores vanish, as they do for lanes whose offset
+// lies outside, so neither needs a branch.
+constexpr unsigned REACH = 1u << 28, OUTSIDE = 1u << 31;   // an offset of OUTSIDE stays outside when it is divided by an element's size
+struct Span { const void* base; unsigned reach; };
+__device__ __forceinline__ Span span_of(const void* p, size_t byte) { return {p ? (const char*)p + byte : nullptr, p ? REACH : 0u}; }
+
+// BYTES (1 to 16) of a lane as whole registers
+constexpr int words(int bytes) { return bytes > 4 ? bytes / 4 : 1; }
+template <int BYTES>
+__device__ __forceinline__ void buffer_load(Span s, unsigned off, unsigned* r) {
+#ifdef __HIP_DEVICE_COMPILE__   // the host pass has no descriptors
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)s.base, 0, s.reach, 0x00020000);
+    if constexpr (BYTES == 16) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 0);
+        r[0] = v[0], r[1] = v[1], r[2] = v[2], r[3] = v[3];
+    } else if constexpr (BYTES == 8) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b64(rsrc, off, 0, 0);
+        r[0] = v[0], r[1] = v[1];
+    } else if constexpr (BYTES == 4) {
+        r[0] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, off, 0, 0);
+    } else if constexpr (BYTES == 2) {
+        r[0] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rsrc, off, 0, 0);
+    } else {
+        r[0] = (unsigned char)__builtin_amdgcn_raw_buffer_load_b8(rsrc, off, 0, 0);
+    }
+#endif
+}
+constexpr int PAST_L2 = 2;   // the nt bit: results that nobody reads back soon
+template <int BYTES>
+__device__ __forceinline__ void buffer_store(Span s, unsigned off, const unsigned* v) {
+#ifdef __HIP_DEVICE_COMPILE__
+    typedef unsigned __attribute__((ext_vector_type(4))) u4;
+    typedef unsigned __attribute__((ext_vector_type(2))) u2;
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)s.base, 0, s.reach, 0x00020000);
+    if constexpr (BYTES == 16) __builtin_amdgcn_raw_buffer_store_b128(u4{v[0], v[1], v[2], v[3]}, rsrc, off, 0, PAST_L2);
+    else if constexpr (BYTES == 8) __builtin_amdgcn_raw_buffer_store_b64(u2{v[0], v[1]}, rsrc, off, 0, PAST_L2);
+    else if constexpr (BYTES == 4) __builtin_amdgcn_raw_buffer_store_b32(v[0], rsrc, off, 0, PAST_L2);
+    else __builtin_amdgcn_raw_buffer_store_b16((unsigned short)v[0], rsrc, off, 0, PAST_L2);
+#endif
+}
+// element i of a lane's words, and the words of a lane's elements
+template <typename T, int V>
+__device__ __forceinline__ float element(const unsigned* w, int i) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, w[i]);
+    else return (float)__builtin_bit_cast(T, (unsigned short)(V == 1 ? w[i] : w[i / 2] >> (i % 2 * 16)));
+}
+template <typename T>
+__device__ __forceinline__ unsigned bits(float x) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(unsigned, x);
+    else return __builtin_bit_cast(unsigned short, (T)x);
+}
+
+// The elements of one lane: NV vectors of V, vector k at column (k * G + lane) * V.  V is one where rows do not divide into vectors
+// or an operand is not aligned to one.
 template <typename T, int G, int NV, int V>
 struct Row {
-    static constexpr int E = NV * V, NG = THREADS / G;
+    static constexpr int E = NV * V, NG = THREADS / G, ROWS = G < 64 ? 64 / G : 1, BYTES = V * (int)sizeof(T);   // ROWS: of a wave
+    static constexpr int W = words(BYTES), WB = words(V);   // registers of a vector, and of a byte mask's
     // whether a row is loaded while the one before it is worked on: two waves a SIMD do not cover the memory's latency by
-    // themselves; rows of many f32 would not fit the registers
-    static constexpr bool AHEAD = E * sizeof(T) <= 32;
-    struct Raw { PclipPack<T, V> v[NV]; };
-    static __device__ __forceinline__ void load_raw(const void* base, size_t at, int d, Raw& r) {
-        const T* p = (const T*)base + at;
+    // themselves; rows of many registers would not fit twice
+    static constexpr bool AHEAD = NV * W <= 8;
+    static __device__ __forceinline__ int col(int k) { return (k * G + (int)(threadIdx.x % G)) * V; }
+    static __device__ __forceinline__ int in_wave() { return G < 64 ? (int)(threadIdx.x & 63) / G : 0; }
+    // byte offsets of the lane's vectors from the wave's first row
+    static __device__ __forceinline__ void offsets(int d, unsigned (&off)[NV]) {
+#pragma unroll
+        for (int k = 0; k < NV; k++) off[k] = col(k) < d ? (unsigned)(in_wave() * d + col(k)) * (unsigned)sizeof(T) : OUTSIDE;
+    }
+    static __device__ __forceinline__ void load(Span s, const unsigned (&off)[NV], unsigned skip, unsigned (&r)[NV * W]) {
+#pragma unroll
+        for (int k = 0; k < NV; k++) buffer_load<BYTES>(s, off[k] | skip, r + k * W);
+    }
+    static __device__ __forceinline__ void store(Span s, const unsigned (&off)[NV], unsigned skip, const float (&x)[E]) {
 #pragma unroll
         for (int k = 0; k < NV; k++) {
-            const int valid = d - col(k);
-            if (valid >= V) {
-                r.v[k] = *(const PclipPack<T, V>*)(p + col(k));
-            } else {
+            unsigned v[W];
 #pragma unroll
-                for (int i = 0; i < V; i++) r.v[k].v[i] = i < valid ? p[col(k) + i] : (T)0.f;
-            }
+            for (int i = 0; i < W; i++) v[i] = BYTES / W == 4 && sizeof(T) == 2 ? bits<T>(x[k * V + 2 * i]) | bits<T>(x[k * V + 2 * i + 1]) << 16 : bits<T>(x[k * V + i]);
+            buffer_store<BYTES>(s, off[k] | skip, v);
         }
     }
-    static __device__ __forceinline__ void widen(const Raw& r, float (&x)[E]) {
+    static __device__ __forceinline__ void widen(const unsigned (&r)[NV * W], float (&x)[E]) {
 #pragma unroll
-        for (int i = 0; i < E; i++) x[i] = (float)r.v[i / V].v[i % V];
+        for (int i = 0; i < E; i++) x[i] = element<T, V>(r + i / V * W, i % V);
     }
     static __device__ __forceinline__ void fill(float (&x)[E], float v) {
 #pragma unroll
         for (int i = 0; i < E; i++) x[i] = v;
     }
-    static __device__ __forceinline__ int col(int k) { return (k * G + (int)(threadIdx.x % G)) * V; }
-    template <typename S>
-    static __device__ __forceinline__ void load(const S* p, int d, float (&x)[E]) {
+    // a row of the gate: values of T, or bytes (nonzero = 1)
+    struct Gate { unsigned t[NV * W], b[NV * WB]; };
+    static __device__ __forceinline__ void load_gate(const NormGateArgs& A, int row0, const unsigned (&off)[NV], unsigned skip, Gate& r) {
+        if (A.gate_kind == PCLIP_GATE_BYTES) {
+            const Span s = span_of(A.gate, (size_t)row0 * A.d);
 #pragma unroll
-        for (int k = 0; k < NV; k++) load_f32<S, V>(p + col(k), d - col(k), *(float(*)[V])(x + k * V));
+            for (int k = 0; k < NV; k++) buffer_load<V>(s, (off[k] | skip) / (unsigned)sizeof(T), r.b + k * WB);
+        } else if (A.gate_kind == PCLIP_GATE_ROWS) {
+            const unsigned first = A.gate_rows == 1 ? (unsigned)row0 : (unsigned)row0 / (unsigned)A.gate_rows;
+            const Span s = span_of(A.gate, (size_t)first * A.d * sizeof(T));
+            unsigned back = 0;   // the lane's gate row may be an earlier one than its own row's place from the wave's first
+            if (ROWS > 1 && A.gate_rows > 1)
+                back = (unsigned)(in_wave() - (int)((unsigned)(row0 + in_wave()) / (unsigned)A.gate_rows - first)) * (unsigned)A.d * (unsigned)sizeof(T);
+#pragma unroll
+            for (int k = 0; k < NV; k++) buffer_load<BYTES>(s, (off[k] | skip) >= OUTSIDE ? OUTSIDE : off[k] - back, r.t + k * W);
+        }
     }
-    template <typename S>
-    static __device__ __forceinline__ void store(S* p, int d, const float (&x)[E]) {
+    static __device__ __forceinline__ void widen_gate(const NormGateArgs& A, const Gate& r, float (&g)[E]) {
+        if (A.gate_kind == PCLIP_GATE_BYTES) {
 #pragma unroll
-        for (int k = 0; k < NV; k++) stream_f32<S, V>(p + col(k), d - col(k), *(const float(*)[V])(x + k * V));
+            for (int i = 0; i < E; i++) g[i] = r.b[i / V * WB + i % V / 4] >> (i % V % 4 * 8) & 255u ? 1.f : 0.f;
+        } else if (A.gate_kind == PCLIP_GATE_ROWS) {
+            widen(r.t, g);
+        } else {
+            fill(g, 1.f);
+        }
     }
     // Affine parameters.  Lanes that take row after row of one place keep theirs in registers when each has a place of its own
     // (G = 256); waves that share the places read them from LDS, as f32 padded to whole vectors, again for each row: in
@@ -152,49 +229,22 @@ struct Row {
             return !p || c >= d ? other : f32 ? ((const float*)p)[c] : (float)((const T*)p)[c];
         }
         __device__ __forceinline__ void get(int k, int d, float (&x)[V]) const {
+            if constexpr (OWN) {
 #pragma unroll
-            for (int i = 0; i < V; i += 4) {
-                if constexpr (OWN) {
+                for (int i = 0; i < V; i++) x[i] = own[k * V + i];
+            } else if constexpr (V == 1) {
+                x[0] = lds[col(k) < d ? col(k) : 0];   // lanes behind the row use any
+            } else {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) x[i + j] = own[k * V + i + j];
-                } else {
+                for (int i = 0; i < V; i += 4) {
                     const int c = col(k) + i;
-                    const f32x4 v = *(const f32x4*)(lds + (c < d ? c : 0));   // lanes behind the row use any
+                    const f32x4 v = *(const f32x4*)(lds + (c < d ? c : 0));
 #pragma unroll
                     for (int j = 0; j < 4; j++) x[i + j] = v[j];
                 }
             }
         }
     };
-    // a row of the gate: values of T, or bytes (nonzero = 1)
-    struct RawGate { Raw t; PclipPack<uint8_t, V> b[NV]; };
-    static __device__ __forceinline__ void load_gate(const NormGateArgs& A, int row, RawGate& r) {
-        if (A.gate_kind == PCLIP_GATE_BYTES) {
-            const uint8_t* p = (const uint8_t*)A.gate + (size_t)row * A.d;
-#pragma unroll
-            for (int k = 0; k < NV; k++) {
-                const int valid = A.d - col(k);
-                if (valid >= V) {
-                    r.b[k] = *(const PclipPack<uint8_t, V>*)(p + col(k));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; i++) r.b[k].v[i] = i < valid ? p[col(k) + i] : 0;
-                }
-            }
-        } else if (A.gate_kind == PCLIP_GATE_ROWS) {
-            load_raw(A.gate, (size_t)((unsigned)row / (unsigned)A.gate_rows) * A.d, A.d, r.t);
-        }
-    }
-    static __device__ __forceinline__ void widen_gate(const NormGateArgs& A, const RawGate& r, float (&g)[E]) {
-        if (A.gate_kind == PCLIP_GATE_BYTES) {
-#pragma unroll
-            for (int i = 0; i < E; i++) g[i] = r.b[i / V].v[i % V] ? 1.f : 0.f;
-        } else if (A.gate_kind == PCLIP_GATE_ROWS) {
-            widen(r.t, g);
-        } else {
-            fill(g, 1.f);
-        }
-    }
     static __device__ __forceinline__ void affine(float (&x)[E], float mean, float rstd, const Param& w, const Param& b, int d) {
 #pragma unroll
         for (int k = 0; k < NV; k++) {
@@ -219,13 +269,14 @@ struct Row {
         q = 0.f;
         s = 0.f;
 #pragma unroll
-        for (int k = 0; k < NV; k++)
+        for (int k = 0; k < NV; k++) {
+            const float m = col(k) < d ? mean : 0.f;   // nothing behind the row is off its mean
 #pragma unroll
-            for (int i = 0; i < V; i++)
-                if (col(k) + i < d) {
-                    const float c = x[k * V + i] - mean;
-                    q = fmaf(c, c, q);
-                }
+            for (int i = 0; i < V; i++) {
+                const float c = x[k * V + i] - m;
+                q = fmaf(c, c, q);
+            }
+        }
         row_sum2<G>(q, s, lds);
         rstd = 1.f / sqrtf(q * inv + eps);
     }
@@ -236,7 +287,7 @@ __global__ __launch_bounds__(THREADS) void norm_gate_fwd_kernel(const NormGateAr
     using R = Row<T, G, NV, V>;
     constexpr int E = R::E;
     __shared__ float lds[4][2];
-    const int d = A.d;
+    const int d = A.d, rows = A.rows;
     extern __shared__ __attribute__((aligned(16))) float params[];
     typename R::Param wa, ba, wb, bb;
     wa.stage(A.wa, A.param_f32, d, 1.f, params);
@@ -244,44 +295,47 @@ __global__ __launch_bounds__(THREADS) void norm_gate_fwd_kernel(const NormGateAr
     wb.stage(A.wb, A.param_f32, d, 1.f, params + 2 * padded(d));
     bb.stage(A.bb, A.param_f32, d, 0.f, params + 3 * padded(d));
     __syncthreads();
-    struct { typename R::Raw u, r; typename R::RawGate g; } in;
-    auto load = [&](int row) {
-        R::load_raw(A.u, (size_t)row * d, d, in.u);
-        if (A.r) R::load_raw(A.r, (size_t)row * d, d, in.r);
-        R::load_gate(A, row, in.g);
+    unsigned off[NV];
+    R::offsets(d, off);
+    unsigned in_u[NV * R::W], in_r[NV * R::W];   // a row as it was read
+    typename R::Gate in_g;
+    auto skip = [&](int row0) { return R::ROWS > 1 && rows - row0 <= R::in_wave() ? OUTSIDE : 0u; };
+    auto load = [&](int row0) {
+        const size_t at = (size_t)row0 * d * sizeof(T);
+        R::load(span_of(A.u, at), off, skip(row0), in_u);
+        R::load(span_of(A.r, at), off, skip(row0), in_r);
+        R::load_gate(A, row0, off, skip(row0), in_g);
     };
     const int stride = gridDim.x * R::NG;
-    int row = blockIdx.x * R::NG + (int)threadIdx.x / G;
-    if (R::AHEAD && row < A.rows) load(row);
-    for (; row < A.rows; row += stride) {
+    int row0 = blockIdx.x * R::NG + (G == 256 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * R::ROWS);
+    if (R::AHEAD && row0 < rows) load(row0);
+    for (; row0 < rows; row0 += stride) {
         asm volatile("" ::: "memory");   // parameters in LDS are read again for each row
-        const size_t at = (size_t)row * d;
         float u[E], y[E], g[E];
-        if (!R::AHEAD) load(row);
-        R::widen(in.u, u);
-        if (A.r) R::widen(in.r, y);
-        else R::fill(y, 0.f);
-        R::widen_gate(A, in.g, g);
-        if (R::AHEAD && A.rows - row > stride) load(row + stride);
+        if (!R::AHEAD) load(row0);
+        R::widen(in_u, u);
+        R::widen(in_r, y);
+        R::widen_gate(A, in_g, g);
+        if (R::AHEAD && rows - row0 > stride) load(row0 + stride);
         float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
         if (A.after) {
             R::stats(u, A.after, d, A.eps, st.x, st.y, lds);
             R::affine(u, st.x, st.y, wa, ba, d);
         }
 #pragma unroll
-        for (int k = 0; k < NV; k++)
+        for (int k = 0; k < NV; k++) {
+            const float scale = R::col(k) < d ? A.scale : 0.f;
 #pragma unroll
-            for (int j = 0; j < V; j++) {
-                const int i = k * V + j;
-                y[i] = R::col(k) + j < d ? fmaf(A.scale, u[i] * g[i], y[i]) : 0.f;
-            }
-        R::store((T*)A.y + at, d, y);
+            for (int i = 0; i < V; i++) y[k * V + i] = fmaf(scale, u[k * V + i] * g[k * V + i], y[k * V + i]);
+        }
+        const size_t at = (size_t)row0 * d * sizeof(T);
+        R::store(span_of(A.y, at), off, skip(row0), y);
         if (A.before) {
             R::stats(y, A.before, d, A.eps, st.z, st.w, lds);
             R::affine(y, st.z, st.w, wb, bb, d);
-            R::store((T*)A.n + at, d, y);
+            R::store(span_of(A.n, at), off, skip(row0), y);
         }
-        if (A.stats && threadIdx.x % G == 0) A.stats[row] = st;
+        if (A.stats && threadIdx.x % G == 0 && !skip(row0)) A.stats[row0 + R::in_wave()] = st;
     }
 }
 
@@ -324,7 +378,7 @@ __global__ __launch_bounds__(THREADS, NV * V > 12 ? 1 : 2) void norm_gate_bwd_ke
     constexpr int E = R::E;
     __shared__ float lds[4][2];
     __shared__ float buf[G == 256 ? 1 : 4 * G * E];
-    const int d = A.d, slot = (int)threadIdx.x / G;
+    const int d = A.d;
     const float inv = 1.f / (float)d;
     float swa[E], sba[E], swb[E], sbb[E], sg[E];
 #pragma unroll
@@ -336,42 +390,53 @@ __global__ __launch_bounds__(THREADS, NV * V > 12 ? 1 : 2) void norm_gate_bwd_ke
     wb.stage(A.wb, A.param_f32, d, 1.f, params + 2 * padded(d));
     __syncthreads();
     const bool before = A.before && A.dn;
-    struct { typename R::Raw u, r, dy, dn; typename R::RawGate g; float4 st; } in;
-    in.st = make_float4(0.f, 1.f, 0.f, 1.f);
-    auto load = [&](int row) {
-        const size_t at = (size_t)row * d;
-        if (A.stats) in.st = A.stats[row];
-        R::load_raw(A.u, at, d, in.u);
-        if (A.dy) R::load_raw(A.dy, at, d, in.dy);
-        if (before) R::load_raw(A.dn, at, d, in.dn);
-        if (before && A.r) R::load_raw(A.r, at, d, in.r);
-        R::load_gate(A, row, in.g);
+    unsigned off[NV];
+    R::offsets(d, off);
+    unsigned in_u[NV * R::W], in_r[NV * R::W], in_dy[NV * R::W], in_dn[NV * R::W];   // a row as it was read
+    typename R::Gate in_g;
+    float4 in_st;
+    int first = 0, last = 0;
+    auto skip = [&](int row0) { return R::ROWS > 1 && last - row0 <= R::in_wave() ? OUTSIDE : 0u; };
+    auto load = [&](int row0) {
+        const size_t at = (size_t)row0 * d * sizeof(T);
+        const unsigned s = skip(row0);
+        in_st = make_float4(0.f, 1.f, 0.f, 1.f);
+        if (A.stats && !s) in_st = A.stats[row0 + R::in_wave()];
+        R::load(span_of(A.u, at), off, s, in_u);
+        R::load(span_of(A.dy, at), off, s, in_dy);
+        if (before) {
+            R::load(span_of(A.dn, at), off, s, in_dn);
+            R::load(span_of(A.r, at), off, s, in_r);
+        }
+        R::load_gate(A, row0, off, s, in_g);
     };
     const int g0 = A.chunks > 1 ? (int)blockIdx.x / A.chunks : (int)blockIdx.x * A.groups_per_block;
     const int g1 = A.chunks > 1 ? g0 + 1 : min(g0 + A.groups_per_block, A.groups);
     for (int grp = g0; grp < g1; grp++) {
         // (group + 1) * group_rows <= rows: no overflow
-        int first = grp * A.group_rows, last = first + A.group_rows;
+        first = grp * A.group_rows, last = first + A.group_rows;
         if (A.chunks > 1) {
             const long long from = first + (long long)((int)blockIdx.x % A.chunks) * A.chunk_rows;
             first = (int)min(from, (long long)last);
             last = (int)min(from + A.chunk_rows, (long long)last);
         }
-        if (R::AHEAD && first + slot < last) load(first + slot);
-        for (int row = first + slot; row < last; row += R::NG) {
+        int row0 = first + (G == 256 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * R::ROWS);
+        if (R::AHEAD && row0 < last) load(row0);
+        for (; row0 < last; row0 += R::NG) {
             asm volatile("" ::: "memory");   // parameters in LDS are read again for each row
-            const size_t at = (size_t)row * d;
             float u[E], t[E], g[E], h[E], q[E];
-            if (!R::AHEAD) load(row);
-            const float4 st = in.st;
-            R::widen(in.u, u);
-            if (A.dy) R::widen(in.dy, t);
-            else R::fill(t, 0.f);
-            if (before) R::widen(in.dn, q);
-            if (before && A.r) R::widen(in.r, h);
-            else R::fill(h, 0.f);
-            R::widen_gate(A, in.g, g);
-            if (R::AHEAD && last - row > R::NG) load(row + R::NG);
+            if (!R::AHEAD) load(row0);
+            const float4 st = in_st;
+            R::widen(in_u, u);
+            R::widen(in_dy, t);
+            if (before) {
+                R::widen(in_dn, q);
+                R::widen(in_r, h);
+            }
+            R::widen_gate(A, in_g, g);
+            if (R::AHEAD && last - row0 > R::NG) load(row0 + R::NG);
+            const size_t at = (size_t)row0 * d * sizeof(T);
+            const unsigned s = skip(row0);
             float v[E];   // the value that the gate multiplies
             if (A.after) {
 #pragma unroll
@@ -413,22 +478,23 @@ __global__ __launch_bounds__(THREADS, NV * V > 12 ? 1 : 2) void norm_gate_bwd_ke
 #pragma unroll
                 for (int i = 0; i < E; i++) t[i] = fmaf(st.w, q[i] - m1 - h[i] * m2, t[i]);
             }
-            if (A.dr) R::store((T*)A.dr + at, d, t);
+            R::store(span_of(A.dr, at), off, s, t);
             if (A.dg && !A.sum_gate) {
                 float e[E];
 #pragma unroll
                 for (int i = 0; i < E; i++) e[i] = A.scale * v[i] * t[i];
-                R::store((T*)A.dg + at, d, e);
+                R::store(span_of(A.dg, at), off, s, e);
             }
             float m1 = 0.f, m2 = 0.f;
 #pragma unroll
             for (int k = 0; k < NV; k++) {
                 float wk[V];
                 wa.get(k, d, wk);
+                const float scale = R::col(k) < d ? A.scale : 0.f;   // nothing behind the row enters the sums
 #pragma unroll
                 for (int j = 0; j < V; j++) {
                     const int i = k * V + j;
-                    const float in = R::col(k) + j < d ? A.scale * t[i] : 0.f;   // nothing behind the row enters the sums
+                    const float in = scale * t[i];
                     sg[i] = fmaf(v[i], in, sg[i]);
                     t[i] = g[i] * in;                                            // dv
                     swa[i] = fmaf(t[i], u[i], swa[i]);
@@ -445,7 +511,7 @@ __global__ __launch_bounds__(THREADS, NV * V > 12 ? 1 : 2) void norm_gate_bwd_ke
 #pragma unroll
                 for (int i = 0; i < E; i++) t[i] = st.y * (t[i] - m1 - u[i] * m2);
             }
-            if (A.du) R::store((T*)A.du + at, d, t);
+            R::store(span_of(A.du, at), off, s, t);
         }
         if (A.sum_gate) {
             float* to = A.part_g + ((size_t)grp * A.chunks + (A.chunks > 1 ? (int)blockIdx.x % A.chunks : 0)) * d;
@@ -555,15 +621,30 @@ int launch(const NormGateArgs& A, bool fwd, int blocks, hipStream_t st) {
     else norm_gate_bwd_kernel<T, G, NV, V><<<blocks, THREADS, bytes, st>>>(A);
     return PCLIP_OK;
 }
+template <typename T, int V8>
+int launch_width(const NormGateArgs& A, const Shape& s, bool fwd, int blocks, hipStream_t st) {
+    // V8: elements of an access of eight; four go in one access, or one by one
+    constexpr int V4 = V8 == 1 ? 1 : 4;
+    const int each = s.vectors * s.width;
+    if (s.lanes == 16) return each == 4 ? launch<T, 16, 4 / V4, V4>(A, fwd, blocks, st) : launch<T, 16, 8 / V8, V8>(A, fwd, blocks, st);
+    if (s.lanes == 64)
+        return each == 4 ? launch<T, 64, 4 / V4, V4>(A, fwd, blocks, st)
+                         : each == 8 ? launch<T, 64, 8 / V8, V8>(A, fwd, blocks, st) : launch<T, 64, 12 / V4, V4>(A, fwd, blocks, st);
+    return each == 4 ? launch<T, 256, 4 / V4, V4>(A, fwd, blocks, st)
+                     : each == 8 ? launch<T, 256, 8 / V8, V8>(A, fwd, blocks, st) : launch<T, 256, 16 / V8, V8>(A, fwd, blocks, st);
+}
+// whether every row of every operand begins at a multiple of its vectors' width
+template <typename T>
+bool in_vectors(const NormGateArgs& A, const Shape& s) {
+    const bool bytes = A.gate_kind == PCLIP_GATE_BYTES;
+    uintptr_t bits = (uintptr_t)A.u | (uintptr_t)A.r | (uintptr_t)A.y | (uintptr_t)A.n | (uintptr_t)A.dy | (uintptr_t)A.dn | (uintptr_t)A.du | (uintptr_t)A.dr |
+                     (uintptr_t)A.dg | (bytes ? (uintptr_t)A.gate * sizeof(T) : (uintptr_t)A.gate);
+    return bits % (s.width * sizeof(T)) == 0 && A.d % s.width == 0;
+}
 template <typename T>
 int launch_type(const NormGateArgs& A, int dtype, bool fwd, int blocks, hipStream_t st) {
-    constexpr int W = PclipVec<T>::N, H = W == 8 ? 1 : 2;   // eight elements in one access or in two
     const Shape s = shape_of(A.d, dtype);
-    const int each = s.vectors * s.width;
-    if (s.lanes == 16) return each == 4 ? launch<T, 16, 1, 4>(A, fwd, blocks, st) : launch<T, 16, H, W>(A, fwd, blocks, st);
-    if (s.lanes == 64)
-        return each == 4 ? launch<T, 64, 1, 4>(A, fwd, blocks, st) : each == 8 ? launch<T, 64, H, W>(A, fwd, blocks, st) : launch<T, 64, 3, 4>(A, fwd, blocks, st);
-    return each == 4 ? launch<T, 256, 1, 4>(A, fwd, blocks, st) : each == 8 ? launch<T, 256, H, W>(A, fwd, blocks, st) : launch<T, 256, 2 * H, W>(A, fwd, blocks, st);
+    return in_vectors<T>(A, s) ? launch_width<T, PclipVec<T>::N>(A, s, fwd, blocks, st) : launch_width<T, 1>(A, s, fwd, blocks, st);
 }
 int launch_kernel(const NormGateArgs& A, int dtype, bool fwd, int blocks, hipStream_t st) {
     if (dtype == PCLIP_DT_F32) return launch_type<float>(A, dtype, fwd, blocks, st);
