@@ -14,16 +14,17 @@
 // backward from u and r instead of being read.  Statistics, sums and y are f32; n is taken from the f32 y, not
 // from its rounded copy.  Column sums (affine and broadcast-gate gradients) stay in registers over a workgroup's
 // rows, then go to the workspace, one row a workgroup, and are added by a second kernel in a fixed order: no atomics.
+// Operands are reached through buffer descriptors, for which a place outside a row, or an operand that is not there, is an
+// offset out of reach and no branch: with branches round every access, and the scalar registers their masks took, the
+// waves spent more time on those than on the rows (45 -> 32 us forward, 113 -> 54 us backward for 32,768 x 640 bf16 with
+// gate, residual and both norms; 168 and 252 MB, that is 5.3 and 4.7 TB/s).
 #include "elem.h"
 
 namespace {
 
 constexpr int THREADS = 256;
 constexpr int MAX_D = PCLIP_NORM_MAX_D;
-#ifndef FB
-#define FB 1024
-#endif
-constexpr int FWD_BLOCKS = FB;   // four workgroups a compute unit, which then take row after row
+constexpr int FWD_BLOCKS = 1024;   // four workgroups a compute unit, which then take row after row
 
 struct NormGateArgs {
     const void *u, *r, *gate;
@@ -46,7 +47,7 @@ struct NormGateArgs {
 __host__ __device__ __forceinline__ int padded(int d) { return (d + 3) & ~3; }
 
 // every lane's value plus those of the three lanes at its place in the other rows of 16, by exchanging rows between two
-// registers (no trip through LDS)
+// registers: no trip through LDS, which costs 2 to 4 % of the wide rows' backward
 __device__ __forceinline__ float add_rows_of_16(float v) {
 #ifdef __HIP_DEVICE_COMPILE__
     const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -68,13 +69,7 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float (*lds)[2]) {
     PCLIP_DPP_ADD2(0x141);
     PCLIP_DPP_ADD2(0x140);
 #undef PCLIP_DPP_ADD2
-    if constexpr (G == 64) {   // waves that run on by themselves hide the trip through LDS (112 us backward for 32,768 x 640 bf16, 116 without it) ...
-        a += __shfl_xor(a, 16);
-        b += __shfl_xor(b, 16);
-        a += __shfl_xor(a, 32);
-        b += __shfl_xor(b, 32);
-    }
-    if constexpr (G == 256) {   // ... waves that wait for each other do not (40 us for 3003 x 1283 f32, 36 without)
+    if constexpr (G >= 64) {
         a = add_rows_of_16(a);
         b = add_rows_of_16(b);
     }
@@ -590,8 +585,8 @@ Shape shape_of(int d, int dtype) {
     return wide ? Shape{256, 2, 8} : Shape{256, 4, 4};
 }
 
-// How the backward divides the rows over workgroups (see NormGateArgs).  512 workgroups, two a compute unit, are aimed
-// at: more would write more partial sums than the rows themselves hold at the training sizes.
+// How the backward divides the rows over workgroups (see NormGateArgs).  With column sums 512 workgroups, two a compute unit,
+// are aimed at: more write more partial sums (1024: 60 us instead of 54 for 32,768 x 640, 39 instead of 30 for 3003 x 1283).
 void plan(NormGateArgs& A, int dtype, bool sums, int& blocks) {
     const int slots = THREADS / shape_of(A.d, dtype).lanes;
     const int target = sums ? 512 : 2048;
