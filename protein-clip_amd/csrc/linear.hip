@@ -478,73 +478,131 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_direct_kernel(const Gemm
     finish<T, FI, FJ, EPI>(A, acc, ones, sum_rows, lds, i0 + wi, j0 + wj, split);
 }
 
-// out[e] = sum over the splits' slabs, in their order, rounded once; blocks behind those of the weight's gradient add the row
-// sums to the bias's.  16 lanes x 4 elements and 16 parts of the splits a workgroup.
+// out[e] = sum over the splits' slabs in a fixed order, rounded once; blocks behind those of the weight's gradient sum the bias's.
+// A workgroup takes 16 x 4 elements in 16 parts of the splits, of the bias's few elements and many splits 4 x 4 in 64 parts.
 struct SlabSum {
     const float* slab[2];
     void* out[2];
     long long n[2];
-    int splits, blocks;   // blocks: of the first sum
+    int splits[2], blocks;   // blocks: of the first sum
 };
+constexpr int SUM_LANES[2] = {16, 4};
 template <typename T>
 __global__ __launch_bounds__(256) void slab_sum_kernel(const SlabSum A) {
-    __shared__ float lds[16][16][4];
-    const int lane = threadIdx.x & 15, part = threadIdx.x >> 4, which = (int)blockIdx.x >= A.blocks;
-    const long long n = A.n[which], e = (((long long)blockIdx.x - (which ? A.blocks : 0)) * 16 + lane) * 4, left = n - e;
+    __shared__ float lds[256][4];
+    const int which = (int)blockIdx.x >= A.blocks, lanes = which ? SUM_LANES[1] : SUM_LANES[0], parts = 256 / lanes, splits = A.splits[which];
+    const int lane = threadIdx.x % lanes, part = threadIdx.x / lanes;
+    const long long n = A.n[which], e = (((long long)blockIdx.x - (which ? A.blocks : 0)) * lanes + lane) * 4, left = n - e;
     const int valid = left < 4 ? (int)left : 4;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
     if (valid > 0)
 #pragma unroll 4
-        for (int k = part; k < A.splits; k += 16) {
+        for (int k = part; k < splits; k += parts) {
             float v[4];
             load_f32<float, 4>(A.slab[which] + (size_t)k * n + e, valid, v);
 #pragma unroll
             for (int c = 0; c < 4; c++) s[c] += v[c];
         }
+    for (int o = 128; o >= lanes; o >>= 1) {
 #pragma unroll
-    for (int c = 0; c < 4; c++) lds[part][lane][c] = s[c];
-    __syncthreads();
-    if (part == 0 && valid > 0) {
+        for (int c = 0; c < 4; c++) lds[threadIdx.x][c] = s[c];
+        __syncthreads();
+        if ((int)threadIdx.x < o)
 #pragma unroll
-        for (int p = 1; p < 16; p++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) s[c] += lds[p][lane][c];
-        store_f32<T, 4>((T*)A.out[which] + e, valid, s);
+            for (int c = 0; c < 4; c++) s[c] += lds[threadIdx.x + o][c];
+        __syncthreads();
     }
+    if (part == 0 && valid > 0) store_f32<T, 4>((T*)A.out[which] + e, valid, s);
 }
 
-// dz = dy * slope, or dy where the output is positive.  Four accesses of each operand are under way at once (one: 245 us
-// for 65,536 x 2560 bf16 in and out with the slope, four: 197 us, 5.1 TB/s).
+// dz = dy * slope, or dy where the output is positive, rounded; and the column sums of the unrounded products, from which the
+// bias's gradient comes (the rounded ones would bring it the errors of M roundings).  `lanes` neighbouring threads take a row's
+// vectors, 256 / lanes rows at once; a workgroup takes `rows` rows of its columns, with four accesses of each operand under way.
+struct SlopeArgs {
+    const void *dy, *saved;
+    void *dz, *db;        // db: written when one workgroup holds all rows
+    float* sums;          // [workgroups over the rows][N], or NULL when no sums are wanted or db takes them
+    int is_output, M, N, lanes, rows;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, const void* __restrict__ saved, int is_output, long long n, T* __restrict__ dz) {
+__global__ __launch_bounds__(256) void slope_kernel(const SlopeArgs A) {
     constexpr int V = PclipVec<T>::N, AHEAD = 4;
-    const T* y = (const T*)saved;
-    const SlopeOf<T>* slope = (const SlopeOf<T>*)saved;
-    auto one = [&](T d, T s, SlopeOf<T> q) { return is_output ? ((float)s > 0.f ? (float)d : 0.f) : (float)d * ((float)q * SLOPE_UNIT<T>); };
-    const long long stride = (long long)gridDim.x * 256 * V;
-    for (long long first = ((long long)blockIdx.x * 256 + threadIdx.x) * V; first < n; first += stride * AHEAD) {
-        PclipPack<T, V> d[AHEAD], s[AHEAD];
+    typedef PclipPack<T, V> Pack;
+    __shared__ float lds[256][V + 1];
+    const int c = ((int)blockIdx.x * A.lanes + (int)threadIdx.x % A.lanes) * V, valid = A.N - c, step = 256 / A.lanes;
+    const int begin = (int)blockIdx.y * A.rows, end = A.M - begin > A.rows ? begin + A.rows : A.M;
+    const T *dy = (const T*)A.dy, *saved = (const T*)A.saved;   // the slopes are as wide
+    T* dz = (T*)A.dz;
+    float sum[V];
 #pragma unroll
-        for (int q = 0; q < AHEAD; q++) {
-            const long long e = first + q * stride;
-            if (e + V <= n) {
-                d[q] = *(const PclipPack<T, V>*)(dy + e);
-                s[q] = *(const PclipPack<T, V>*)(y + e);   // the slopes are as wide
+    for (int i = 0; i < V; i++) sum[i] = 0.f;
+    auto product = [&](T d, T s, SlopeOf<T> q) { return A.is_output ? ((float)s > 0.f ? (float)d : 0.f) : (float)d * ((float)q * SLOPE_UNIT<T>); };
+    int row = begin + (int)threadIdx.x / A.lanes;
+    // the last vector of a row that does not divide into vectors is read from V columns before the row's end on, and what
+    // it shares with the one before is left out (rows shorter than a vector go element by element)
+    const int twice = valid >= V ? 0 : V - valid;
+    if (valid > 0 && A.N >= V) {
+        const int from = c - twice;
+        auto use = [&](const Pack& d, const Pack& s, size_t at) {
+            const auto q = __builtin_bit_cast(PclipPack<SlopeOf<T>, V>, s);
+            float x[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                x[i] = product(d.v[i], s.v[i], q.v[i]);
+                sum[i] += x[i];
             }
-        }
-#pragma unroll
-        for (int q = 0; q < AHEAD; q++) {
-            const long long e = first + q * stride;
-            if (e + V <= n) {
-                const auto t = __builtin_bit_cast(PclipPack<SlopeOf<T>, V>, s[q]);
-                float x[V];
-#pragma unroll
-                for (int i = 0; i < V; i++) x[i] = one(d[q].v[i], s[q].v[i], t.v[i]);
-                store_f32<T, V>(dz + e, V, x);
+            if (twice == 0) {
+                store_f32<T, V>(dz + at, V, x);
             } else {
-                for (long long k = e; k < n; k++) dz[k] = (T)one(dy[k], y[k], slope[k]);
+#pragma unroll
+                for (int i = 1; i < V; i++)
+                    if (i >= twice) dz[at + i] = (T)x[i];
             }
+        };
+        for (; end - row > (AHEAD - 1) * step; row += AHEAD * step) {
+            Pack d[AHEAD], s[AHEAD];
+#pragma unroll
+            for (int q = 0; q < AHEAD; q++) {
+                const size_t at = (size_t)(row + q * step) * A.N + from;
+                d[q] = *(const Pack*)(dy + at);
+                s[q] = *(const Pack*)(saved + at);
+            }
+#pragma unroll
+            for (int q = 0; q < AHEAD; q++) use(d[q], s[q], (size_t)(row + q * step) * A.N + from);
         }
+        for (; row < end; row += step) {
+            const size_t at = (size_t)row * A.N + from;
+            use(*(const Pack*)(dy + at), *(const Pack*)(saved + at), at);
+        }
+#pragma unroll
+        for (int i = 0; i < V; i++) {   // the columns from c on come first
+            float moved = sum[i];
+#pragma unroll
+            for (int k = 1; k < V; k++)
+                if (twice == k && i + k < V) moved = sum[i + k];
+            sum[i] = moved;
+        }
+    } else if (valid > 0) {
+        for (; row < end; row += step)
+#pragma unroll
+            for (int i = 0; i < V; i++)
+                if (i < valid) {
+                    const size_t at = (size_t)row * A.N + c + i;
+                    const float x = product(dy[at], saved[at], ((const SlopeOf<T>*)saved)[at]);
+                    sum[i] += x;
+                    dz[at] = (T)x;
+                }
+    }
+    if (!A.sums && !A.db) return;
+#pragma unroll
+    for (int i = 0; i < V; i++) lds[threadIdx.x][i] = sum[i];
+    __syncthreads();
+    if ((int)threadIdx.x < A.lanes && valid > 0) {
+        for (int t = A.lanes; t < 256; t += A.lanes)
+#pragma unroll
+            for (int i = 0; i < V; i++) sum[i] += lds[threadIdx.x + t][i];
+        if (A.db) store_f32<T, V>((T*)A.db + c, valid, sum);
+        else store_f32<float, V>(A.sums + (size_t)blockIdx.y * A.N + c, valid, sum);
     }
 }
 
@@ -630,15 +688,47 @@ int forward(const GemmArgs& A, int act, hipStream_t st) {
     return launch_rows<T, true, true, PCLIP_ACT_SILU>(A, st);
 }
 
+// how slope_kernel divides M x N: lanes a row, workgroups over the columns and over the rows (of 64 rows at least), rows of each
+struct SlopePlan { int lanes, over_n, over_m, rows; };
+SlopePlan slope_plan(int M, int N, int dtype) {
+    const int V = dtype == PCLIP_DT_F32 ? 4 : 8, vecs = (N + V - 1) / V;
+    int lanes = 1;
+    while (lanes < vecs && lanes < 64) lanes *= 2;
+    const int over_n = (vecs + lanes - 1) / lanes;
+    long long rows = ((long long)M * over_n + 2047) / 2048;   // eight workgroups a compute unit
+    if (rows < 64) rows = 64;
+    return {lanes, over_n, (int)((M + rows - 1) / rows), (int)rows};
+}
+
+// where the parts of the workspace lie
+struct BackwardLayout { size_t sums, slab, row_sum, bytes; };   // dz at 0
+BackwardLayout backward_layout(int M, int K, int N, int dtype, int act) {
+    BackwardLayout L = {};
+    if (act != PCLIP_ACT_NONE) {
+        const SlopePlan s = slope_plan(M, N, dtype);
+        L.sums = pclip_align_up((size_t)M * N * pclip_dtype_size(dtype), 256);
+        L.slab = L.sums + (s.over_m > 1 ? pclip_align_up((size_t)s.over_m * N * sizeof(float), 256) : 0);
+    }
+    const RowPlan p = row_plan(M, K, N, dtype);
+    L.row_sum = L.slab + (p.splits > 1 ? pclip_align_up((size_t)p.splits * N * K * sizeof(float), 256) : 0);
+    L.bytes = L.row_sum + (p.splits > 1 && act == PCLIP_ACT_NONE ? (size_t)p.splits * N * sizeof(float) : 0);
+    return L;
+}
+
 template <typename T>
 int backward(const T* x, const T* w, const T* dy, const void* saved, int is_output, int M, int K, int N, int dtype, int act, T* dx, T* dw, T* db, char* ws,
              hipStream_t st) {
+    const BackwardLayout L = backward_layout(M, K, N, dtype, act);
+    const RowPlan p = row_plan(M, K, N, dtype);
+    SlabSum S = {};
     const T* dz = dy;
     if (act != PCLIP_ACT_NONE) {
-        const long long n = (long long)M * N, want = (n + 256 * PclipVec<T>::N - 1) / (256 * PclipVec<T>::N);
-        slope_kernel<T><<<want < 4096 ? (int)want : 4096, 256, 0, st>>>(dy, saved, is_output, n, (T*)ws);
+        const SlopePlan s = slope_plan(M, N, dtype);
+        SlopeArgs A = {dy, saved, ws, nullptr, nullptr, is_output, M, N, s.lanes, s.rows};
+        if (db && s.over_m == 1) A.db = db;
+        else if (db) A.sums = (float*)(ws + L.sums), S.slab[1] = A.sums, S.out[1] = db, S.n[1] = N, S.splits[1] = s.over_m;
+        slope_kernel<T><<<dim3(s.over_n, s.over_m), 256, 0, st>>>(A);
         dz = (const T*)ws;
-        ws += pclip_align_up((size_t)n * sizeof(T), 256);
     }
     if (dx) {
         GemmArgs A = {};
@@ -646,23 +736,23 @@ int backward(const T* x, const T* w, const T* dy, const void* saved, int is_outp
         const int rc = launch_rows<T, true, false, EPI_STORE>(A, st);
         if (rc) return rc;
     }
-    if (dw || db) {
-        const RowPlan p = row_plan(M, K, N, dtype);
+    const bool sum_here = db && act == PCLIP_ACT_NONE;   // dz is dy, exactly: its sums ride on the product
+    if (dw || sum_here) {
         GemmArgs A = {};
         A.P = dz, A.Q = x, A.ldp = N, A.ldq = K, A.I = N, A.J = K, A.K = M, A.k_split = p.k_split, A.splits = p.splits;
-        A.sum_rows = db != nullptr;
+        A.sum_rows = sum_here;
         if (p.splits == 1) {
-            A.out = dw, A.slope = db;
+            A.out = dw, A.slope = sum_here ? db : nullptr;
         } else {
-            A.slab = (float*)ws;
-            A.row_sum = A.slab + (size_t)p.splits * N * K;
+            A.slab = (float*)(ws + L.slab), A.row_sum = (float*)(ws + L.row_sum);
+            if (dw) S.slab[0] = A.slab, S.out[0] = dw, S.n[0] = (long long)N * K, S.splits[0] = p.splits, S.blocks = (int)((S.n[0] + 4 * SUM_LANES[0] - 1) / (4 * SUM_LANES[0]));
+            if (sum_here) S.slab[1] = A.row_sum, S.out[1] = db, S.n[1] = N, S.splits[1] = p.splits;
         }
         const int rc = launch_product<T, false, false, EPI_SLAB>(A, p.tile, p.tile, st);
-        if (rc || p.splits == 1) return rc;
-        const long long n = (long long)N * K;
-        SlabSum S = {{A.slab, A.row_sum}, {dw, db}, {n, N}, p.splits, dw ? (int)((n + 63) / 64) : 0};
-        slab_sum_kernel<T><<<S.blocks + (db ? (N + 63) / 64 : 0), 256, 0, st>>>(S);
+        if (rc) return rc;
     }
+    const int blocks = S.blocks + (S.out[1] ? (N + 4 * SUM_LANES[1] - 1) / (4 * SUM_LANES[1]) : 0);
+    if (blocks) slab_sum_kernel<T><<<blocks, 256, 0, st>>>(S);
     return PCLIP_OK;
 }
 
@@ -693,9 +783,7 @@ extern "C" int pclip_linear_fwd(const void* x, const void* w, const void* bias, 
 
 extern "C" size_t pclip_linear_bwd_workspace_bytes(int M, int K, int N, int dtype, int activation) {
     if (check_sizes("linear_bwd", M, K, N, dtype, activation)) return 0;
-    const RowPlan p = row_plan(M, K, N, dtype);
-    const size_t dz = activation == PCLIP_ACT_NONE ? 0 : pclip_align_up((size_t)M * N * pclip_dtype_size(dtype), 256);
-    return dz + (p.splits > 1 ? (size_t)p.splits * N * ((size_t)K + 1) * sizeof(float) : 0);
+    return backward_layout(M, K, N, dtype, activation).bytes;
 }
 
 extern "C" int pclip_linear_bwd(const void* x, const void* w, const void* dy, const void* saved, int saved_is_output, int M, int K, int N, int dtype,
@@ -703,7 +791,7 @@ extern "C" int pclip_linear_bwd(const void* x, const void* w, const void* dy, co
     int rc = check_sizes("linear_bwd", M, K, N, dtype, activation);
     if (rc) return rc;
     PCLIP_REQUIRE(dy && (!dx || w) && (!dw || x), "linear_bwd: null pointer");
-    PCLIP_REQUIRE(x || !db, "linear_bwd: the bias gradient runs with the weight's product and needs x");
+    PCLIP_REQUIRE(x || !db || activation != PCLIP_ACT_NONE, "linear_bwd: the bias gradient runs with the weight's product and needs x");
     PCLIP_REQUIRE(activation == PCLIP_ACT_NONE || saved, "linear_bwd: what the forward saved is needed");
     PCLIP_REQUIRE(!saved_is_output || activation == PCLIP_ACT_RELU, "linear_bwd: only relu's slope can be read from the output");
     const size_t need = pclip_linear_bwd_workspace_bytes(M, K, N, dtype, activation);
