@@ -235,6 +235,40 @@ __device__ __forceinline__ void add_rows(const typename Mfma<T>::Frag (&fp)[FI],
     }
 }
 
+// f32 products are summed in runs of RUN steps (256 k values), whose sums are added: one chain over 2560 k values ends up 1e-6 off,
+// twice what a library's product is.  16-bit results do not show it.
+constexpr int RUN = 8;
+template <typename T, int FI, int FJ>
+struct Runs {
+    static constexpr bool ON = sizeof(T) == 4;
+    f32x4 total[ON ? FI : 1][ON ? FJ : 1], total_ones[ON ? FI / 2 : 1];
+    int step = 0;
+    __device__ __forceinline__ Runs() {
+        if constexpr (ON)
+#pragma unroll
+            for (int i = 0; i < FI; i++) {
+                total_ones[i / 2] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < FJ; j++) total[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+    }
+    static __device__ __forceinline__ void move(f32x4& total, f32x4& acc, bool last) {
+        total += acc;
+        acc = last ? total : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ void end_of_step(f32x4 (&acc)[FI][FJ], f32x4 (&ones)[FI / 2], bool last) {
+        if constexpr (ON) {
+            if (++step % RUN && !last) return;
+#pragma unroll
+            for (int i = 0; i < FI; i++) {
+                if (i % 2 == 0) move(total_ones[i / 2], ones[i / 2], last);
+#pragma unroll
+                for (int j = 0; j < FJ; j++) move(total[i][j], acc[i][j], last);
+            }
+        }
+    }
+};
+
 // Workgroups go to the eight XCDs in turn; give each XCD a run of neighbouring tiles, which share rows of P or Q in its L2.
 __device__ __forceinline__ int xcd_order(int b, int n) {
     const int xcd = b & 7, q = n >> 3, r = n & 7;
@@ -362,6 +396,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_kernel(const GemmArgs A)
 #pragma unroll
         for (int j = 0; j < FJ; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    Runs<T, FI, FJ> runs;
     Frag one;
 #pragma unroll
     for (int e = 0; e < PclipVec<T>::N; e++) one[e] = (T)1.f;
@@ -391,6 +426,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_kernel(const GemmArgs A)
                 for (int j = 0; j < FJ; j++) acc[i][j] = Mfma<T>::step(fq[j], fp[i], acc[i][j]);
             if (sum_rows) add_rows<T, FI>(fp, one, wj == 0, ones);
         }
+        runs.end_of_step(acc, ones, k + KSTEP<T> >= k_end);
         buf ^= 1;
     }
 
@@ -448,6 +484,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_direct_kernel(const Gemm
 #pragma unroll
         for (int j = 0; j < FJ; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    Runs<T, FI, FJ> runs;
     Frag one;
 #pragma unroll
     for (int e = 0; e < PclipVec<T>::N; e++) one[e] = (T)1.f;
@@ -474,6 +511,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_direct_kernel(const Gemm
                 for (int j = 0; j < FJ; j++) acc[i][j] = Mfma<T>::step(fq[s][j], fp[s][i], acc[i][j]);
             if (sum_rows) add_rows<T, FI>(fp[s], one, wj == 0, ones);
         }
+        runs.end_of_step(acc, ones, k + KSTEP<T> >= k_end);
     }
     finish<T, FI, FJ, EPI>(A, acc, ones, sum_rows, lds, i0 + wi, j0 + wj, split);
 }
@@ -631,7 +669,8 @@ template <typename T, bool DIRECT, bool PK, bool QK, int EPI>
 int launch_size(const GemmArgs& A, int bi, int bj, hipStream_t st) {
     if constexpr (DIRECT && EPI != EPI_SLAB && sizeof(T) == 2)
         if (bi == 256) return launch_tile<T, 256, 128, DIRECT, PK, QK, EPI>(A, st);
-    if (bi >= 128) return launch_tile<T, 128, 128, DIRECT, PK, QK, EPI>(A, st);
+    if constexpr (EPI == EPI_SLAB || sizeof(T) == 2)   // f32 rows go in small tiles only, see launch_rows
+        if (bi >= 128) return launch_tile<T, 128, 128, DIRECT, PK, QK, EPI>(A, st);
     return launch_tile<T, 64, 64, DIRECT, PK, QK, EPI>(A, st);
 }
 // whether every row of both operands begins at a multiple of 16 bytes
