@@ -412,7 +412,7 @@ def _check_disjoint(src, dst):
 
 def grad_clip(src, dst=None, max_norm: float = 0.0, eps: float = 1e-6) -> torch.Tensor:
     """Norm [1] of all elements of the tensors ``src``; with ``dst`` (tensors of the same shapes; ``src`` itself: in place)
-    also ``dst = src * min(1, max_norm / (norm + eps))``.  One launch a pass for every 120 tensors."""
+    also ``dst = src * min(1, max_norm / (norm + eps))``.  One launch a pass."""
     in_place = dst is src
     src = list(src)
     n = len(src)

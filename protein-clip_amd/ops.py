@@ -331,7 +331,13 @@ def clip_grads(grads, max_norm: float, out=None, eps: float = 1e-6, kernels=None
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grads: max_norm must be zero or more, got {max_norm}")
     grads = list(grads)
-    return (kernels or _hip_kernels).grad_clip(grads, grads if out is None else out, max_norm, float(eps)).reshape(())
+    written = grads if out is None else list(out)
+    norm = (kernels or _hip_kernels).grad_clip(grads, written, max_norm, float(eps)).reshape(())
+    try:   # torch does not see the kernels' writes: a backward that still needs the old values must be refused
+        torch.autograd.graph.increment_version(written)
+    except RuntimeError:   # tensors of inference mode have no version
+        torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
+    return norm
 
 
 def clip_grad_norm_(parameters, max_norm: float, eps: float = 1e-6, error_if_nonfinite: bool = False, kernels=None) -> torch.Tensor:

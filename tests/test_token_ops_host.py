@@ -313,3 +313,40 @@ def test_entry_options(monkeypatch):
     monkeypatch.setattr(sys, "argv", ["main.py", "--token-dtype", "bf16", "--max-grad-norm", "1.5"])
     args = entry.parse_args({"epochs": 1, "batch_size": 2})
     assert entry.TOKEN_DTYPES[args.token_dtype] is torch.bfloat16 and args.max_grad_norm == 1.5
+
+
+class _RawWriter:
+    """Writes the tensors' memory as the kernels do: without torch knowing."""
+
+    @staticmethod
+    def grad_clip(src, dst=None, max_norm=0.0, eps=1e-6):
+        norm = torch.sqrt(sum((t.detach().double() ** 2).sum() for t in src)).float()
+        values = [t.detach() * torch.clamp(max_norm / (norm + eps), max=1.0) for t in src]
+        for v, d in zip(values, dst):
+            d.detach().numpy()[...] = v.numpy()
+        return norm.reshape(1)
+
+
+@pytest.mark.parametrize("where", ["in place", "out"])
+def test_clipping_counts_as_a_write(where):
+    """A backward that needs a value which clipping has overwritten is refused, as after torch's own in-place operations."""
+    from protein_clip_amd import ops
+    a = torch.ones(8, requires_grad=True)
+    v = torch.ones(8)
+    y = (a * v).sum()   # keeps v
+    if where == "in place":
+        ops.clip_grads([v], 0.5, kernels=_RawWriter)
+    else:
+        ops.clip_grads([torch.ones(8)], 0.5, out=[v], kernels=_RawWriter)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_clipping_tensors_of_inference_mode():
+    """Tensors made in inference mode have no version; they are clipped with the others."""
+    from protein_clip_amd import ops
+    with torch.inference_mode():
+        v = torch.ones(3)
+    w = torch.ones(1)
+    ops.clip_grads([v, w], 1.0, kernels=_RawWriter)
+    assert abs(v[0].item() - 0.5) < 1e-6 and w._version == 1
