@@ -7,7 +7,8 @@
 // neighbouring chunks, so it searches the table once.  Up to TENSORS tensors the table travels in the kernels' arguments;
 // longer ones are written to the workspace first, TENSORS entries a launch, and each pass is one launch all the
 // same (five tables of 120 tensors in turn left the device half empty at every end: 118 -> 77 us for the first pass over
-// the 490 tensors of a 30-layer trunk in bf16, 3.9 TB/s; the second, into f32, 192 us, 4.6 TB/s).  Nothing is copied from the host, so a captured graph replays it as it stands.
+// the 490 tensors of a 30-layer trunk in bf16, 3.9 TB/s; the second, into f32, 192 us, 4.6 TB/s).  Nothing is
+// copied from the host, so a captured graph replays it as it stands.
 //
 // Squares are summed in f64: f32 squares of gradients beyond 1.8e19 would overflow and those below 1e-23 vanish, and
 // the conversion and multiply-add cost an eighth of the time the memory needs.  The order of summation is fixed by

@@ -180,7 +180,7 @@ __device__ __forceinline__ float activate(float z, float& slope) {
 }
 
 // The slope is kept for the backward: as it is for f32, for 16-bit types as 16-bit whole numbers in steps of
-// 1 / (0.875 * 32767) (slopes lie between -0.13 and 1.13; half a step is a fourteenth of an f16 rounding at one, and the
+// 1 / (0.875 * 32767) (slopes lie between -0.13 and 1.13; half a step is a fourteenth of an f16 rounding just below one, and the
 // hardware packs two such numbers in one instruction), so that dz is rounded once, not twice.
 template <typename T> using SlopeOf = std::conditional_t<sizeof(T) == 4, float, short>;
 template <typename T> constexpr float SLOPE_UNIT = sizeof(T) == 4 ? 1.f : 1.f / (0.875f * 32767.f);
@@ -437,8 +437,8 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_kernel(const GemmArgs A)
 // LDS is enough, because a wave takes all its fragments of a step into registers first; the next tile is on its way while
 // the matrix cores work, and two or three workgroups share a compute unit.  Chunks outside the matrix are read at an offset
 // beyond the descriptor's range, which writes zeros.  Bound by the matrix cores and the reads of LDS (a 64 x 64 part of a
-// tile reads 16 KB for 32 matrix instructions, 128 x 64 24 KB for 64): 65,536 x 2560 -> 640 bf16 238 us, 900 TFLOP/s; dW 265 us,
-// 810; 16,384 x 1280 -> 1280 55 us, 970.  The staged form: 521 at 16,383 x 1283 -> 1279.
+// tile reads 16 KB for 32 matrix instructions, 128 x 64 24 KB for 64): 65,536 x 2560 -> 640 bf16 235 us, 910 TFLOP/s; dW 263 us,
+// 820; 16,384 x 1280 -> 1280 52.5 us, 1023.  The staged form: 521 at 16,383 x 1283 -> 1279.
 template <typename T, int BI, int BJ, int WI, int WJ, bool PK, bool QK, int EPI>
 __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_direct_kernel(const GemmArgs A) {
     typedef Tile<T, BI, PK> TP;
@@ -555,7 +555,8 @@ __global__ __launch_bounds__(256) void slab_sum_kernel(const SlabSum A) {
     if (part == 0 && valid > 0) store_f32<T, 4>((T*)A.out[which] + e, valid, s);
 }
 
-// Bound by memory: 1.0 GB for 65,536 x 2560 bf16 in 206 us, 4.9 TB/s (with one access under way instead of four 245 us).
+// Bound by memory: 1.0 GB for 65,536 x 2560 bf16 in 206 us, 4.9 TB/s (before the column sums were added: 180-197 us, with one access under
+// way instead of four 245).
 // dz = dy * slope, or dy where the output is positive, rounded; and the column sums of the unrounded products, from which the
 // bias's gradient comes (the rounded ones would bring it the errors of M roundings).  `lanes` neighbouring threads take a row's
 // vectors, 256 / lanes rows at once; a workgroup takes `rows` rows of its columns, with four accesses of each operand under way.

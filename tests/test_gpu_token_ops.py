@@ -508,3 +508,140 @@ def test_gradients_against_differences(ops):
             diff = (shift(h) - shift(-h)).item() / (2 * h)
         exact = (grads[k].double() * way.double()).sum().item()
         assert abs(diff - exact) <= 2.0 ** -8 * (1 + grads[k].norm().item()), k
+
+
+# ---- calls at the edges of what is allowed -------------------------------------------------------------------------
+def test_clip_of_many_tensors_captured(ops):
+    """A table of more tensors than the kernels' arguments hold, written anew by every replay: replays on new values, with eager
+    calls of another table between them, equal the eager results."""
+    g = torch.Generator().manual_seed(31)
+    src = [make(g, BF16, 1 + 37 * (k % 11)).cuda() for k in range(250)]
+    other = [make(g, F32, 5 + k % 7).cuda() for k in range(200)]
+    dst = [torch.empty(v.shape, device="cuda") for v in src]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.clip_grads(src, 0.5, out=dst)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = ops.clip_grads(src, 0.5, out=dst)
+    for turn in range(3):
+        for v in src:
+            v.mul_(-0.75)
+        want = [torch.empty_like(d) for d in dst]
+        want_norm = ops.clip_grads(src, 0.5, out=want)
+        ops.clip_grads(other, 0.5)
+        for d in dst:
+            d.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(norm, want_norm) and all(torch.equal(a, b) for a, b in zip(dst, want)), f"turn {turn}"
+
+
+def test_two_threads_on_two_streams(ops):
+    """Two threads run the step on inputs and streams of their own at once; each result equals the one computed alone."""
+    import threading
+    cases = []
+    for k in range(2):
+        x, p, keep = _token_params(BF16)
+        x = (x * (1 + k)).cuda()
+        keep = keep.cuda()
+        alone = _token_step(ops, x, {n: leaf(v) for n, v in p.items()}, keep)
+        cases.append((x, {n: leaf(v) for n, v in p.items()}, keep, alone))
+    torch.cuda.synchronize()
+    results = [None, None]
+
+    def work(k):
+        x, p, keep, _ = cases[k]
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            outs = [_token_step(ops, x, p, keep) for _ in range(5)]
+        stream.synchronize()
+        results[k] = outs
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    for k in range(2):
+        assert results[k] is not None, f"thread {k} ended early"
+        for outs in results[k]:
+            assert all(torch.equal(a, b) for a, b in zip(outs, cases[k][3])), f"thread {k}"
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("width", [16, 128, 640, 1280, 2560])
+def test_norm_gate_at_odd_addresses(ops, t, width):
+    """Operands that begin one element (a mask: one byte) behind an aligned address."""
+    g = torch.Generator().manual_seed(width)
+    rows = 37
+    u, r, el, dy, dn = (make(g, t, rows, width) for _ in range(5))
+    keep = torch.rand(rows, width, generator=g) >= 0.2
+
+    def shifted(v):
+        flat = torch.zeros(v.numel() + 1, dtype=v.dtype, device="cuda")
+        flat[1:] = v.cuda().reshape(-1)
+        return flat[1:].view(v.shape)
+
+    for gate in (el, keep):
+        want = R.norm_gate_bounds(wide(u), wide(r), wide(gate), 0.75, (None, None), (None, None), "layer", wide(dy), wide(dn), t)
+        a, b, gt = shifted(u).requires_grad_(True), shifted(r).requires_grad_(True), shifted(gate)
+        if gate is el:
+            gt.requires_grad_(True)
+        y, n = ops.norm_gate_residual(a, b, gt, scale=0.75, after=(None, None), before=(None, None))
+        R.assert_within(y, *want["y"], "y")
+        R.assert_within(n, *want["n"], "n")
+        torch.autograd.backward((y, n), (shifted(dy), shifted(dn)))
+        R.assert_within(a.grad, *want["u"], "du")
+        R.assert_within(b.grad, *want["residual"], "dresidual")
+        if gate is el:
+            R.assert_within(gt.grad, want["gate"][0], R.rounded(*want["gate"], t), "dgate")
+
+
+def test_byte_mask_keeps_what_is_not_zero(ops):
+    u = torch.arange(1.0, 9.0, device="cuda").view(2, 4)
+    gate = torch.tensor([[0, 1, 2, 255], [128, 0, 0, 3]], dtype=torch.uint8, device="cuda")
+    assert torch.equal(ops.norm_gate_residual(u, gate=gate, scale=2.0), torch.where(gate != 0, 2 * u, 0 * u))
+
+
+def test_one_tensor_in_two_places(ops):
+    """The same tensor as block output, residual and gate, and as the input and the residual of a layer: its gradients add up."""
+    g = torch.Generator().manual_seed(3)
+    v, w, dy = make(g, F32, 9, 24), make(g, F32, 24, 24, std=0.2), make(g, F32, 9, 24)
+    a, b = v.double().requires_grad_(True), leaf(v)
+    (R.norm_gate(a, a, a, 0.5, (None, None), None, "layer")[0] * dy.double()).sum().backward()
+    (ops.norm_gate_residual(b, b, b, scale=0.5, after=(None, None)) * dy.cuda()).sum().backward()
+    # values of order one to four, some sixty operations, sums over 24 terms
+    R.assert_within(b.grad, a.grad, 64 * 24 * R.U * (1 + a.grad.abs()), "norm_gate")
+    a, b = v.double().requires_grad_(True), leaf(v)
+    (R.linear(a, w.double(), None, a, "silu") * dy.double()).sum().backward()
+    (ops.linear_act(b, w.cuda(), residual=b, activation="silu") * dy.cuda()).sum().backward()
+    R.assert_within(b.grad, a.grad, 64 * 24 * R.U * (1 + a.grad.abs()), "linear")
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("rows,width,out", [(3, 65536, 2), (3, 2, 65536), (1, 65535, 1)])
+def test_linear_at_the_widest(ops, t, rows, width, out):
+    g = torch.Generator().manual_seed(out)
+    x, w, dy = make(g, t, rows, width), make(g, t, out, width, std=1 / math.sqrt(width)), make(g, t, rows, out)
+    b = make(g, t, out)
+    want = R.linear_bounds(x.double(), w.double(), b.double(), None, dy.double(), "none", t)
+    xs, ws, bs = leaf(x), leaf(w), leaf(b)
+    y = ops.linear_act(xs, ws, bs)
+    y.backward(dy.cuda())
+    R.assert_within(y, *want["y"], "y")
+    for p, n in ((xs, "x"), (ws, "weight"), (bs, "bias")):
+        R.assert_within(p.grad, *want[n], "d" + n)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_beyond_the_limits_is_refused(ops, t):
+    from protein_clip_amd._lib import PclipError
+    z = lambda *s: torch.zeros(*s, dtype=t, device="cuda")
+    for x, w in ((z(1, 65537), z(1, 65537)), (z(1, 1), z(65537, 1))):
+        with pytest.raises(PclipError, match="widths"):
+            ops.linear_act(x, w)
+    with pytest.raises(PclipError, match="row width"):
+        ops.norm_gate_residual(z(2, 4097), after=(None, None))
