@@ -343,8 +343,8 @@ int pclip_filip_prep_bwd(const float* h, const float* dn, int B, int T, int d, i
  * 1 <= K, N <= PCLIP_LINEAR_MAX_DIM.  Products and sums are f32 (bf16 / f16 operands on the matrix cores, f32
  * operands on their f32 form); y is rounded once.
  * activation: 0 none, 1 relu, 2 gelu (the exact one, with erf), 3 silu.
- * slope: NULL, or [M,N] f32 (dtype f32) or of 16-bit whole numbers (bf16, f16; 0.875 * 32767 steps to
- * one): act'(z), kept for the backward.  Not needed for activation 0, nor for relu without a residual, where the
+ * slope: NULL, or [M,N], of f32 (dtype f32 and f16: act'(z)) or f16 (dtype bf16: act'(z) * 2^15),
+ * kept for the backward.  Not needed for activation 0, nor for relu without a residual, where the
  * backward reads the sign of y.
  *
  * Backward: dy [M,N] -> dz = dy * act'(z), rounded to `dtype`;

@@ -35,12 +35,15 @@ __device__ __forceinline__ void store_f32(T* p, int valid, const float (&v)[V]) 
             if (i < valid) p[i] = (T)v[i];
     }
 }
-// 8 or 16 bytes past the L2 (results that nobody reads back soon: they would push out what the kernel still reads)
+// 8, 16 or 32 bytes past the L2 (results that nobody reads back soon: they would push out what the kernel still reads)
 template <typename P>
 __device__ __forceinline__ void store_past_l2(void* p, const P& a) {
-    static_assert(sizeof(P) == 16 || sizeof(P) == 8, "one access");
-    typedef unsigned __attribute__((ext_vector_type(sizeof(P) / 4), aligned(1))) Any;
-    __builtin_nontemporal_store(__builtin_bit_cast(Any, a), (Any*)p);
+    static_assert(sizeof(P) == 32 || sizeof(P) == 16 || sizeof(P) == 8, "one access or two");
+    typedef unsigned __attribute__((ext_vector_type(sizeof(P) == 8 ? 2 : 4), aligned(1))) Any;
+    struct Parts { Any part[sizeof(P) / sizeof(Any)]; };
+    const Parts all = __builtin_bit_cast(Parts, a);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(P) / sizeof(Any)); i++) __builtin_nontemporal_store(all.part[i], (Any*)p + i);
 }
 template <typename T, int V>
 __device__ __forceinline__ void stream_f32(T* p, int valid, const float (&v)[V]) {

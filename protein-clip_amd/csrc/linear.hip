@@ -179,32 +179,20 @@ __device__ __forceinline__ float activate(float z, float& slope) {
     }
 }
 
-// The slope is kept for the backward: as it is for f32, for 16-bit types as 16-bit whole numbers in steps of
-// 1 / (0.875 * 32767) (slopes lie between -0.13 and 1.13; half a step is a fourteenth of an f16 rounding just below one, and the
-// hardware packs two such numbers in one instruction), so that dz is rounded once, not twice.
-template <typename T> using SlopeOf = std::conditional_t<sizeof(T) == 4, float, short>;
-template <typename T> constexpr float SLOPE_UNIT = sizeof(T) == 4 ? 1.f : 1.f / (0.875f * 32767.f);
+// The slope is kept for the backward with the precision of a product's operand at every size, since the gradients of units that lie far
+// out rest on small slopes: in f32 for f32 and f16 operands, for bf16 as a 16-bit float of 11 bits (three more than dz keeps), times 2^15, which
+// puts slopes down to 2^-29 (gelu at -6.6, silu at -23) among its normal numbers and those up to 1.13 below its largest.  16-bit fixed
+// point, which was 1e-5 off near one, was 3 % off at gelu's -4 and zero from -5 on; f16 operands want more bits near one than a
+// 16-bit float has (their error would rise from 2.9e-4 to 3.6e-4).
+template <typename T> struct SlopeFormat { typedef float Type; static constexpr float SCALE = 1.f; };
+template <> struct SlopeFormat<__bf16> { typedef _Float16 Type; static constexpr float SCALE = 32768.f; };
+template <typename T> using SlopeOf = typename SlopeFormat<T>::Type;
 
 template <typename T, int V>
-__device__ __forceinline__ void store_slope(SlopeOf<T>* p, int valid, const float (&v)[V]) {
-    if constexpr (sizeof(T) == 4) {
-        stream_f32<T, V>(p, valid, v);
-    } else {
-        PclipPack<short, V> a;
+__device__ __forceinline__ void store_slope(SlopeOf<T>* p, int valid, float (&v)[V]) {
 #pragma unroll
-        for (int i = 0; i < V; i += 2) {
-            const auto two = __builtin_amdgcn_cvt_pknorm_i16(0.875f * v[i], 0.875f * v[i + 1]);
-            a.v[i] = two[0];
-            a.v[i + 1] = two[1];
-        }
-        if (valid >= V) {
-            store_past_l2(p, a);
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; i++)
-                if (i < valid) p[i] = a.v[i];
-        }
-    }
+    for (int i = 0; i < V; i++) v[i] *= SlopeFormat<T>::SCALE;
+    stream_f32<SlopeOf<T>, V>(p, valid, v);
 }
 
 // ---- the product -----------------------------------------------------------------------------------
@@ -564,33 +552,38 @@ struct SlopeArgs {
     const void *dy, *saved;
     void *dz, *db;        // db: written when one workgroup holds all rows
     float* sums;          // [workgroups over the rows][N], or NULL when no sums are wanted or db takes them
-    int is_output, M, N, lanes, rows;
+    int M, N, lanes, rows;
 };
-template <typename T>
+// S: the type of what was saved, the slope's or the output's
+template <typename T, typename S, bool IS_OUTPUT>
 __global__ __launch_bounds__(256) void slope_kernel(const SlopeArgs A) {
     constexpr int V = PclipVec<T>::N, AHEAD = 4;
     typedef PclipPack<T, V> Pack;
+    typedef PclipPack<S, V> Saved;
     __shared__ float lds[256][V + 1];
     const int c = ((int)blockIdx.x * A.lanes + (int)threadIdx.x % A.lanes) * V, valid = A.N - c, step = 256 / A.lanes;
     const int begin = (int)blockIdx.y * A.rows, end = A.M - begin > A.rows ? begin + A.rows : A.M;
-    const T *dy = (const T*)A.dy, *saved = (const T*)A.saved;   // the slopes are as wide
+    const T* dy = (const T*)A.dy;
+    const S* saved = (const S*)A.saved;
     T* dz = (T*)A.dz;
     float sum[V];
 #pragma unroll
     for (int i = 0; i < V; i++) sum[i] = 0.f;
-    auto product = [&](T d, T s, SlopeOf<T> q) { return A.is_output ? ((float)s > 0.f ? (float)d : 0.f) : (float)d * ((float)q * SLOPE_UNIT<T>); };
+    auto product = [](T d, S s) {
+        if constexpr (IS_OUTPUT) return (float)s > 0.f ? (float)d : 0.f;
+        else return (float)d * ((float)s * (1.f / SlopeFormat<T>::SCALE));
+    };
     int row = begin + (int)threadIdx.x / A.lanes;
     // the last vector of a row that does not divide into vectors is read from V columns before the row's end on, and what
     // it shares with the one before is left out (rows shorter than a vector go element by element)
     const int twice = valid >= V ? 0 : V - valid;
     if (valid > 0 && A.N >= V) {
         const int from = c - twice;
-        auto use = [&](const Pack& d, const Pack& s, size_t at) {
-            const auto q = __builtin_bit_cast(PclipPack<SlopeOf<T>, V>, s);
+        auto use = [&](const Pack& d, const Saved& s, size_t at) {
             float x[V];
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                x[i] = product(d.v[i], s.v[i], q.v[i]);
+                x[i] = product(d.v[i], s.v[i]);
                 sum[i] += x[i];
             }
             if (twice == 0) {
@@ -602,19 +595,20 @@ __global__ __launch_bounds__(256) void slope_kernel(const SlopeArgs A) {
             }
         };
         for (; end - row > (AHEAD - 1) * step; row += AHEAD * step) {
-            Pack d[AHEAD], s[AHEAD];
+            Pack d[AHEAD];
+            Saved s[AHEAD];
 #pragma unroll
             for (int q = 0; q < AHEAD; q++) {
                 const size_t at = (size_t)(row + q * step) * A.N + from;
                 d[q] = *(const Pack*)(dy + at);
-                s[q] = *(const Pack*)(saved + at);
+                s[q] = *(const Saved*)(saved + at);
             }
 #pragma unroll
             for (int q = 0; q < AHEAD; q++) use(d[q], s[q], (size_t)(row + q * step) * A.N + from);
         }
         for (; row < end; row += step) {
             const size_t at = (size_t)row * A.N + from;
-            use(*(const Pack*)(dy + at), *(const Pack*)(saved + at), at);
+            use(*(const Pack*)(dy + at), *(const Saved*)(saved + at), at);
         }
 #pragma unroll
         for (int i = 0; i < V; i++) {   // the columns from c on come first
@@ -630,7 +624,7 @@ __global__ __launch_bounds__(256) void slope_kernel(const SlopeArgs A) {
             for (int i = 0; i < V; i++)
                 if (i < valid) {
                     const size_t at = (size_t)row * A.N + c + i;
-                    const float x = product(dy[at], saved[at], ((const SlopeOf<T>*)saved)[at]);
+                    const float x = product(dy[at], saved[at]);
                     sum[i] += x;
                     dz[at] = (T)x;
                 }
@@ -767,10 +761,12 @@ int backward(const T* x, const T* w, const T* dy, const void* saved, int is_outp
     const T* dz = dy;
     if (act != PCLIP_ACT_NONE) {
         const SlopePlan s = slope_plan(M, N, dtype);
-        SlopeArgs A = {dy, saved, ws, nullptr, nullptr, is_output, M, N, s.lanes, s.rows};
+        SlopeArgs A = {dy, saved, ws, nullptr, nullptr, M, N, s.lanes, s.rows};
         if (db && s.over_m == 1) A.db = db;
         else if (db) A.sums = (float*)(ws + L.sums), S.slab[1] = A.sums, S.out[1] = db, S.n[1] = N, S.splits[1] = s.over_m;
-        slope_kernel<T><<<dim3(s.over_n, s.over_m), 256, 0, st>>>(A);
+        const dim3 grid(s.over_n, s.over_m);
+        if (is_output) slope_kernel<T, T, true><<<grid, 256, 0, st>>>(A);
+        else slope_kernel<T, SlopeOf<T>, false><<<grid, 256, 0, st>>>(A);
         dz = (const T*)ws;
     }
     if (dx) {

@@ -260,7 +260,7 @@ def _linear_sizes(x, w):
 
 
 def _slope_type(dtype):
-    return F32 if dtype == F32 else torch.int16   # whole steps, see pclip.h
+    return torch.float16 if dtype == torch.bfloat16 else F32   # see pclip.h
 
 
 def linear_fwd(x, w, bias=None, residual=None, activation: str = "none", want_slope: bool = False):

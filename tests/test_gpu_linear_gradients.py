@@ -1,0 +1,70 @@
+"""GPU tests of what the linear layer keeps for its backward and what its gradients make of it."""
+import pytest
+import torch
+
+import token_ref as R
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+TYPES = [F32, BF16, F16]
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    import protein_clip_amd  # noqa: F401
+    from protein_clip_amd import _lib, ops as _ops
+    assert _lib.load().pclip_check_device(0) == 0, _lib.load().pclip_last_error()
+    return _ops
+
+
+def slope_error(z, slope, t):
+    """Relative precision everywhere: exp(-z^2 / 2) and exp(z) turn the argument's roundings (four, of z^2 / 2 or z) into relative ones,
+    the fitted tail and the hardware's exp and reciprocal bring 4e-6; near the zero of gelu's slope (z = -0.75) and silu's (z = -1.28) two terms
+    of at most 0.3 cancel.  bfloat16 keeps the slope as a float of 11 bits, down to 2^-40."""
+    relative = 4e-6 + (z * z / 2 + z.abs()) * 4 * R.U
+    err = slope.abs() * relative + torch.where(z.abs() < 3, 4e-6, 0.0)
+    return err + (R.half(F16) * slope.abs() + 2.0 ** -40 if t == BF16 else 0.0)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("name", ["gelu", "silu"])
+def test_slopes_of_saturated_units(ops, t, name):
+    """One unit of one input, so that the gradient is the slope: as exact, relatively, far from zero as near it."""
+    low = -6.5 if name == "gelu" else -14.0   # gelu's slope there is 1.7e-9, silu's 1.1e-5
+    z = torch.cat([torch.linspace(low, -3.0, 300), torch.linspace(-3.0, 8.0, 100)]).to(t)
+    x = z[:, None].cuda().requires_grad_(True)
+    y = ops.linear_act(x, torch.ones(1, 1, dtype=t, device="cuda"), activation=name)
+    dy = torch.ones_like(y)
+    y.backward(dy)
+    z = z.double()
+    slope = R.act(z, name)[1]
+    R.assert_within(x.grad[:, 0], slope, R.rounded(slope, slope_error(z, slope, t), t), "dx")
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("name,centre", [("gelu", -4.5), ("gelu", -6.0), ("silu", -12.0), ("silu", -15.0)])
+@pytest.mark.parametrize("res", [False, True])
+def test_gradients_of_a_layer_of_saturated_units(ops, t, name, centre, res):
+    """Every unit's input lies around ``centre``: dx, dW and db still have the precision of their type."""
+    g = torch.Generator().manual_seed(7)
+    M, K, N = 200, 24, 40
+    x, w = (torch.randn(M, K, generator=g) * 0.5).to(t), (torch.randn(N, K, generator=g) * 0.2).to(t)
+    b, dy = torch.full((N,), centre).to(t), (torch.randn(M, N, generator=g) * 64).to(t)
+    xw, ww, bw, dw = (v.double() for v in (x, w, b, dy))
+    z = xw @ ww.t() + bw
+    ez = (K + 1) * R.U * (xw.abs() @ ww.abs().t() + bw.abs())
+    slope = R.act(z, name)[1]
+    es = slope_error(z, slope, t) + slope.abs() * (z.abs() + 2) * ez   # the logarithm of the slope changes by |z| + 1 / |z| at most
+    dz = dw * slope
+    edz = dw.abs() * es
+    rounded_dz = R.rounded(dz, edz, t)
+    sums = lambda value, err, size, n: (value, R.rounded(value, err + (n + 8) * R.U * (size + err), t))
+    leaves = [v.cuda().requires_grad_(True) for v in (x, w, b)]
+    y = ops.linear_act(*leaves, torch.zeros(M, N, dtype=t, device="cuda") if res else None, activation=name)
+    grads = torch.autograd.grad(y, leaves, dy.cuda())
+    R.assert_within(grads[0], *sums(dz @ ww, rounded_dz @ ww.abs(), dz.abs() @ ww.abs(), N), "dx")
+    R.assert_within(grads[1], *sums(dz.t() @ xw, rounded_dz.t() @ xw.abs(), dz.abs().t() @ xw.abs(), M), "dW")
+    R.assert_within(grads[2], *sums(dz.sum(0), edz.sum(0), dz.abs().sum(0), M), "db")
