@@ -147,8 +147,8 @@ struct Tile {
 template <bool EXACT, int ACT>
 __device__ __forceinline__ float activate(float z, float& slope) {
     if constexpr (ACT == PCLIP_ACT_RELU) {
-        slope = z > 0.f ? 1.f : 0.f;
-        return z > 0.f ? z : (z != z ? z : 0.f);   // NaN stays
+        slope = z <= 0.f ? 0.f : 1.f;   // a NaN passes, both ways
+        return z <= 0.f ? 0.f : z;
     } else if constexpr (ACT == PCLIP_ACT_GELU && EXACT) {
         const float phi = 0.5f * erfcf(z * -0.70710678118654752f);
         slope = fmaf(fminf(fmaxf(z, -40.f), 40.f) * 0.39894228040143268f, expf(-0.5f * z * z), phi);
@@ -570,7 +570,7 @@ __global__ __launch_bounds__(256) void slope_kernel(const SlopeArgs A) {
 #pragma unroll
     for (int i = 0; i < V; i++) sum[i] = 0.f;
     auto product = [](T d, S s) {
-        if constexpr (IS_OUTPUT) return (float)s > 0.f ? (float)d : 0.f;
+        if constexpr (IS_OUTPUT) return (float)s <= 0.f ? 0.f : (float)d;   // an output that is NaN has slope one, as in the forward
         else return (float)d * ((float)s * (1.f / SlopeFormat<T>::SCALE));
     };
     int row = begin + (int)threadIdx.x / A.lanes;

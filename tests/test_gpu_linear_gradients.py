@@ -68,3 +68,31 @@ def test_gradients_of_a_layer_of_saturated_units(ops, t, name, centre, res):
     R.assert_within(grads[0], *sums(dz @ ww, rounded_dz @ ww.abs(), dz.abs() @ ww.abs(), N), "dx")
     R.assert_within(grads[1], *sums(dz.t() @ xw, rounded_dz.t() @ xw.abs(), dz.abs().t() @ xw.abs(), M), "dW")
     R.assert_within(grads[2], *sums(dz.sum(0), edz.sum(0), dz.abs().sum(0), M), "db")
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("name", ["none", "relu", "gelu", "silu"])
+@pytest.mark.parametrize("res", [False, True])
+def test_nan_reaches_the_gradients(ops, t, name, res):
+    """A NaN row of the weight makes its unit's outputs NaN; its gradients are torch's: NaN where the slope is computed from the value,
+    dy where ReLU passes it on.  The other units stay finite."""
+    g = torch.Generator().manual_seed(9)
+    M, K, N = 90, 24, 33
+    x, w, b, dy = (torch.randn(*s, generator=g).to(t) for s in ((M, K), (N, K), (N,), (M, N)))
+    w[5] = float("nan")
+    plain = [v.double().requires_grad_(True) for v in (x, w, b)]
+    z = plain[0] @ plain[1].t() + plain[2]
+    act = {"none": lambda v: v, "relu": torch.relu, "gelu": torch.nn.functional.gelu, "silu": torch.nn.functional.silu}[name]
+    want = torch.autograd.grad(act(z), plain, dy.double())
+    leaves = [v.cuda().requires_grad_(True) for v in (x, w, b)]
+    y = ops.linear_act(*leaves, torch.ones(M, N, dtype=t, device="cuda") if res else None, activation=name)
+    assert y[:, 5].isnan().all() and torch.isfinite(y[:, :5]).all() and torch.isfinite(y[:, 6:]).all()
+    for got, ref, what in zip(torch.autograd.grad(y, leaves, dy.cuda()), want, ("dx", "dW", "db")):
+        got = got.double().cpu()
+        assert torch.equal(got.isnan(), ref.isnan()), what
+        fine = ~ref.isnan()
+        # 90 products or fewer of values of order one, those of dz rounded: six half steps of the type and 2^-23 a term of the sum of sizes
+        tol = 6 * R.half(t) * (1 + ref[fine].abs()) * 10 + 128 * R.U * 100
+        assert ((got[fine] - ref[fine]).abs() <= tol).all(), what
+
+
