@@ -345,7 +345,7 @@ int pclip_filip_prep_bwd(const float* h, const float* dn, int B, int T, int d, i
  * activation: 0 none, 1 relu, 2 gelu (the exact one, with erf), 3 silu.
  * slope: NULL, or [M,N], of f32 (dtype f32 and f16: act'(z)) or f16 (dtype bf16: act'(z) * 2^15),
  * kept for the backward.  Not needed for activation 0, nor for relu without a residual, where the
- * backward reads the sign of y.
+ * backward reads y: its slope is zero where y is +0.  (relu gives -0 for a value above zero that `dtype` rounds to zero.)
  *
  * Backward: dy [M,N] -> dz = dy * act'(z), rounded to `dtype`;
  *   dx [M,K] = dz W;  dW [N,K] = dz^T x;  db [N] = sum_rows dy * act'(z), of the products before they

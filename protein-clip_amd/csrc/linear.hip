@@ -318,6 +318,11 @@ __device__ __forceinline__ void finish(const GemmArgs& A, f32x4 (&acc)[FI][FJ], 
                     float slope[V];
 #pragma unroll
                     for (int e = 0; e < V; e++) v[e] = activate<sizeof(T) == 4, EPI>(v[e] + bias[e], slope[e]);
+                    if constexpr (EPI == PCLIP_ACT_RELU && sizeof(T) == 2) {
+                        // the backward reads the slope from the output: a value above zero that rounds to zero becomes -0
+#pragma unroll
+                        for (int e = 0; e < V; e++) v[e] = v[e] > 0.f && (float)(T)v[e] == 0.f ? -0.f : v[e];
+                    }
                     if (A.slope) store_slope<T, V>((SlopeOf<T>*)A.slope + at, left, slope);
                     if (A.residual) {
                         float res[V];
@@ -560,6 +565,7 @@ __global__ __launch_bounds__(256) void slope_kernel(const SlopeArgs A) {
     constexpr int V = PclipVec<T>::N, AHEAD = 4;
     typedef PclipPack<T, V> Pack;
     typedef PclipPack<S, V> Saved;
+    typedef std::conditional_t<sizeof(S) == 4, unsigned, unsigned short> Bits;
     __shared__ float lds[256][V + 1];
     const int c = ((int)blockIdx.x * A.lanes + (int)threadIdx.x % A.lanes) * V, valid = A.N - c, step = 256 / A.lanes;
     const int begin = (int)blockIdx.y * A.rows, end = A.M - begin > A.rows ? begin + A.rows : A.M;
@@ -570,7 +576,7 @@ __global__ __launch_bounds__(256) void slope_kernel(const SlopeArgs A) {
 #pragma unroll
     for (int i = 0; i < V; i++) sum[i] = 0.f;
     auto product = [](T d, S s) {
-        if constexpr (IS_OUTPUT) return (float)s <= 0.f ? 0.f : (float)d;   // an output that is NaN has slope one, as in the forward
+        if constexpr (IS_OUTPUT) return __builtin_bit_cast(Bits, s) == 0 ? 0.f : (float)d;   // zero only at +0; NaN, and -0 (see finish), pass
         else return (float)d * ((float)s * (1.f / SlopeFormat<T>::SCALE));
     };
     int row = begin + (int)threadIdx.x / A.lanes;

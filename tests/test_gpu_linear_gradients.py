@@ -96,3 +96,20 @@ def test_nan_reaches_the_gradients(ops, t, name, res):
         assert ((got[fine] - ref[fine]).abs() <= tol).all(), what
 
 
+
+
+def test_relu_outputs_too_small_for_their_type(ops):
+    """float16 rounds values up to 2^-25 to zero.  Their slope is one all the same; that of zero and of negative values is zero."""
+    scale = torch.tensor([1.0, 0.5, 0.0, -0.5, -1.0, 2.0 ** -10, -(2.0 ** -10)])
+    x = (scale[:, None] * 2.0 ** -13).to(F16).cuda().requires_grad_(True)
+    w = torch.full((1, 1), 2.0 ** -13, dtype=F16, device="cuda", requires_grad=True)
+    b = torch.zeros(1, dtype=F16, device="cuda", requires_grad=True)
+    y = ops.linear_act(x, w, b, activation="relu")
+    assert not y.any()
+    y.backward(torch.full_like(y, 512.0))
+    kept = (scale > 0).double()
+    assert torch.equal(x.grad[:, 0].double().cpu(), kept * 2.0 ** -4)
+    assert b.grad.item() == 512 * kept.sum().item()
+    # the sum of three products of 512 and x's own values, rounded once
+    want = 512 * (x.detach()[:, 0].double().cpu() * kept).sum()
+    assert abs(w.grad.item() - want.item()) <= R.half(F16) * want.item()
