@@ -19,6 +19,7 @@ from typing import Optional
 
 import torch
 import torch.distributed as dist
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import kernels as _hip_kernels
@@ -174,7 +175,11 @@ def _linear_fwd(x, weight, bias, residual, activation, want_slope, K):
     return K.linear_fwd(_contiguous(x), _contiguous(weight), _contiguous(bias), _contiguous(residual), activation, want_slope)
 
 
-def _wants_grad(*tensors) -> bool:
+def _wants_autograd(*tensors) -> bool:
+    """Whether the call has to go through its autograd function: an operand takes a gradient, or something else watches (forward-mode
+    tangents, a tracer, a functorch transform), which must see the function and refuse or record it, not the memory it writes."""
+    if forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None or torch._C._are_functorch_transforms_active():
+        return True
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -209,7 +214,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
             residual = residual.to(x.dtype)
         if residual.shape != shape:
             residual = residual.expand(shape)
-    if _wants_grad(x, weight, bias, residual):
+    if _wants_autograd(x, weight, bias, residual):
         return _LinearAct.apply(x, weight, bias, residual, activation, K)
     return _linear_fwd(x, weight, bias, residual, activation, False, K)[0]
 
@@ -309,7 +314,7 @@ def norm_gate_residual(u: torch.Tensor, residual: Optional[torch.Tensor] = None,
         if residual.shape != u.shape:
             residual = residual.expand(u.shape)
     cfg = (gate_rows, float(scale), norm if after is not None else None, norm if before is not None else None, float(eps), K)
-    if _wants_grad(u, residual, gate, wa, ba, wb, bb):
+    if _wants_autograd(u, residual, gate, wa, ba, wb, bb):
         return _NormGate.apply(u, residual, gate, wa, ba, wb, bb, cfg)
     y, n, _ = _norm_fwd(*map(_contiguous, (u, residual, gate, wa, ba, wb, bb)), cfg, False)
     return y if n is None else (y, n)
@@ -318,8 +323,19 @@ def norm_gate_residual(u: torch.Tensor, residual: Optional[torch.Tensor] = None,
 # --------------------------------------------------------------------------------------
 # gradient norm and clipping   (between backward and step of modules/training_utils.py:7, 92)
 # --------------------------------------------------------------------------------------
+def _check_nothing_watches(what: str, tensors):
+    """No autograd function stands before these calls: what would lose a tangent or be missing from a trace is refused."""
+    if torch._C._get_tracing_state() is not None or torch._C._are_functorch_transforms_active():
+        raise NotImplementedError(f"{what} cannot be traced or transformed")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 def grad_norm(grads, kernels=None) -> torch.Tensor:
-    """L2 norm of all elements of the tensors ``grads`` as a 0-d float32 tensor on their device, without a host sync."""
+    """L2 norm of all elements of the tensors ``grads`` as a 0-d float32 tensor on their device, without a host sync.  Outside
+    of autograd, as clipping is: the norm has no gradient."""
+    grads = list(grads)
+    _check_nothing_watches("grad_norm", grads)
     return (kernels or _hip_kernels).grad_clip(grads).reshape(())
 
 
@@ -332,6 +348,7 @@ def clip_grads(grads, max_norm: float, out=None, eps: float = 1e-6, kernels=None
         raise ValueError(f"clip_grads: max_norm must be zero or more, got {max_norm}")
     grads = list(grads)
     written = grads if out is None else list(out)
+    _check_nothing_watches("clip_grads", grads + written)
     norm = (kernels or _hip_kernels).grad_clip(grads, written, max_norm, float(eps)).reshape(())
     try:   # torch does not see the kernels' writes: a backward that still needs the old values must be refused
         torch.autograd.graph.increment_version(written)

@@ -1,0 +1,96 @@
+"""CPU tests of how the token-head operators meet autograd: forward-mode tangents, tracing and transforms that would miss what the kernels
+write, and what is kept for the backward.  The stand-in provider writes memory as the kernels do, without torch knowing."""
+import os
+import sys
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+for _p in (ROOT, os.path.join(ROOT, "tests")):
+    if _p not in sys.path:
+        sys.path.insert(0, _p)
+
+import token_cpu_provider as P  # noqa: E402
+
+
+def _raw(t):
+    if t is None:
+        return None
+    out = torch.empty(tuple(int(v) for v in t.shape), dtype=t.dtype)
+    out.numpy()[...] = t.detach().numpy()
+    return out
+
+
+def _seen(t):
+    return t.detach() if isinstance(t, torch.Tensor) else t
+
+
+class _Raw:
+    """The provider's results in memory that torch did not see being written."""
+
+    linear_fwd = staticmethod(lambda *a: tuple(_raw(t) for t in P.linear_fwd(*map(_seen, a))))
+    norm_gate_fwd = staticmethod(lambda *a: tuple(_raw(t) for t in P.norm_gate_fwd(*map(_seen, a))))
+
+    @staticmethod
+    def grad_clip(src, dst=None, max_norm=0.0, eps=1e-6):
+        norm = P.grad_clip([t.detach() for t in src])
+        for s, d in zip(src, dst or []):
+            d.detach().numpy()[...] = (s.detach() * torch.clamp(max_norm / (norm + eps), max=1.0)).numpy()
+        return norm
+
+
+def _calls():
+    from protein_clip_amd import ops
+    g = torch.Generator().manual_seed(0)
+    w, r = torch.randn(8, 8, generator=g), torch.randn(3, 8, generator=g)
+    one = torch.ones(8)
+    return {"linear_act": lambda x: ops.linear_act(x, w, activation="gelu", kernels=_Raw),
+            "linear_act weight": lambda x: ops.linear_act(r, x.t() @ x, kernels=_Raw),
+            "linear_act residual": lambda x: ops.linear_act(r, w, residual=x, kernels=_Raw),
+            "norm_gate_residual": lambda x: ops.norm_gate_residual(x, after=(one, None), kernels=_Raw),
+            "norm_gate_residual two outputs": lambda x: ops.norm_gate_residual(r, x, before=(None, None), kernels=_Raw)[1]}
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("name", sorted(_calls()))
+def test_tangents_are_refused_not_dropped(name, grad):
+    call = _calls()[name]
+    x = torch.randn(3, 8, generator=torch.Generator().manual_seed(1))
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        with pytest.raises(NotImplementedError, match="jvp"):
+            call(forward_ad.make_dual(x, torch.ones_like(x)))
+        assert torch.equal(call(x), call(x.clone()))   # no operand has a tangent: the level alone refuses nothing
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(call, (x,), (x,))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(call)(x[None])
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("name", sorted(_calls()))
+def test_traces_hold_the_operator(name):
+    """A trace of a call gives the call's results on new inputs, with and without gradients wanted."""
+    call = _calls()[name]
+    for requires in (False, True):
+        g = torch.Generator().manual_seed(2)
+        traced = torch.jit.trace(call, (torch.randn(3, 8, generator=g).requires_grad_(requires),))
+        x = torch.randn(3, 8, generator=g)
+        torch.testing.assert_close(traced(x), call(x))
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_clipping_is_refused_where_it_would_not_be_seen():
+    from protein_clip_amd import ops
+    v = torch.ones(4)
+    for call in (lambda t: ops.grad_norm([t], kernels=_Raw), lambda t: ops.clip_grads([t], 1.0, kernels=_Raw), lambda t: ops.clip_grads([v.clone()], 1.0, out=[t], kernels=_Raw)):
+        with forward_ad.dual_level():
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(forward_ad.make_dual(v.clone(), torch.ones(4)))
+            call(v.clone())
+        with pytest.raises(NotImplementedError, match="traced"):
+            torch.jit.trace(lambda t: call(t.clone()), (v,))
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            torch.func.vmap(call)(v[None])
+    assert torch.equal(v, torch.ones(4)) and ops.grad_norm(iter([v]), kernels=_Raw).item() == 2
