@@ -351,8 +351,9 @@ int pclip_filip_prep_bwd(const float* h, const float* dn, int B, int T, int d, i
  *   dx [M,K] = dz W;  dW [N,K] = dz^T x;  db [N] = sum_rows dy * act'(z), of the products before they
  *   are rounded      (the residual's gradient is dy)
  * saved: the forward's slope, or y with saved_is_output = 1 (relu without a residual), NULL for
- * activation 0.  dx, dW, db are overwritten; each may be NULL (x is read for dW, and for db with activation 0; w for
- * dx).  ws: 16-byte aligned, may be NULL where the query says 0.  Sums over rows run in a fixed
+ * activation 0.  dx, dW, db are overwritten; each may be NULL (x is read for dW, w for
+ * dx, and either may be NULL otherwise; but a call for dx and db with activation 0 has x as well).  db without dW is a column sum.
+ * ws: 16-byte aligned, may be NULL where the query says 0.  Sums over rows run in a fixed
  * order: the same inputs give the same bits.
  * ------------------------------------------------------------------------------------- */
 #define PCLIP_ACT_NONE 0

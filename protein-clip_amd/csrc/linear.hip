@@ -281,7 +281,7 @@ __device__ __forceinline__ void finish(const GemmArgs& A, f32x4 (&acc)[FI][FJ], 
                 for (int e = 0; e < 4; e++) v[e] = acc[fi][fj][e];
                 if (j >= A.J) continue;
                 if (A.slab) store_f32<float, 4>(A.slab + ((size_t)split * A.I + i) * A.J + j, A.J - j, v);
-                else if (A.out) store_f32<T, 4>((T*)A.out + (size_t)i * A.J + j, A.J - j, v);
+                else store_f32<T, 4>((T*)A.out + (size_t)i * A.J + j, A.J - j, v);
             }
             const bool first = (threadIdx.x >> 6 & 1) == 0;   // the column of waves, see add_rows
             if (sum_rows && lane < 16 && first == (fi < FI / 2)) {
@@ -555,12 +555,13 @@ __global__ __launch_bounds__(256) void slab_sum_kernel(const SlabSum A) {
 // vectors, 256 / lanes rows at once; a workgroup takes `rows` rows of its columns, with four accesses of each operand under way.
 struct SlopeArgs {
     const void *dy, *saved;
-    void *dz, *db;        // db: written when one workgroup holds all rows
+    void *dz, *db;        // dz: NULL when only the sums are wanted; db: written when one workgroup holds all rows
     float* sums;          // [workgroups over the rows][N], or NULL when no sums are wanted or db takes them
     int M, N, lanes, rows;
 };
-// S: the type of what was saved, the slope's or the output's
-template <typename T, typename S, bool IS_OUTPUT>
+// HOW: what dy is multiplied by; S: its type
+enum { BY_SLOPE, BY_OUTPUT, BY_NOTHING };   // BY_NOTHING: dz is dy and not written, only the sums are wanted (S is not read)
+template <typename T, typename S, int HOW>
 __global__ __launch_bounds__(256) void slope_kernel(const SlopeArgs A) {
     constexpr int V = PclipVec<T>::N, AHEAD = 4;
     typedef PclipPack<T, V> Pack;
@@ -576,7 +577,8 @@ __global__ __launch_bounds__(256) void slope_kernel(const SlopeArgs A) {
 #pragma unroll
     for (int i = 0; i < V; i++) sum[i] = 0.f;
     auto product = [](T d, S s) {
-        if constexpr (IS_OUTPUT) return __builtin_bit_cast(Bits, s) == 0 ? 0.f : (float)d;   // zero only at +0; NaN, and -0 (see finish), pass
+        if constexpr (HOW == BY_NOTHING) return (float)d;
+        else if constexpr (HOW == BY_OUTPUT) return __builtin_bit_cast(Bits, s) == 0 ? 0.f : (float)d;   // zero only at +0; NaN, and -0 (see finish), pass
         else return (float)d * ((float)s * (1.f / SlopeFormat<T>::SCALE));
     };
     int row = begin + (int)threadIdx.x / A.lanes;
@@ -592,6 +594,7 @@ __global__ __launch_bounds__(256) void slope_kernel(const SlopeArgs A) {
                 x[i] = product(d.v[i], s.v[i]);
                 sum[i] += x[i];
             }
+            if (HOW == BY_NOTHING || !dz) return;
             if (twice == 0) {
                 store_f32<T, V>(dz + at, V, x);
             } else {
@@ -607,14 +610,15 @@ __global__ __launch_bounds__(256) void slope_kernel(const SlopeArgs A) {
             for (int q = 0; q < AHEAD; q++) {
                 const size_t at = (size_t)(row + q * step) * A.N + from;
                 d[q] = *(const Pack*)(dy + at);
-                s[q] = *(const Saved*)(saved + at);
+                if constexpr (HOW != BY_NOTHING) s[q] = *(const Saved*)(saved + at);
             }
 #pragma unroll
             for (int q = 0; q < AHEAD; q++) use(d[q], s[q], (size_t)(row + q * step) * A.N + from);
         }
         for (; row < end; row += step) {
             const size_t at = (size_t)row * A.N + from;
-            use(*(const Pack*)(dy + at), *(const Saved*)(saved + at), at);
+            if constexpr (HOW == BY_NOTHING) use(*(const Pack*)(dy + at), Saved{}, at);
+            else use(*(const Pack*)(dy + at), *(const Saved*)(saved + at), at);
         }
 #pragma unroll
         for (int i = 0; i < V; i++) {   // the columns from c on come first
@@ -630,9 +634,9 @@ __global__ __launch_bounds__(256) void slope_kernel(const SlopeArgs A) {
             for (int i = 0; i < V; i++)
                 if (i < valid) {
                     const size_t at = (size_t)row * A.N + c + i;
-                    const float x = product(dy[at], saved[at]);
+                    const float x = HOW == BY_NOTHING ? (float)dy[at] : product(dy[at], saved[at]);
                     sum[i] += x;
-                    dz[at] = (T)x;
+                    if (HOW != BY_NOTHING && dz) dz[at] = (T)x;
                 }
     }
     if (!A.sums && !A.db) return;
@@ -743,14 +747,18 @@ SlopePlan slope_plan(int M, int N, int dtype) {
     return {lanes, over_n, (int)((M + rows - 1) / rows), (int)rows};
 }
 
-// where the parts of the workspace lie
+// where the parts of the workspace lie; `product`: dW is wanted, `bias_alone`: db without it
 struct BackwardLayout { size_t sums, slab, row_sum, bytes; };   // dz at 0
-BackwardLayout backward_layout(int M, int K, int N, int dtype, int act) {
+BackwardLayout backward_layout(int M, int K, int N, int dtype, int act, bool product, bool bias_alone) {
     BackwardLayout L = {};
-    if (act != PCLIP_ACT_NONE) {
+    if (act != PCLIP_ACT_NONE) L.sums = pclip_align_up((size_t)M * N * pclip_dtype_size(dtype), 256);
+    if (act != PCLIP_ACT_NONE || bias_alone) {
         const SlopePlan s = slope_plan(M, N, dtype);
-        L.sums = pclip_align_up((size_t)M * N * pclip_dtype_size(dtype), 256);
         L.slab = L.sums + (s.over_m > 1 ? pclip_align_up((size_t)s.over_m * N * sizeof(float), 256) : 0);
+    }
+    if (!product) {
+        L.bytes = L.slab;
+        return L;
     }
     const RowPlan p = row_plan(M, K, N, dtype);
     L.row_sum = L.slab + (p.splits > 1 ? pclip_align_up((size_t)p.splits * N * K * sizeof(float), 256) : 0);
@@ -761,19 +769,21 @@ BackwardLayout backward_layout(int M, int K, int N, int dtype, int act) {
 template <typename T>
 int backward(const T* x, const T* w, const T* dy, const void* saved, int is_output, int M, int K, int N, int dtype, int act, T* dx, T* dw, T* db, char* ws,
              hipStream_t st) {
-    const BackwardLayout L = backward_layout(M, K, N, dtype, act);
+    const bool bias_alone = db && !dw;
+    const BackwardLayout L = backward_layout(M, K, N, dtype, act, dw, bias_alone);
     const RowPlan p = row_plan(M, K, N, dtype);
     SlabSum S = {};
     const T* dz = dy;
-    if (act != PCLIP_ACT_NONE) {
+    if (act != PCLIP_ACT_NONE || bias_alone) {
         const SlopePlan s = slope_plan(M, N, dtype);
-        SlopeArgs A = {dy, saved, ws, nullptr, nullptr, M, N, s.lanes, s.rows};
+        SlopeArgs A = {dy, saved, dx || dw ? ws : nullptr, nullptr, nullptr, M, N, s.lanes, s.rows};
         if (db && s.over_m == 1) A.db = db;
         else if (db) A.sums = (float*)(ws + L.sums), S.slab[1] = A.sums, S.out[1] = db, S.n[1] = N, S.splits[1] = s.over_m;
         const dim3 grid(s.over_n, s.over_m);
-        if (is_output) slope_kernel<T, T, true><<<grid, 256, 0, st>>>(A);
-        else slope_kernel<T, SlopeOf<T>, false><<<grid, 256, 0, st>>>(A);
-        dz = (const T*)ws;
+        if (act == PCLIP_ACT_NONE) slope_kernel<T, T, BY_NOTHING><<<grid, 256, 0, st>>>(A);
+        else if (is_output) slope_kernel<T, T, BY_OUTPUT><<<grid, 256, 0, st>>>(A);
+        else slope_kernel<T, SlopeOf<T>, BY_SLOPE><<<grid, 256, 0, st>>>(A);
+        if (act != PCLIP_ACT_NONE) dz = (const T*)ws;
     }
     if (dx) {
         GemmArgs A = {};
@@ -781,8 +791,8 @@ int backward(const T* x, const T* w, const T* dy, const void* saved, int is_outp
         const int rc = launch_rows<T, true, false, EPI_STORE>(A, st);
         if (rc) return rc;
     }
-    const bool sum_here = db && act == PCLIP_ACT_NONE;   // dz is dy, exactly: its sums ride on the product
-    if (dw || sum_here) {
+    if (dw) {
+        const bool sum_here = db && act == PCLIP_ACT_NONE;   // dz is dy, exactly: its sums ride on the product
         GemmArgs A = {};
         A.P = dz, A.Q = x, A.ldp = N, A.ldq = K, A.I = N, A.J = K, A.K = M, A.k_split = p.k_split, A.splits = p.splits;
         A.sum_rows = sum_here;
@@ -790,7 +800,7 @@ int backward(const T* x, const T* w, const T* dy, const void* saved, int is_outp
             A.out = dw, A.slope = sum_here ? db : nullptr;
         } else {
             A.slab = (float*)(ws + L.slab), A.row_sum = (float*)(ws + L.row_sum);
-            if (dw) S.slab[0] = A.slab, S.out[0] = dw, S.n[0] = (long long)N * K, S.splits[0] = p.splits, S.blocks = (int)((S.n[0] + 4 * SUM_LANES[0] - 1) / (4 * SUM_LANES[0]));
+            S.slab[0] = A.slab, S.out[0] = dw, S.n[0] = (long long)N * K, S.splits[0] = p.splits, S.blocks = (int)((S.n[0] + 4 * SUM_LANES[0] - 1) / (4 * SUM_LANES[0]));
             if (sum_here) S.slab[1] = A.row_sum, S.out[1] = db, S.n[1] = N, S.splits[1] = p.splits;
         }
         const int rc = launch_product<T, false, false, EPI_SLAB>(A, p.tile, p.tile, st);
@@ -828,7 +838,8 @@ extern "C" int pclip_linear_fwd(const void* x, const void* w, const void* bias, 
 
 extern "C" size_t pclip_linear_bwd_workspace_bytes(int M, int K, int N, int dtype, int activation) {
     if (check_sizes("linear_bwd", M, K, N, dtype, activation)) return 0;
-    return backward_layout(M, K, N, dtype, activation).bytes;
+    const size_t product = backward_layout(M, K, N, dtype, activation, true, false).bytes, bias = backward_layout(M, K, N, dtype, activation, false, true).bytes;
+    return product > bias ? product : bias;
 }
 
 extern "C" int pclip_linear_bwd(const void* x, const void* w, const void* dy, const void* saved, int saved_is_output, int M, int K, int N, int dtype,
@@ -836,10 +847,10 @@ extern "C" int pclip_linear_bwd(const void* x, const void* w, const void* dy, co
     int rc = check_sizes("linear_bwd", M, K, N, dtype, activation);
     if (rc) return rc;
     PCLIP_REQUIRE(dy && (!dx || w) && (!dw || x), "linear_bwd: null pointer");
-    PCLIP_REQUIRE(x || !db || activation != PCLIP_ACT_NONE, "linear_bwd: the bias gradient runs with the weight's product and needs x");
+    PCLIP_REQUIRE(x || !db || !dx || activation != PCLIP_ACT_NONE, "linear_bwd: dx and db of a layer without activation in one call needs x");
     PCLIP_REQUIRE(activation == PCLIP_ACT_NONE || saved, "linear_bwd: what the forward saved is needed");
     PCLIP_REQUIRE(!saved_is_output || activation == PCLIP_ACT_RELU, "linear_bwd: only relu's slope can be read from the output");
-    const size_t need = pclip_linear_bwd_workspace_bytes(M, K, N, dtype, activation);
+    const size_t need = backward_layout(M, K, N, dtype, activation, dw, db && !dw).bytes;
     PCLIP_REQUIRE(need == 0 || (ws && ws_bytes >= need), "linear_bwd: workspace too small (%zu bytes, need %zu)", ws_bytes, need);
     PCLIP_REQUIRE(((uintptr_t)ws & 15) == 0, "linear_bwd: the workspace must be 16-byte aligned");
     hipStream_t st = (hipStream_t)stream;

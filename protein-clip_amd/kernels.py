@@ -277,24 +277,46 @@ def linear_fwd(x, w, bias=None, residual=None, activation: str = "none", want_sl
     return y, slope
 
 
+def _linear_bwd_sizes(x, w, dy):
+    """The sizes and the type of a backward whose call may lack x or w."""
+    if x is not None and w is not None:
+        return _linear_sizes(x, w)
+    code, N = _typed(dy, "dy"), dy.shape[-1]
+    one = x if w is None else w
+    K = 1 if one is None else one.shape[-1]   # nothing is as wide as the input when neither is there
+    if one is not None and (one.dtype != dy.dtype or one.device != dy.device or not one.is_contiguous() or one.shape != (dy.shape[:-1] if w is None else (N,)) + (K,)):
+        raise _lib.PclipError(f"linear: {tuple(one.shape)} {one.dtype} on {one.device} does not fit dy {tuple(dy.shape)} {dy.dtype} on {dy.device}, "
+                              "or is not contiguous")
+    if not (1 <= K <= LINEAR_MAX_DIM and 1 <= N <= LINEAR_MAX_DIM):
+        raise _lib.PclipError(f"linear: widths {K} -> {N} (1 to {LINEAR_MAX_DIM})")
+    M = dy.numel() // N
+    _check_rows(M, "linear")
+    return M, K, N, code
+
+
 def linear_bwd(x, w, dy, saved=None, saved_is_output: bool = False, activation: str = "none", want_dx: bool = True, want_dw: bool = True,
                want_db: bool = True):
     """Returns (dx, dw, db), None where not wanted.  ``saved``: the forward's slope, or its output with
-    ``saved_is_output`` (relu without a residual), None for activation "none"."""
-    M, K, N, code = _linear_sizes(x, w)
-    dev, dtype, act = x.device, x.dtype, ACTIVATIONS[activation]
-    shape = x.shape[:-1] + (N,)
+    ``saved_is_output`` (relu without a residual), None for activation "none".  ``x`` may be None where dw is not wanted, ``w`` where
+    dx is not."""
+    if (want_dw and x is None) or (want_dx and w is None):
+        raise _lib.PclipError("linear: the weight's gradient needs x, the input's needs the weight")
+    M, K, N, code = _linear_bwd_sizes(x, w, dy)
+    like, act = dy if x is None else x, ACTIVATIONS[activation]
+    dev, dtype, shape = like.device, like.dtype, like.shape[:-1] + (N,)
     g = _operand(dy, "dy", shape, dtype, dev)
     s = _operand(saved, "saved", shape, dtype if saved_is_output else _slope_type(dtype), dev)
+    if want_dx and want_db and x is None and not act:   # the C entry takes these two together with x only
+        return linear_bwd(None, w, dy, want_dw=False, want_db=False)[0], None, linear_bwd(None, None, dy, want_dx=False, want_dw=False)[2]
     lib = _lib.load()
-    dx = _empty_like(x) if want_dx else None
-    dw = _empty_like(w) if want_dw else None
-    db = _empty(w.shape[:1], dtype, dev) if want_db else None
+    dx = _empty(shape[:-1] + (K,), dtype, dev) if want_dx else None
+    dw = _empty((N, K), dtype, dev) if want_dw else None
+    db = _empty((N,), dtype, dev) if want_db else None
     # scratch of the call's own (not the stream's shared buffer): a captured graph keeps it for its replays
     nbytes = lib.pclip_linear_bwd_workspace_bytes(M, K, N, code, act)
     ws = _empty((nbytes,), torch.uint8, dev) if nbytes else None
-    _launch(dev, lib.pclip_linear_bwd, "pclip_linear_bwd", x.data_ptr(), w.data_ptr(), g, s, int(saved_is_output), M, K, N, code, act, ptr(dx), ptr(dw), ptr(db),
-            ptr(ws), nbytes, stream_of(x))
+    _launch(dev, lib.pclip_linear_bwd, "pclip_linear_bwd", ptr(x), ptr(w), g, s, int(saved_is_output), M, K, N, code, act, ptr(dx), ptr(dw), ptr(db),
+            ptr(ws), nbytes, stream_of(dy))
     return dx, dw, db
 
 

@@ -144,12 +144,13 @@ ACTIVATIONS = tuple(_hip_kernels.ACTIVATIONS)
 class _LinearAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, K):
-        product = any(ctx.needs_input_grad[:3])
-        output = activation == "relu" and residual is None   # the sign of y says where the slope is one
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        product = need_x or need_w or need_b
+        output = activation == "relu" and residual is None   # y says where the slope is one
         x, weight = _contiguous(x), _contiguous(weight)
         y, slope = _linear_fwd(x, weight, bias, residual, activation, product and activation != "none" and not output, K)
-        ctx.K, ctx.activation, ctx.output = K, activation, output
-        ctx.save_for_backward(x, weight, y if output and product else slope)
+        ctx.K, ctx.activation, ctx.output, ctx.width = K, activation, output, x.shape[-1]
+        ctx.save_for_backward(x if need_w else None, weight if need_x else None, y if output and product else slope)   # no operand that no gradient reads
         return y
 
     @staticmethod
@@ -158,8 +159,8 @@ class _LinearAct(torch.autograd.Function):
         x, weight, saved = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         dx = dw = db = None
-        if x.numel() == 0:
-            dx, dw, db = torch.zeros_like(x), torch.zeros_like(weight), weight.new_zeros(weight.shape[0])
+        if dy.numel() == 0:
+            dx, dw, db = (dy.new_zeros(s) for s in (dy.shape[:-1] + (ctx.width,), (dy.shape[-1], ctx.width), dy.shape[-1:]))
         elif need_x or need_w or need_b:
             dx, dw, db = ctx.K.linear_bwd(x, weight, _contiguous(dy), saved, ctx.output, ctx.activation, need_x, need_w, need_b)
         return dx if need_x else None, dw if need_w else None, db if need_b else None, dy if need_r else None, None, None

@@ -113,3 +113,20 @@ def test_relu_outputs_too_small_for_their_type(ops):
     # the sum of three products of 512 and x's own values, rounded once
     want = 512 * (x.detach()[:, 0].double().cpu() * kept).sum()
     assert abs(w.grad.item() - want.item()) <= R.half(F16) * want.item()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("rows,width,out", [(1, 8, 3), (37, 24, 40), (64, 16, 16), (65, 7, 5), (5000, 40, 136), (20000, 8, 600)])
+@pytest.mark.parametrize("name", ["none", "relu", "gelu"])
+def test_gradients_of_some_operands_only(ops, t, rows, width, out, name):
+    """The bias alone, with the input, with the weight: each as when all are wanted."""
+    g = torch.Generator().manual_seed(rows)
+    x, w, b, dy = ((torch.randn(*s, generator=g) * f).to(t) for s, f in (((rows, width), 1.0), ((out, width), width ** -0.5), ((out,), 1.0), ((rows, out), 1.0)))
+    want = R.linear_bounds(x.double(), w.double(), b.double(), None, dy.double(), name, t)
+    for mask in (4, 5, 6, 1, 2):
+        leaves = [v.cuda().requires_grad_(bool(mask >> i & 1)) for i, v in enumerate((x, w, b))]
+        y = ops.linear_act(*leaves, activation=name)
+        wanted = [v for v in leaves if v.requires_grad]
+        names = [n for v, n in zip(leaves, ("x", "weight", "bias")) if v.requires_grad]
+        for got, n in zip(torch.autograd.grad(y, wanted, dy.cuda()), names):
+            R.assert_within(got, *want[n], f"{mask}: {n}")

@@ -94,3 +94,38 @@ def test_clipping_is_refused_where_it_would_not_be_seen():
         with pytest.raises((NotImplementedError, RuntimeError)):
             torch.func.vmap(call)(v[None])
     assert torch.equal(v, torch.ones(4)) and ops.grad_norm(iter([v]), kernels=_Raw).item() == 2
+
+
+def _kept(y):
+    """The tensors that a result's graph holds on to, those of its own function only."""
+    return [t for t in y.grad_fn.saved_tensors if t is not None]
+
+
+@pytest.mark.parametrize("activation,res", [("none", False), ("relu", False), ("relu", True), ("gelu", True)])
+def test_linear_keeps_what_its_gradients_read(activation, res):
+    """x for the weight's gradient, the weight for the input's, the slope or the output for any; a frozen operand's partner may change."""
+    from protein_clip_amd import ops
+    for mask in range(1, 8):
+        x, w, b = (torch.ones(*s).requires_grad_(bool(mask >> i & 1)) for i, s in enumerate(((3, 8), (4, 8), (4,))))
+        y = ops.linear_act(x, w, b, torch.ones(3, 4) if res else None, activation=activation, kernels=P)
+        kept = _kept(y)
+        assert any(t is x for t in kept) == bool(mask & 2) and any(t is w for t in kept) == bool(mask & 1)
+        assert len(kept) == bool(mask & 1) + bool(mask & 2) + (activation != "none")
+        with torch.no_grad():
+            if not mask & 2:
+                x.add_(1)
+            if not mask & 1:
+                w.add_(1)
+        grads = torch.autograd.grad(y.sum(), [v for v in (x, w, b) if v.requires_grad])
+        assert [g.shape for g in grads] == [v.shape for v in (x, w, b) if v.requires_grad]
+
+
+def test_bias_gradients_alone_on_the_host():
+    """Which operands the kernels' wrapper wants for which gradient, refused before anything is launched."""
+    from protein_clip_amd import kernels
+    from protein_clip_amd._lib import PclipError
+    x, w, dy = torch.ones(3, 8), torch.ones(4, 8), torch.ones(3, 4)
+    for args, want in (((None, w, dy), (True, True, True)), ((x, None, dy), (True, False, False)), ((None, None, dy), (False, False, True)), ((None, w, dy), (True, False, True)),
+                       ((None, torch.ones(5, 8), dy), (True, False, False))):
+        with pytest.raises(PclipError):
+            kernels.linear_bwd(*args, want_dx=want[0], want_dw=want[1], want_db=want[2])
