@@ -226,9 +226,11 @@ class _NormGate(torch.autograd.Function):
     def forward(ctx, u, r, gate, wa, ba, wb, bb, cfg):
         ctx.set_materialize_grads(False)
         u, r, gate, wa, ba, wb, bb = map(_contiguous, (u, r, gate, wa, ba, wb, bb))
+        _, _, after, before, _, _ = cfg
         y, n, stats = _norm_fwd(u, r, gate, wa, ba, wb, bb, cfg, True)
-        ctx.cfg = cfg
-        ctx.save_for_backward(u, r, gate, wa, ba, wb, bb, stats)
+        # without a norm and the gate's gradient, du is dy through the gate; the residual is read only to make y again for the second norm
+        ctx.cfg, ctx.plain = cfg, after is None and before is None and not ctx.needs_input_grad[2]
+        ctx.save_for_backward(None if ctx.plain else u, r if before else None, gate, wa, ba, wb, bb, stats)
         return y if n is None else (y, n)
 
     @staticmethod
@@ -237,11 +239,17 @@ class _NormGate(torch.autograd.Function):
         u, r, gate, wa, ba, wb, bb, stats = ctx.saved_tensors
         gate_rows, scale, after, before, eps, K = ctx.cfg
         need = ctx.needs_input_grad[:7]
-        if dy is None and dn is None:
+        like = dn if dy is None else dy
+        if like is None:
             return (None,) * 8
-        if u.numel() == 0:
-            return tuple(torch.zeros_like(t) if w else None for t, w in zip((u, r, gate, wa, ba, wb, bb), need)) + (None,)
-        return K.norm_gate_bwd(u, r, gate, gate_rows, scale, after, wa, ba, before, wb, bb, eps, stats, _contiguous(dy), _contiguous(dn), need) + (None,)
+        if like.numel() == 0:
+            return tuple(torch.zeros_like(t) if w else None for t, w in zip((like, like, gate, wa, ba, wb, bb), need)) + (None,)
+        dy, dn = _contiguous(dy), _contiguous(dn)
+        dr = dy if need[1] and not before else None
+        if ctx.plain:
+            return (K.norm_gate_fwd(dy, None, gate, gate_rows, scale)[0] if need[0] else None, dr) + (None,) * 6
+        grads = K.norm_gate_bwd(u, r, gate, gate_rows, scale, after, wa, ba, before, wb, bb, eps, stats, dy, dn, (need[0], need[1] and dr is None, *need[2:]))
+        return (grads[0], grads[1] if dr is None else dr, *grads[2:], None)
 
 
 def _norm_fwd(u, r, gate, wa, ba, wb, bb, cfg, want_stats):

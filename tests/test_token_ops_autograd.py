@@ -129,3 +129,34 @@ def test_bias_gradients_alone_on_the_host():
                        ((None, torch.ones(5, 8), dy), (True, False, False))):
         with pytest.raises(PclipError):
             kernels.linear_bwd(*args, want_dx=want[0], want_dw=want[1], want_db=want[2])
+
+
+@pytest.mark.parametrize("after", [None, "norm"])
+@pytest.mark.parametrize("before", [None, "norm"])
+@pytest.mark.parametrize("gate", [None, "mask", "learned"])
+def test_norm_gate_keeps_what_its_gradients_read(after, before, gate):
+    """The residual only for the second norm; the block's output only where a norm or the gate's gradient reads it.  What is not kept may be
+    changed in place before the backward."""
+    from protein_clip_amd import ops
+    g = torch.Generator().manual_seed(3)
+    make = lambda: torch.randn(5, 8, generator=g)
+    u, r, dy, dn = make().requires_grad_(True), make().requires_grad_(True), make(), make()
+    gt = {None: None, "mask": make() > 0, "learned": torch.randn(8, generator=g).requires_grad_(True)}[gate]
+    w = torch.randn(8, generator=g).requires_grad_(True)
+    pair = lambda on: None if on is None else (w, None)
+    want = P._norm_gate(u, r, gt, 1 if gate != "learned" else 5, 0.5, after and "layer", w, None, before and "layer", w, None, 1e-5)
+    leaves = [t for t in (u, r, gt, w) if t is not None and t.requires_grad and (t is not w or after or before)]
+    cot = (dy, dn) if before else (dy,)
+    refs = torch.autograd.grad([o for o in want if o is not None], leaves, cot)
+    outs = ops.norm_gate_residual(u, r, gt, scale=0.5, after=pair(after), before=pair(before), kernels=P)
+    outs = outs if before else (outs,)
+    kept = _kept(outs[0])
+    assert any(t is r for t in kept) == bool(before)
+    assert any(t is u for t in kept) == bool(after or before or gate == "learned")
+    with torch.no_grad():
+        if not before:
+            r.add_(1)
+        if not (after or before or gate == "learned"):
+            u.add_(1)
+    for got, ref in zip(torch.autograd.grad(outs, leaves, cot), refs):
+        torch.testing.assert_close(got, ref, rtol=1e-4, atol=1e-5)
