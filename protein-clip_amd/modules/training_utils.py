@@ -140,13 +140,13 @@ def _sum_head_grads(model, group=None, max_grad_norm=None):
         return
     flat = torch.cat([g.reshape(-1) for g in grads])
     dist.all_reduce(flat, group=group)
+    parts = [v.view(g.shape) for v, g in zip(flat.split([g.numel() for g in grads]), grads)]
     if max_grad_norm is not None:
-        ops.clip_grads([v.view(g.shape) for v, g in zip(flat.split([g.numel() for g in grads]), grads)], max_grad_norm, out=grads)
-        return
-    offset = 0
-    for g in grads:
-        g.copy_(flat[offset:offset + g.numel()].view_as(g))
-        offset += g.numel()
+        # straight into the gradients; one of another layout than its part is clipped in the part and copied like the others without clipping
+        ops.clip_grads(parts, max_grad_norm, out=[g if g.is_contiguous() else v for v, g in zip(parts, grads)])
+    for v, g in zip(parts, grads):
+        if max_grad_norm is None or not g.is_contiguous():
+            g.copy_(v)
 
 
 def train_gc(model, data_loader, tokenizer, optimizer, scaler, device, accumulated_batches=1, group=None, max_grad_norm=None):

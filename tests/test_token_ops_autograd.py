@@ -160,3 +160,40 @@ def test_norm_gate_keeps_what_its_gradients_read(after, before, gate):
             u.add_(1)
     for got, ref in zip(torch.autograd.grad(outs, leaves, cot), refs):
         torch.testing.assert_close(got, ref, rtol=1e-4, atol=1e-5)
+
+
+class _Strict(_Raw):
+    """Takes what the kernels take: a destination of its source's layout, without gaps."""
+
+    @staticmethod
+    def grad_clip(src, dst=None, max_norm=0.0, eps=1e-6):
+        from protein_clip_amd import kernels
+        for s, d in zip(src, dst or []):
+            assert kernels._dense(s) and kernels._dense(d) and s.shape == d.shape and (s.stride() == d.stride() or s.is_contiguous() and d.is_contiguous())
+        return _Raw.grad_clip(src, dst, max_norm, eps)
+
+
+def test_summed_gradients_of_any_layout_are_clipped(monkeypatch):
+    """The way back from the flat buffer of the sum over ranks: with a limit, gradients of every layout that it fills without one, also those
+    with gaps, and the norm is the sum's."""
+    from protein_clip_amd import ops
+    from protein_clip_amd.modules import training_utils as U
+    monkeypatch.setattr(ops, "_hip_kernels", _Strict)
+    monkeypatch.setattr(U.dist, "all_reduce", lambda t, group=None: t.mul_(2))   # two ranks with the same gradients
+
+    def model():
+        g = torch.Generator().manual_seed(0)
+        m = torch.nn.ParameterList([torch.nn.Parameter(torch.zeros(s)) for s in ((6, 4), (3, 2, 5), (7,), (4, 4), (5,))])
+        for p, lay in zip(m, (lambda v: v.t().contiguous().t(), lambda v: v.permute(2, 0, 1).contiguous().permute(1, 2, 0), lambda v: v, lambda v: torch.stack([v, v], 2)[:, :, 0],
+                              lambda v: v)):
+            p.grad = lay(torch.randn(p.shape, generator=g))
+        return m
+
+    free, clipped = model(), model()
+    strides = [p.grad.stride() for p in clipped]
+    U._sum_head_grads(free)
+    U._sum_head_grads(clipped, max_grad_norm=0.5)
+    size = torch.sqrt(sum((p.grad.double() ** 2).sum() for p in free)).item()
+    for p, q, st in zip(free, clipped, strides):
+        torch.testing.assert_close(q.grad, p.grad * (0.5 / size), rtol=1e-5, atol=1e-7)
+        assert q.grad.stride() == st
