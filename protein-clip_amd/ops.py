@@ -366,9 +366,10 @@ def clip_grads(grads, max_norm: float, out=None, eps: float = 1e-6, kernels=None
     return norm
 
 
-def clip_grad_norm_(parameters, max_norm: float, eps: float = 1e-6, error_if_nonfinite: bool = False, kernels=None) -> torch.Tensor:
-    """Clips the gradients of ``parameters`` (an iterable of tensors, or one) in place and returns their norm before clipping, as
-    ``torch.nn.utils.clip_grad_norm_`` does; parameters without a gradient are left out.  With
+def clip_grad_norm_(parameters, max_norm: float, *, eps: float = 1e-6, error_if_nonfinite: bool = False, kernels=None) -> torch.Tensor:
+    """Clips the gradients of ``parameters`` (an iterable of tensors, or one) in place and returns their L2 norm before clipping, as
+    ``torch.nn.utils.clip_grad_norm_`` does (whose third argument by position, the norm's type, is not taken: the norm is
+    the L2 norm); parameters without a gradient are left out.  With
     ``error_if_nonfinite`` the norm is read by the host first and the gradients stay as they are when it is not finite."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = [p.grad for p in parameters if p.grad is not None]

@@ -197,3 +197,14 @@ def test_summed_gradients_of_any_layout_are_clipped(monkeypatch):
     for p, q, st in zip(free, clipped, strides):
         torch.testing.assert_close(q.grad, p.grad * (0.5 / size), rtol=1e-5, atol=1e-7)
         assert q.grad.stride() == st
+
+
+def test_clip_grad_norm_takes_no_third_argument_by_position():
+    """torch's own function has the norm's type there: a call written for it must not set eps in silence."""
+    from protein_clip_amd import ops
+    p = torch.nn.Parameter(torch.zeros(4))
+    p.grad = torch.ones(4)
+    with pytest.raises(TypeError):
+        ops.clip_grad_norm_([p], 1.0, 2.0, kernels=_Raw)
+    assert torch.equal(p.grad, torch.ones(4))
+    assert ops.clip_grad_norm_([p], 1.0, eps=0.0, error_if_nonfinite=True, kernels=_Raw).item() == 2 and torch.equal(p.grad, torch.full((4,), 0.5))
