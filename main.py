@@ -26,7 +26,8 @@ def main():
     tokenizer, esm_model, input_dim, _ = entry.load_trunk(args, device)
     embedding_dim, h1, h2, dropout = 128, 2, 2, 0.1
     loaders = entry.make_loaders(args, rank)
-    scaler = GradScaler("cuda", enabled=False)  # the loss kernels are f32: nothing to scale
+    # the loss kernels are f32, so only the gradients of a float16 token head need scaling
+    scaler = GradScaler("cuda", enabled=args.token_dtype == "f16" and torch.cuda.is_available())
 
     def build():
         return models.ExtendedCLIP(input_dim, embedding_dim, h1, h2, dropout, esm_model, entry.TOKEN_DTYPES[args.token_dtype])

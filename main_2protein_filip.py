@@ -12,6 +12,7 @@ import os
 import sys
 
 import torch
+from torch.amp import GradScaler
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 import protein_clip_amd  # noqa: E402,F401
@@ -26,12 +27,14 @@ def main():
     tokenizer, esm_model, input_dim, _ = entry.load_trunk(args, device)
     embedding_dim, h1, h2, dropout = 128, 2, 2, 0.1
     loaders = entry.make_loaders(args, rank, pep_len=(50, args.max_len))   # both chains are proteins
+    # the score and loss kernels take and give f32, so only the gradients of a float16 token head need scaling
+    scaler = GradScaler("cuda", enabled=args.token_dtype == "f16" and torch.cuda.is_available())
 
     def build():
         return models.ExtendedFILIP(input_dim, embedding_dim, h1, h2, dropout, esm_model, entry.TOKEN_DTYPES[args.token_dtype])
 
     def train_epoch(model, loader, optimizer):
-        return training_utils_filip.train(model, loader, optimizer, tokenizer, device, max_grad_norm=args.max_grad_norm)
+        return training_utils_filip.train(model, loader, optimizer, tokenizer, device, max_grad_norm=args.max_grad_norm, scaler=scaler)
 
     def evaluate(model, loader):
         return training_utils_filip.evaluate(model, loader, tokenizer, device)

@@ -47,41 +47,72 @@ def _tokenise(tokenizer, sequences, device):
     return tokenizer(sequences, return_tensors="pt", padding=True).to(device)
 
 
-def _process_batch(model, batch_data, tokenizer, device, compute_grad=False):
+def _process_batch(model, batch_data, tokenizer, device, compute_grad=False, scaler=None):
     peptides, receptors = batch_data
     pep, rec = model(_tokenise(tokenizer, peptides, device), _tokenise(tokenizer, receptors, device))
     loss = _contrastive_loss(pep, rec.t())
     if compute_grad:
-        loss.backward()
+        _backward(loss, scaler)
     return loss.item()
+
+
+def _loss_scaler(model, scaler, device):
+    """The scaler that a loop's backward runs under: the caller's, or one of the loop's own where that scales nothing and the towers' token
+    heads compute in float16: the gradients of a mean over batch and tokens, 1e-7 or so an element, would lie among float16's
+    subnormal numbers (steps of 6e-8) or below them."""
+    if scaler is not None and scaler.is_enabled():
+        return scaler
+    if any(getattr(m, "token_dtype", None) == torch.float16 for m in model.modules()):
+        return torch.amp.GradScaler(torch.device(device).type)
+    return scaler
+
+
+def _backward(loss, scaler):
+    (loss if scaler is None else scaler.scale(loss)).backward()
 
 
 def _distributed() -> bool:
     return dist.is_available() and dist.is_initialized() and dist.get_world_size() > 1
 
 
-def _finish_grads(model, max_grad_norm=None):
-    """What lies between the backward and the optimizer's step: the sum over the ranks and, when asked for, the
-    clipping of the global gradient norm (of the sum, so that every rank scales by the same factor)."""
+def _clip(model, optimizer, max_grad_norm, scaler=None):
+    """Clips the gradients of the model's parameters; under a scaler those that the optimizer steps, which are the ones it unscales."""
+    parameters = model.parameters()
+    if scaler is not None and scaler.is_enabled():
+        scaler.unscale_(optimizer)
+        parameters = [p for group in optimizer.param_groups for p in group["params"]]
+    ops.clip_grad_norm_(parameters, max_grad_norm)
+
+
+def _finish_step(model, optimizer, max_grad_norm=None, scaler=None):
+    """What follows a backward: the sum over the ranks, when asked for the clipping of the global gradient norm (of the sum, so that
+    every rank scales by the same factor, and without the loss's scale), and the optimizer's step."""
+    scaled = scaler is not None and scaler.is_enabled()
     if _distributed():
-        _sum_head_grads(model, max_grad_norm=max_grad_norm)
-    elif max_grad_norm is not None:
-        ops.clip_grad_norm_(model.parameters(), max_grad_norm)
+        _sum_head_grads(model, max_grad_norm=None if scaled else max_grad_norm)
+    if max_grad_norm is not None and (scaled or not _distributed()):
+        _clip(model, optimizer, max_grad_norm, scaler)
+    if scaled:
+        scaler.step(optimizer)
+        scaler.update()
+    else:
+        optimizer.step()
 
 
-def train(model, data_loader, optimizer, tokenizer, device, max_grad_norm=None):
+def train(model, data_loader, optimizer, tokenizer, device, max_grad_norm=None, scaler=None):
     """One epoch, one optimizer step per batch; returns the mean batch loss.  Under
     ``torch.distributed`` the loss of a batch spans the batches of all ranks (all-gather inside
     the loss) and every rank back-propagates its own rows, so the head gradients are summed over
     the ranks before the step.  ``max_grad_norm``: clip the global gradient norm to this (None: no clipping,
-    as in the reference)."""
+    as in the reference).  ``scaler``: a ``torch.amp.GradScaler`` for the loss; towers with float16 token heads get one for the
+    epoch when there is none."""
     model.train()
+    scaler = _loss_scaler(model, scaler, device)
     running = 0.0
     for batch in data_loader:
         optimizer.zero_grad()
-        running += _process_batch(model, batch, tokenizer, device, compute_grad=True)
-        _finish_grads(model, max_grad_norm)
-        optimizer.step()
+        running += _process_batch(model, batch, tokenizer, device, compute_grad=True, scaler=scaler)
+        _finish_step(model, optimizer, max_grad_norm, scaler)
     return running / len(data_loader)
 
 
@@ -153,8 +184,10 @@ def train_gc(model, data_loader, tokenizer, optimizer, scaler, device, accumulat
     """Big-batch epoch (training_utils.py:92-155): every ``accumulated_batches`` sub-batches
     form one contrastive batch and one optimizer step.  Trailing sub-batches that do not fill
     a batch are encoded and dropped, as in the reference.  ``max_grad_norm``: as in :func:`train`, applied to
-    the unscaled gradients.  Returns the mean big-batch loss."""
+    the unscaled gradients.  ``scaler``: one that is not enabled is replaced, for the epoch, where the towers' token heads are
+    float16.  Returns the mean big-batch loss."""
     model.train()
+    scaler = _loss_scaler(model, scaler, device)
     distributed = _distributed()
     total, big_batches = 0.0, 0
     pending = []
@@ -180,8 +213,7 @@ def train_gc(model, data_loader, tokenizer, optimizer, scaler, device, accumulat
         if distributed:
             _sum_head_grads(model, group)
         if max_grad_norm is not None:
-            scaler.unscale_(optimizer)
-            ops.clip_grad_norm_(model.parameters(), max_grad_norm)
+            _clip(model, optimizer, max_grad_norm, scaler)
         scaler.step(optimizer)
         scaler.update()
         optimizer.zero_grad()
