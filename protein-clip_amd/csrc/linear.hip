@@ -263,6 +263,12 @@ __device__ __forceinline__ int xcd_order(int b, int n) {
     return xcd * q + min(xcd, r) + (b >> 3);
 }
 
+// between the writes and the reads of LDS by which the lanes of a wave exchange values, and before the next writes
+__device__ __forceinline__ void wave_exchange() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // What a wave does with its accumulators: rows from i0, columns from j0 on.
 template <typename T, int FI, int FJ, int EPI>
 __device__ __forceinline__ void finish(const GemmArgs& A, f32x4 (&acc)[FI][FJ], f32x4 (&ones)[FI / 2], bool sum_rows, char* lds, int i0, int j0, int split) {
@@ -291,7 +297,8 @@ __device__ __forceinline__ void finish(const GemmArgs& A, f32x4 (&acc)[FI][FJ], 
         }
     } else {
         // 16 rows at a time through LDS (a wave's own part of it), after which a lane holds the V columns of one 16-byte access and
-        // neighbouring lanes neighbouring ones: whole lines are written, and read of the residual
+        // neighbouring lanes neighbouring ones: whole lines are written, and read of the residual.  Only lanes of one wave exchange values,
+        // whose LDS accesses are executed in order: wave_exchange keeps the compiler to that order, and no instruction comes of it
         constexpr int V = PclipVec<T>::N, WC = FJ * 16, PITCH = WC + 4, LANES = WC / V, ROWS = 64 / LANES;
         __syncthreads();
         float* own = (float*)lds + (threadIdx.x >> 6) * 16 * PITCH;
@@ -306,6 +313,7 @@ __device__ __forceinline__ void finish(const GemmArgs& A, f32x4 (&acc)[FI][FJ], 
         for (int fi = 0; fi < FI; fi++) {
 #pragma unroll
             for (int fj = 0; fj < FJ; fj++) *(f32x4*)(own + (lane & 15) * PITCH + fj * 16 + (lane >> 4) * 4) = acc[fi][fj];
+            wave_exchange();
 #pragma unroll
             for (int first = 0; first < 16; first += ROWS) {
                 const int row = first + lane / LANES, i = i0 + fi * 16 + row;
@@ -333,6 +341,7 @@ __device__ __forceinline__ void finish(const GemmArgs& A, f32x4 (&acc)[FI][FJ], 
                 }
                 stream_f32<T, V>((T*)A.out + at, left, v);
             }
+            wave_exchange();
         }
     }
 }
