@@ -203,7 +203,7 @@ struct GemmArgs {
     const void *P, *Q;
     int ldp, ldq, I, J;
     long long K, k_split;           // contraction length, and the part of one workgroup (a multiple of KSTEP)
-    int tiles_i, tiles_j, splits;
+    int tiles_i, tiles_j, splits, blocks;   // blocks: tiles of all splits
     const void *bias, *residual;    // forward
     void *out, *slope;
     float *slab, *row_sum;          // EPI_SLAB: [splits][I][J], [splits][I]; slab NULL (one split): straight into out and slope
@@ -256,6 +256,11 @@ struct Runs {
         }
     }
 };
+
+// A launch has fewer than 2^32 threads, and a column of 2^31 rows has more tiles than that: workgroups lie in planes of PLANE (a
+// multiple of eight, so that the order below goes on over their border), of which the last may hold some that have no tile.
+constexpr int PLANE = 1 << 23;
+__device__ __forceinline__ int workgroup() { return (int)(blockIdx.y * PLANE + blockIdx.x); }
 
 // Workgroups go to the eight XCDs in turn; give each XCD a run of neighbouring tiles, which share rows of P or Q in its L2.
 __device__ __forceinline__ int xcd_order(int b, int n) {
@@ -356,7 +361,8 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_kernel(const GemmArgs A)
     extern __shared__ __attribute__((aligned(16))) char lds[];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int b = xcd_order(blockIdx.x, gridDim.x);
+    if (workgroup() >= A.blocks) return;
+    int b = xcd_order(workgroup(), A.blocks);
     const int tj = b % A.tiles_j;
     b /= A.tiles_j;
     const int ti = b % A.tiles_i, split = b / A.tiles_i;
@@ -451,7 +457,8 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_direct_kernel(const Gemm
     extern __shared__ __attribute__((aligned(16))) char lds[];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int b = xcd_order(blockIdx.x, gridDim.x);
+    if (workgroup() >= A.blocks) return;
+    int b = xcd_order(workgroup(), A.blocks);
     const int tj = b % A.tiles_j;
     b /= A.tiles_j;
     const int ti = b % A.tiles_i, split = b / A.tiles_i;
@@ -675,8 +682,10 @@ int launch_tile(GemmArgs A, hipStream_t st) {
     A.tiles_j = (A.J + BJ - 1) / BJ;
     const long long blocks = (long long)A.tiles_i * A.tiles_j * A.splits;
     PCLIP_REQUIRE(blocks <= 0x7fffffffll, "linear: too many tiles (%lld)", blocks);
-    if constexpr (DIRECT) gemm_direct_kernel<T, BI, BJ, 2, 2, PK, QK, EPI><<<(int)blocks, 256, bytes, st>>>(A);
-    else gemm_kernel<T, BI, BJ, 2, 2, PK, QK, EPI><<<(int)blocks, 256, bytes, st>>>(A);
+    A.blocks = (int)blocks;
+    const dim3 grid(A.blocks < PLANE ? A.blocks : PLANE, (unsigned)((blocks + PLANE - 1) / PLANE));
+    if constexpr (DIRECT) gemm_direct_kernel<T, BI, BJ, 2, 2, PK, QK, EPI><<<grid, 256, bytes, st>>>(A);
+    else gemm_kernel<T, BI, BJ, 2, 2, PK, QK, EPI><<<grid, 256, bytes, st>>>(A);
     return PCLIP_OK;
 }
 

@@ -67,3 +67,23 @@ def test_float16_heads_train_under_a_scaled_loss(ops, kind):
     off = lambda a, b: (sum(((a[n] - b[n]).double() ** 2).sum() for n in b) / sum((b[n].double() ** 2).sum() for n in b)).sqrt().item()
     want = by_hand(2.0 ** 16)
     assert off(seen, want) < 1e-3 < off(by_hand(1.0), want)
+
+
+def test_linear_of_more_rows_than_a_grid_has_threads(ops):
+    """Narrow layers of more than 2^30 rows, up to the most that is accepted: 2^24 tiles of 64 rows and more, all of them reached."""
+    for rows, back in ((2**30 + 200, True), (2**31 - 2**16, False)):
+        x = torch.zeros(rows, 1, dtype=torch.float16, device="cuda")
+        at = torch.tensor([0, 63, 64, 2**23 * 64 - 1, 2**23 * 64, 2**29 + 5, 2**30 - 1, 2**30, 2**30 + 70, rows - 1], device="cuda")
+        x[at, 0] = torch.arange(1, 11, device="cuda").half()
+        w = torch.full((1, 1), 0.5, dtype=torch.float16, device="cuda", requires_grad=back)
+        x.requires_grad_(back)
+        y = ops.linear_act(x, w)
+        assert torch.equal(y[at, 0].float(), torch.arange(1, 11, device="cuda") * 0.5) and y.count_nonzero().item() == 10
+        if back:
+            with torch.no_grad():
+                dy = y.detach().fill_(2.0)
+            dx, dw = torch.autograd.grad(y, (x, w), dy)
+            assert dw.item() == 2 * 55 and (dx == 1).all()
+            del dx, dy
+        del x, y
+    torch.cuda.empty_cache()
