@@ -53,6 +53,8 @@ __device__ __forceinline__ void load_direct(const void* base, unsigned offset, c
 #endif
 }
 
+constexpr int VMCNT_0 = 0x0F70;   // s_waitcnt: no vector memory access under way; the other counters as they are
+
 template <typename T, int ROWS, bool ALONG_K>
 struct Tile {
     static constexpr int V = PclipVec<T>::N;
@@ -503,6 +505,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_direct_kernel(const Gemm
 
     fetch(k_first);
     for (long long k = k_first; k < k_end; k += KSTEP<T>) {
+        __builtin_amdgcn_s_waitcnt(VMCNT_0);   // this wave's part of the tile has arrived in LDS (the barrier's own fence waits for it as well)
         __syncthreads();   // every wave's part of the tile is there
         Frag fp[2][FI], fq[2][FJ];
 #pragma unroll
