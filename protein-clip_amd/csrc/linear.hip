@@ -333,10 +333,11 @@ __device__ __forceinline__ void finish(const GemmArgs& A, f32x4 (&acc)[FI][FJ], 
                     float slope[V];
 #pragma unroll
                     for (int e = 0; e < V; e++) v[e] = activate<sizeof(T) == 4, EPI>(v[e] + bias[e], slope[e]);
-                    if constexpr (EPI == PCLIP_ACT_RELU && sizeof(T) == 2) {
-                        // the backward reads the slope from the output: a value above zero that rounds to zero becomes -0
+                    if constexpr (EPI == PCLIP_ACT_RELU && std::is_same_v<T, _Float16>) {
+                        // the backward reads the slope from the output: a value above zero that rounds to zero becomes -0 (bfloat16 reaches
+                        // as far down as the f32 sums do)
 #pragma unroll
-                        for (int e = 0; e < V; e++) v[e] = v[e] > 0.f && (float)(T)v[e] == 0.f ? -0.f : v[e];
+                        for (int e = 0; e < V; e++) v[e] = v[e] > 0.f && v[e] <= 0x1p-25f ? -0.f : v[e];
                     }
                     if (A.slope) store_slope<T, V>((SlopeOf<T>*)A.slope + at, left, slope);
                     if (A.residual) {
