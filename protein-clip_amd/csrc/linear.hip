@@ -699,19 +699,19 @@ template <typename T, bool DIRECT, bool PK, bool QK, int EPI>
 int launch_size(const GemmArgs& A, int bi, int bj, hipStream_t st) {
     if constexpr (DIRECT && EPI != EPI_SLAB && sizeof(T) == 2)
         if (bi == 256) return launch_tile<T, 256, 128, DIRECT, PK, QK, EPI>(A, st);
-    if constexpr (EPI == EPI_SLAB || sizeof(T) == 2)   // f32 rows go in small tiles only, see launch_rows
+    if constexpr ((EPI == EPI_SLAB && DIRECT) || sizeof(T) == 2)   // f32 rows go in small tiles only, see launch_rows and row_plan
         if (bi >= 128) return launch_tile<T, 128, 128, DIRECT, PK, QK, EPI>(A, st);
     return launch_tile<T, 64, 64, DIRECT, PK, QK, EPI>(A, st);
 }
 // whether every row of both operands begins at a multiple of 16 bytes
 template <typename T>
-bool direct(const GemmArgs& A) {
-    const uintptr_t bits = (uintptr_t)A.P | (uintptr_t)A.Q | (uintptr_t)A.ldp * sizeof(T) | (uintptr_t)A.ldq * sizeof(T);
+bool direct(const void* P, const void* Q, int ldp, int ldq) {
+    const uintptr_t bits = (uintptr_t)P | (uintptr_t)Q | (uintptr_t)ldp * sizeof(T) | (uintptr_t)ldq * sizeof(T);
     return (bits & 15) == 0;
 }
 template <typename T, bool PK, bool QK, int EPI>
 int launch_product(const GemmArgs& A, int bi, int bj, hipStream_t st) {
-    return direct<T>(A) ? launch_size<T, true, PK, QK, EPI>(A, bi, bj, st) : launch_size<T, false, PK, QK, EPI>(A, bi, bj, st);
+    return direct<T>(A.P, A.Q, A.ldp, A.ldq) ? launch_size<T, true, PK, QK, EPI>(A, bi, bj, st) : launch_size<T, false, PK, QK, EPI>(A, bi, bj, st);
 }
 
 // Forward and dx: the tile whose workgroups are done first.  A compute unit's share is its number of workgroups times the tile's
@@ -736,13 +736,16 @@ int launch_rows(const GemmArgs& A, hipStream_t st) {
 
 // The product over the rows (dW): tile size, the number of splits and their length.  The tile is 128 x 128, or 64 x 64 where a side is
 // no longer, and for f32 with few tiles: 16 waves then share a compute unit instead of 8 (4096 x 640 -> 128: 22 us instead
-// of 28; 16,384 x 1280 -> 1280, a hundred tiles: 658 instead of 492).
+// of 28; 16,384 x 1280 -> 1280, a hundred tiles: 658 instead of 492), and where f32 operands are staged, whose fetched registers and the
+// runs' sums of a 128 x 128 tile do not fit (spilled, 16,383 x 1283 -> 1279 846 us instead of 674; 600 x 2049 -> 2047 120 instead of 79).
 struct RowPlan { int tile, splits; long long k_split; };
-RowPlan row_plan(int M, int K, int N, int dtype) {
+RowPlan row_plan(int M, int K, int N, int dtype, bool staged) {
     const bool f32 = dtype == PCLIP_DT_F32;
-    const int step = f32 ? 32 : 64, tile = K > 64 && N > 64 && !(f32 && tiles(N, K, 128, 128) <= 16) ? 128 : 64;
+    const int step = f32 ? 32 : 64, tile = K > 64 && N > 64 && !(f32 && (staged || tiles(N, K, 128, 128) <= 16)) ? 128 : 64;
     const long long t = tiles(N, K, tile, tile), steps = ((long long)M + step - 1) / step;
-    long long s = 512 / t;                          // two workgroups a compute unit, in one round
+    // two workgroups a compute unit, in one round; of the small staged tiles four, and eight in rounds where the tiles alone leave the last
+    // round half empty (16,383 x 1283 -> 1279: 980 us with two, 817 with four, 674 with eight; 16,384 x 1281 -> 200: 154, 144, 143)
+    long long s = (!(f32 && staged) ? 512 : t > 256 ? 2048 : 1024) / t;
     if (s > (steps + 3) / 4) s = (steps + 3) / 4;   // four steps a workgroup at least
     if (s < 1) s = 1;
     const long long per = (steps + s - 1) / s;
@@ -771,7 +774,7 @@ SlopePlan slope_plan(int M, int N, int dtype) {
 
 // where the parts of the workspace lie; `product`: dW is wanted, `bias_alone`: db without it
 struct BackwardLayout { size_t sums, slab, row_sum, bytes; };   // dz at 0
-BackwardLayout backward_layout(int M, int K, int N, int dtype, int act, bool product, bool bias_alone) {
+BackwardLayout backward_layout(int M, int K, int N, int dtype, int act, bool product, bool bias_alone, bool staged) {
     BackwardLayout L = {};
     if (act != PCLIP_ACT_NONE) L.sums = pclip_align_up((size_t)M * N * pclip_dtype_size(dtype), 256);
     if (act != PCLIP_ACT_NONE || bias_alone) {
@@ -782,7 +785,7 @@ BackwardLayout backward_layout(int M, int K, int N, int dtype, int act, bool pro
         L.bytes = L.slab;
         return L;
     }
-    const RowPlan p = row_plan(M, K, N, dtype);
+    const RowPlan p = row_plan(M, K, N, dtype, staged);
     L.row_sum = L.slab + (p.splits > 1 ? pclip_align_up((size_t)p.splits * N * K * sizeof(float), 256) : 0);
     L.bytes = L.row_sum + (p.splits > 1 && act == PCLIP_ACT_NONE ? (size_t)p.splits * N * sizeof(float) : 0);
     return L;
@@ -790,10 +793,12 @@ BackwardLayout backward_layout(int M, int K, int N, int dtype, int act, bool pro
 
 template <typename T>
 int backward(const T* x, const T* w, const T* dy, const void* saved, int is_output, int M, int K, int N, int dtype, int act, T* dx, T* dw, T* db, char* ws,
-             hipStream_t st) {
+             size_t ws_bytes, hipStream_t st) {
     const bool bias_alone = db && !dw;
-    const BackwardLayout L = backward_layout(M, K, N, dtype, act, dw, bias_alone);
-    const RowPlan p = row_plan(M, K, N, dtype);
+    const bool staged = !direct<T>(act == PCLIP_ACT_NONE ? dy : (const T*)ws, x, N, K);
+    const BackwardLayout L = backward_layout(M, K, N, dtype, act, dw, bias_alone, staged);
+    if (L.bytes > ws_bytes) return pclip_fail(PCLIP_EINVAL, "linear_bwd: workspace too small (%zu bytes, need %zu)", ws_bytes, L.bytes);
+    const RowPlan p = row_plan(M, K, N, dtype, staged);
     SlabSum S = {};
     const T* dz = dy;
     if (act != PCLIP_ACT_NONE || bias_alone) {
@@ -860,8 +865,12 @@ extern "C" int pclip_linear_fwd(const void* x, const void* w, const void* bias, 
 
 extern "C" size_t pclip_linear_bwd_workspace_bytes(int M, int K, int N, int dtype, int activation) {
     if (check_sizes("linear_bwd", M, K, N, dtype, activation)) return 0;
-    const size_t product = backward_layout(M, K, N, dtype, activation, true, false).bytes, bias = backward_layout(M, K, N, dtype, activation, false, true).bytes;
-    return product > bias ? product : bias;
+    size_t most = 0;   // whichever gradients are wanted, at whatever addresses
+    for (int k = 0; k < 3; k++) {
+        const size_t bytes = backward_layout(M, K, N, dtype, activation, k > 0, k == 0, k == 2).bytes;
+        if (bytes > most) most = bytes;
+    }
+    return most;
 }
 
 extern "C" int pclip_linear_bwd(const void* x, const void* w, const void* dy, const void* saved, int saved_is_output, int M, int K, int N, int dtype,
@@ -872,11 +881,9 @@ extern "C" int pclip_linear_bwd(const void* x, const void* w, const void* dy, co
     PCLIP_REQUIRE(x || !db || !dx || activation != PCLIP_ACT_NONE, "linear_bwd: dx and db of a layer without activation in one call needs x");
     PCLIP_REQUIRE(activation == PCLIP_ACT_NONE || saved, "linear_bwd: what the forward saved is needed");
     PCLIP_REQUIRE(!saved_is_output || activation == PCLIP_ACT_RELU, "linear_bwd: only relu's slope can be read from the output");
-    const size_t need = backward_layout(M, K, N, dtype, activation, dw, db && !dw).bytes;
-    PCLIP_REQUIRE(need == 0 || (ws && ws_bytes >= need), "linear_bwd: workspace too small (%zu bytes, need %zu)", ws_bytes, need);
     PCLIP_REQUIRE(((uintptr_t)ws & 15) == 0, "linear_bwd: the workspace must be 16-byte aligned");
     hipStream_t st = (hipStream_t)stream;
-#define PCLIP_LINEAR_BWD(T)                                                                                                                         backward<T>((const T*)x, (const T*)w, (const T*)dy, saved, saved_is_output, M, K, N, dtype, activation, (T*)dx, (T*)dw, (T*)db, (char*)ws, st)
+#define PCLIP_LINEAR_BWD(T)                                                                                                                         backward<T>((const T*)x, (const T*)w, (const T*)dy, saved, saved_is_output, M, K, N, dtype, activation, (T*)dx, (T*)dw, (T*)db, (char*)ws, ws ? ws_bytes : 0, st)
     if (dtype == PCLIP_DT_F32) rc = PCLIP_LINEAR_BWD(float);
     else if (dtype == PCLIP_DT_BF16) rc = PCLIP_LINEAR_BWD(__bf16);
     else rc = PCLIP_LINEAR_BWD(_Float16);
