@@ -362,6 +362,9 @@ int pclip_filip_prep_bwd(const float* h, const float* dn, int B, int T, int d, i
 #define PCLIP_ACT_SILU 3
 int pclip_linear_fwd(const void* x, const void* w, const void* bias, const void* residual, int M, int K, int N, int dtype, int activation,
                      void* y, void* slope, void* stream);
+/* Which tile a product runs on, 64, 128 or 256 rows (for tests and tuning; 0: bad sizes).  product: 0 forward, 1 dx, 2 dW;
+ * aligned: whether the rows of both operands begin at multiples of 16 bytes. */
+int pclip_linear_tile(int M, int K, int N, int dtype, int product, int aligned);
 size_t pclip_linear_bwd_workspace_bytes(int M, int K, int N, int dtype, int activation);
 int pclip_linear_bwd(const void* x, const void* w, const void* dy, const void* saved, int saved_is_output, int M, int K, int N, int dtype,
                      int activation, void* dx, void* dw, void* db, void* ws, size_t ws_bytes, void* stream);
@@ -394,6 +397,8 @@ int pclip_linear_bwd(const void* x, const void* w, const void* dy, const void* s
 int pclip_norm_gate_fwd(const void* u, const void* r, const void* gate, int gate_kind, int gate_rows, float scale, int after, const void* wa,
                         const void* ba, int before, const void* wb, const void* bb, int param_type, float eps, int rows, int d, int dtype,
                         void* y, void* n, float* stats, void* stream);
+/* How a row of aligned operands is held (for tests and tuning): by 16, 64 or 256 lanes, each with `vectors` accesses of `width` elements. */
+int pclip_norm_gate_row(int d, int dtype, int* lanes, int* vectors, int* width);
 size_t pclip_norm_gate_bwd_workspace_bytes(int rows, int d, int dtype, int gate_rows);
 int pclip_norm_gate_bwd(const void* u, const void* r, const void* gate, int gate_kind, int gate_rows, float scale, int after, const void* wa,
                         const void* ba, int before, const void* wb, const void* bb, int param_type, float eps, int rows, int d, int dtype,

@@ -56,9 +56,11 @@ _SIGNATURES = {
     "pclip_filip_bwd_fused": (c_int, [_P, _P, c_int, c_int, _P, _P, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, _P, _P, _P, _P, c_size_t, _P]),
     "pclip_filip_prep_bwd": (c_int, [_P, _P, c_int, c_int, c_int, c_int, _P, c_int, _P, _P]),
     "pclip_linear_fwd": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P, _P, _P]),
+    "pclip_linear_tile": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "pclip_linear_bwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "pclip_linear_bwd": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, _P, _P, _P, _P, c_size_t, _P]),
     "pclip_norm_gate_fwd": (c_int, [_P, _P, _P, c_int, c_int, c_float, c_int, _P, _P, c_int, _P, _P, c_int, c_float, c_int, c_int, c_int, _P, _P, _P, _P]),
+    "pclip_norm_gate_row": (c_int, [c_int, c_int, _P, _P, _P]),
     "pclip_norm_gate_bwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "pclip_norm_gate_bwd": (c_int, [_P, _P, _P, c_int, c_int, c_float, c_int, _P, _P, c_int, _P, _P, c_int, c_float, c_int, c_int, c_int, _P, _P, _P,
                                     _P, _P, _P, _P, _P, _P, _P, _P, c_size_t, _P]),

@@ -720,17 +720,21 @@ int launch_product(const GemmArgs& A, int bi, int bj, hipStream_t st) {
 // loads (4096 x 2560 -> 640: 39 us with one 128 x 128 tile on some units, 31 with three of 64 x 64).  16,384 x 1280 -> 1280: 3 * 256 x 128
 // tiles a unit 63 us, 5 * 128 x 128 56 us.  f32 products wait for the matrix cores whatever the tile, so the smallest,
 // which divides most evenly, always wins (8192 x 640 -> 640: 61 us; 128 x 128 85).
-template <typename T, bool PK, bool QK, int EPI>
-int launch_rows(const GemmArgs& A, hipStream_t st) {
-    if (sizeof(T) == 4) return launch_product<T, PK, QK, EPI>(A, 64, 64, st);
+int row_tile(int I, int J, int dtype) {
+    if (dtype == PCLIP_DT_F32) return 64;
     int best = 64;
     double least = 0.0;
     for (int bi : {64, 128, 256}) {
         const int bj = bi == 64 ? 64 : 128;
-        const double each = (double)((tiles(A.I, A.J, bi, bj) + 255) / 256), reach = (bi == 64 ? 0.62 : bi == 128 ? 1.0 : 1.03) * (each == 1.0 ? 0.6 : 1.0);
+        const double each = (double)((tiles(I, J, bi, bj) + 255) / 256), reach = (bi == 64 ? 0.62 : bi == 128 ? 1.0 : 1.03) * (each == 1.0 ? 0.6 : 1.0);
         const double cost = each * bi * bj / reach;
         if (bi == 64 || cost < least) best = bi, least = cost;
     }
+    return best;
+}
+template <typename T, bool PK, bool QK, int EPI>
+int launch_rows(const GemmArgs& A, hipStream_t st) {
+    const int best = row_tile(A.I, A.J, sizeof(T) == 4 ? PCLIP_DT_F32 : PCLIP_DT_BF16);
     return launch_product<T, PK, QK, EPI>(A, best, best == 64 ? 64 : 128, st);
 }
 
@@ -861,6 +865,13 @@ extern "C" int pclip_linear_fwd(const void* x, const void* w, const void* bias, 
     else if (dtype == PCLIP_DT_BF16) rc = forward<__bf16>(A, activation, st);
     else rc = forward<_Float16>(A, activation, st);
     return rc ? rc : pclip_check_launch("linear_fwd");
+}
+
+extern "C" int pclip_linear_tile(int M, int K, int N, int dtype, int product, int aligned) {
+    if (check_sizes("linear_tile", M, K, N, dtype, 0)) return 0;
+    if (product == 2) return row_plan(M, K, N, dtype, !aligned).tile;
+    const int tile = row_tile(M, product ? K : N, dtype);
+    return !aligned && tile == 256 ? 128 : tile;   // see launch_size
 }
 
 extern "C" size_t pclip_linear_bwd_workspace_bytes(int M, int K, int N, int dtype, int activation) {

@@ -678,6 +678,14 @@ extern "C" int pclip_norm_gate_fwd(const void* u, const void* r, const void* gat
     return rc ? rc : pclip_check_launch("norm_gate_fwd");
 }
 
+extern "C" int pclip_norm_gate_row(int d, int dtype, int* lanes, int* vectors, int* width) {
+    PCLIP_REQUIRE(d >= 1 && d <= MAX_D && pclip_dtype_ok(dtype) && lanes && vectors && width, "norm_gate_row: d=%d or the type, or a null pointer", d);
+    const Shape s = shape_of(d, dtype);
+    *lanes = s.lanes, *vectors = s.vectors, *width = d % s.width == 0 ? s.width : 1;
+    if (*width != s.width) *vectors *= s.width;
+    return PCLIP_OK;
+}
+
 extern "C" size_t pclip_norm_gate_bwd_workspace_bytes(int rows, int d, int dtype, int gate_rows) {
     if (rows < 1 || rows > 0x7fff0000 || d < 1 || d > MAX_D || !pclip_dtype_ok(dtype) || gate_rows < 0 || (gate_rows && rows % gate_rows)) return 0;
     NormGateArgs A = {};
