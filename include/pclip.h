@@ -362,6 +362,11 @@ int pclip_filip_prep_bwd(const float* h, const float* dn, int B, int T, int d, i
 #define PCLIP_ACT_SILU 3
 int pclip_linear_fwd(const void* x, const void* w, const void* bias, const void* residual, int M, int K, int N, int dtype, int activation,
                      void* y, void* slope, void* stream);
+/* The same with scratch of the query's size (16-byte aligned; 0: none is used): f32 products of few tiles split their contraction over more
+ * workgroups, whose f32 sums are added in a fixed order.  Without scratch they run unsplit. */
+size_t pclip_linear_fwd_workspace_bytes(int M, int K, int N, int dtype);
+int pclip_linear_fwd_ws(const void* x, const void* w, const void* bias, const void* residual, int M, int K, int N, int dtype, int activation,
+                        void* y, void* slope, void* ws, size_t ws_bytes, void* stream);
 /* Which tile a product runs on, 64, 128 or 256 rows (for tests and tuning; 0: bad sizes).  product: 0 forward, 1 dx, 2 dW;
  * aligned: whether the rows of both operands begin at multiples of 16 bytes. */
 int pclip_linear_tile(int M, int K, int N, int dtype, int product, int aligned);

@@ -56,6 +56,8 @@ _SIGNATURES = {
     "pclip_filip_bwd_fused": (c_int, [_P, _P, c_int, c_int, _P, _P, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, _P, _P, _P, _P, c_size_t, _P]),
     "pclip_filip_prep_bwd": (c_int, [_P, _P, c_int, c_int, c_int, c_int, _P, c_int, _P, _P]),
     "pclip_linear_fwd": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P, _P, _P]),
+    "pclip_linear_fwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "pclip_linear_fwd_ws": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P, _P, _P, c_size_t, _P]),
     "pclip_linear_tile": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "pclip_linear_bwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "pclip_linear_bwd": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, _P, _P, _P, _P, c_size_t, _P]),

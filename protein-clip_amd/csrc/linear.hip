@@ -276,6 +276,27 @@ __device__ __forceinline__ void wave_exchange() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// bias, activation, slope and residual of V sums in one row of the result, `left` of them inside it
+template <typename T, int EPI, int V>
+__device__ __forceinline__ void epilogue(const GemmArgs& A, size_t at, const float (&bias)[V], int left, float (&v)[V]) {
+    float slope[V];
+#pragma unroll
+    for (int e = 0; e < V; e++) v[e] = activate<sizeof(T) == 4, EPI>(v[e] + bias[e], slope[e]);
+    if constexpr (EPI == PCLIP_ACT_RELU && std::is_same_v<T, _Float16>) {
+        // the backward reads the slope from the output: a value above zero that rounds to zero becomes -0 (bfloat16 reaches
+        // as far down as the f32 sums do)
+#pragma unroll
+        for (int e = 0; e < V; e++) v[e] = v[e] > 0.f && v[e] <= 0x1p-25f ? -0.f : v[e];
+    }
+    if (A.slope) store_slope<T, V>((SlopeOf<T>*)A.slope + at, left, slope);
+    if (A.residual) {
+        float res[V];
+        load_f32<T, V>((const T*)A.residual + at, left, res);
+#pragma unroll
+        for (int e = 0; e < V; e++) v[e] += res[e];
+    }
+}
+
 // What a wave does with its accumulators: rows from i0, columns from j0 on.
 template <typename T, int FI, int FJ, int EPI>
 __device__ __forceinline__ void finish(const GemmArgs& A, f32x4 (&acc)[FI][FJ], f32x4 (&ones)[FI / 2], bool sum_rows, char* lds, int i0, int j0, int split) {
@@ -329,24 +350,7 @@ __device__ __forceinline__ void finish(const GemmArgs& A, f32x4 (&acc)[FI][FJ], 
                 for (int e = 0; e < V; e += 4) *(f32x4*)(v + e) = *(const f32x4*)(own + row * PITCH + c + e);
                 if (i >= A.I || left <= 0) continue;
                 const size_t at = (size_t)i * A.J + j;
-                if constexpr (EPI < EPI_STORE) {
-                    float slope[V];
-#pragma unroll
-                    for (int e = 0; e < V; e++) v[e] = activate<sizeof(T) == 4, EPI>(v[e] + bias[e], slope[e]);
-                    if constexpr (EPI == PCLIP_ACT_RELU && std::is_same_v<T, _Float16>) {
-                        // the backward reads the slope from the output: a value above zero that rounds to zero becomes -0 (bfloat16 reaches
-                        // as far down as the f32 sums do)
-#pragma unroll
-                        for (int e = 0; e < V; e++) v[e] = v[e] > 0.f && v[e] <= 0x1p-25f ? -0.f : v[e];
-                    }
-                    if (A.slope) store_slope<T, V>((SlopeOf<T>*)A.slope + at, left, slope);
-                    if (A.residual) {
-                        float res[V];
-                        load_f32<T, V>((const T*)A.residual + at, left, res);
-#pragma unroll
-                        for (int e = 0; e < V; e++) v[e] += res[e];
-                    }
-                }
+                if constexpr (EPI < EPI_STORE) epilogue<T, EPI, V>(A, at, bias, left, v);
                 stream_f32<T, V>((T*)A.out + at, left, v);
             }
             wave_exchange();
@@ -529,6 +533,30 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_direct_kernel(const Gemm
         runs.end_of_step(acc, ones, k + KSTEP<T> >= k_end);
     }
     finish<T, FI, FJ, EPI>(A, acc, ones, sum_rows, lds, i0 + wi, j0 + wj, split);
+}
+
+// The forward's and dx's split contraction: the slabs of the splits added in order, then the epilogue.  A thread takes four columns of a row.
+template <typename T, int EPI>
+__global__ __launch_bounds__(256) void join_kernel(const GemmArgs A) {
+    const int vecs = (A.J + 3) / 4;
+    const long long n = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (n >= (long long)A.I * vecs) return;
+    const int i = (int)(n / vecs), j = (int)(n % vecs) * 4, left = A.J - j;
+    const size_t at = (size_t)i * A.J + j, slab = (size_t)A.I * A.J;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int k = 0; k < A.splits; k++) {
+        float part[4];
+        load_f32<float, 4>(A.slab + k * slab + at, left, part);
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] += part[e];
+    }
+    if constexpr (EPI < EPI_STORE) {
+        float bias[4] = {0.f, 0.f, 0.f, 0.f};
+        if (A.bias) load_f32<T, 4>((const T*)A.bias + j, left, bias);
+        epilogue<T, EPI, 4>(A, at, bias, left, v);
+    }
+    stream_f32<T, 4>((T*)A.out + at, left, v);
 }
 
 // out[e] = sum over the splits' slabs in a fixed order, rounded once; blocks behind those of the weight's gradient sum the bias's.
@@ -732,9 +760,47 @@ int row_tile(int I, int J, int dtype) {
     }
     return best;
 }
+// How often the contraction of an f32 product over the rows is split.  A 64 x 64 tile keeps a compute unit busy for 0.5 to 0.65 us a step of 32 k values,
+// so few tiles, or some more than divide evenly over the 256 units, leave much of the device idle; splits cost a second launch and two
+// passes over their sums.  In microseconds: rounds of tiles x steps x 0.6, and 4 + 8 ns a tile and split.  Unsplit and split:
+// 1 x 2560 -> 2560 54 and 15 (library 8), 37 x 2369 -> 1280 62 and 15 (10), 1040 x 2560 -> 320 56 and 27 (24), 1108 x 2560 -> 640 56 and 43 (34),
+// 4096 x 2560 -> 640 128 and 116 (114); 300 x 320 -> 320 9.3 and 10.0, 704 x 1280 -> 2560 46 and 54: not split.
+struct Split { int splits, k_split; };
+Split row_split(int I, int J, int K, int dtype) {
+    Split best = {1, (K + 63) / 64 * 64};
+    if (dtype != PCLIP_DT_F32) return best;
+    const long long t = tiles(I, J, 64, 64);
+    const int steps = (K + 31) / 32;
+    if (t > 2048) return best;   // eight rounds and more: the last one weighs little
+    double least = (double)((t + 255) / 256) * steps * 0.6;
+    for (int s = 2; s <= 24 && s * 4 <= steps; s++) {   // four steps at least
+        const int per = (steps + s - 1) / s;
+        const double cost = (double)((t * s + 255) / 256) * per * 0.6 + 4.0 + 0.008 * (double)(t * s);
+        if (cost < least) best = {(steps + per - 1) / per, per * 32}, least = cost;
+    }
+    return best;
+}
+size_t split_bytes(int I, int J, int K, int dtype) {
+    const int s = row_split(I, J, K, dtype).splits;
+    return s > 1 ? pclip_align_up((size_t)s * I * J * sizeof(float), 256) : 0;
+}
+
+// slab: split_bytes of scratch, or NULL: in one
 template <typename T, bool PK, bool QK, int EPI>
-int launch_rows(const GemmArgs& A, hipStream_t st) {
-    const int best = row_tile(A.I, A.J, sizeof(T) == 4 ? PCLIP_DT_F32 : PCLIP_DT_BF16);
+int launch_rows(GemmArgs A, float* slab, hipStream_t st) {
+    constexpr int DTYPE = sizeof(T) == 4 ? PCLIP_DT_F32 : PCLIP_DT_BF16;
+    A.splits = 1, A.k_split = (A.K + 63) / 64 * 64;
+    if constexpr (sizeof(T) == 4) {
+        const Split s = row_split(A.I, A.J, (int)A.K, DTYPE);
+        if (slab && s.splits > 1) {
+            A.splits = s.splits, A.k_split = s.k_split, A.slab = slab;
+            const int rc = launch_product<T, PK, QK, EPI_SLAB>(A, 64, 64, st);
+            if (rc) return rc;
+            join_kernel<T, EPI><<<(unsigned)(((long long)A.I * ((A.J + 3) / 4) + 255) / 256), 256, 0, st>>>(A);
+            return PCLIP_OK;
+        }
+    }
+    const int best = row_tile(A.I, A.J, DTYPE);
     return launch_product<T, PK, QK, EPI>(A, best, best == 64 ? 64 : 128, st);
 }
 
@@ -757,11 +823,11 @@ RowPlan row_plan(int M, int K, int N, int dtype, bool staged) {
 }
 
 template <typename T>
-int forward(const GemmArgs& A, int act, hipStream_t st) {
-    if (act == PCLIP_ACT_NONE) return launch_rows<T, true, true, PCLIP_ACT_NONE>(A, st);
-    if (act == PCLIP_ACT_RELU) return launch_rows<T, true, true, PCLIP_ACT_RELU>(A, st);
-    if (act == PCLIP_ACT_GELU) return launch_rows<T, true, true, PCLIP_ACT_GELU>(A, st);
-    return launch_rows<T, true, true, PCLIP_ACT_SILU>(A, st);
+int forward(const GemmArgs& A, int act, float* slab, hipStream_t st) {
+    if (act == PCLIP_ACT_NONE) return launch_rows<T, true, true, PCLIP_ACT_NONE>(A, slab, st);
+    if (act == PCLIP_ACT_RELU) return launch_rows<T, true, true, PCLIP_ACT_RELU>(A, slab, st);
+    if (act == PCLIP_ACT_GELU) return launch_rows<T, true, true, PCLIP_ACT_GELU>(A, slab, st);
+    return launch_rows<T, true, true, PCLIP_ACT_SILU>(A, slab, st);
 }
 
 // how slope_kernel divides M x N: lanes a row, workgroups over the columns and over the rows (of 64 rows at least), rows of each
@@ -776,15 +842,17 @@ SlopePlan slope_plan(int M, int N, int dtype) {
     return {lanes, over_n, (int)((M + rows - 1) / rows), (int)rows};
 }
 
-// where the parts of the workspace lie; `product`: dW is wanted, `bias_alone`: db without it
-struct BackwardLayout { size_t sums, slab, row_sum, bytes; };   // dz at 0
-BackwardLayout backward_layout(int M, int K, int N, int dtype, int act, bool product, bool bias_alone, bool staged) {
+// where the parts of the workspace lie; `input`: dx is wanted, `product`: dW, `bias_alone`: db without it
+struct BackwardLayout { size_t sums, dx, slab, row_sum, bytes; };   // dz at 0
+BackwardLayout backward_layout(int M, int K, int N, int dtype, int act, bool input, bool product, bool bias_alone, bool staged) {
     BackwardLayout L = {};
     if (act != PCLIP_ACT_NONE) L.sums = pclip_align_up((size_t)M * N * pclip_dtype_size(dtype), 256);
+    L.dx = L.sums;
     if (act != PCLIP_ACT_NONE || bias_alone) {
         const SlopePlan s = slope_plan(M, N, dtype);
-        L.slab = L.sums + (s.over_m > 1 ? pclip_align_up((size_t)s.over_m * N * sizeof(float), 256) : 0);
+        L.dx += s.over_m > 1 ? pclip_align_up((size_t)s.over_m * N * sizeof(float), 256) : 0;
     }
+    L.slab = L.dx + (input ? split_bytes(M, K, N, dtype) : 0);
     if (!product) {
         L.bytes = L.slab;
         return L;
@@ -800,7 +868,7 @@ int backward(const T* x, const T* w, const T* dy, const void* saved, int is_outp
              size_t ws_bytes, hipStream_t st) {
     const bool bias_alone = db && !dw;
     const bool staged = !direct<T>(act == PCLIP_ACT_NONE ? dy : (const T*)ws, x, N, K);
-    const BackwardLayout L = backward_layout(M, K, N, dtype, act, dw, bias_alone, staged);
+    const BackwardLayout L = backward_layout(M, K, N, dtype, act, dx, dw, bias_alone, staged);
     if (L.bytes > ws_bytes) return pclip_fail(PCLIP_EINVAL, "linear_bwd: workspace too small (%zu bytes, need %zu)", ws_bytes, L.bytes);
     const RowPlan p = row_plan(M, K, N, dtype, staged);
     SlabSum S = {};
@@ -818,8 +886,8 @@ int backward(const T* x, const T* w, const T* dy, const void* saved, int is_outp
     }
     if (dx) {
         GemmArgs A = {};
-        A.P = dz, A.Q = w, A.ldp = N, A.ldq = K, A.I = M, A.J = K, A.K = N, A.k_split = (N + 63) / 64 * 64, A.splits = 1, A.out = dx;
-        const int rc = launch_rows<T, true, false, EPI_STORE>(A, st);
+        A.P = dz, A.Q = w, A.ldp = N, A.ldq = K, A.I = M, A.J = K, A.K = N, A.out = dx;
+        const int rc = launch_rows<T, true, false, EPI_STORE>(A, (float*)(ws + L.dx), st);
         if (rc) return rc;
     }
     if (dw) {
@@ -852,19 +920,32 @@ int check_sizes(const char* who, int M, int K, int N, int dtype, int act) {
 
 }  // namespace
 
-extern "C" int pclip_linear_fwd(const void* x, const void* w, const void* bias, const void* residual, int M, int K, int N, int dtype, int activation,
-                                void* y, void* slope, void* stream) {
+extern "C" size_t pclip_linear_fwd_workspace_bytes(int M, int K, int N, int dtype) {
+    if (check_sizes("linear_fwd", M, K, N, dtype, 0)) return 0;
+    return split_bytes(M, N, K, dtype);
+}
+
+extern "C" int pclip_linear_fwd_ws(const void* x, const void* w, const void* bias, const void* residual, int M, int K, int N, int dtype, int activation,
+                                   void* y, void* slope, void* ws, size_t ws_bytes, void* stream) {
     int rc = check_sizes("linear_fwd", M, K, N, dtype, activation);
     if (rc) return rc;
     PCLIP_REQUIRE(x && w && y, "linear_fwd: null pointer");
+    const size_t need = ws ? split_bytes(M, N, K, dtype) : 0;
+    PCLIP_REQUIRE(ws_bytes >= need, "linear_fwd: workspace too small (%zu bytes, need %zu)", ws_bytes, need);
+    PCLIP_REQUIRE(((uintptr_t)ws & 15) == 0, "linear_fwd: the workspace must be 16-byte aligned");
     GemmArgs A = {};
-    A.P = x, A.Q = w, A.ldp = K, A.ldq = K, A.I = M, A.J = N, A.K = K, A.k_split = (K + 63) / 64 * 64, A.splits = 1;
+    A.P = x, A.Q = w, A.ldp = K, A.ldq = K, A.I = M, A.J = N, A.K = K;
     A.bias = bias, A.residual = residual, A.out = y, A.slope = slope;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == PCLIP_DT_F32) rc = forward<float>(A, activation, st);
-    else if (dtype == PCLIP_DT_BF16) rc = forward<__bf16>(A, activation, st);
-    else rc = forward<_Float16>(A, activation, st);
+    if (dtype == PCLIP_DT_F32) rc = forward<float>(A, activation, (float*)ws, st);
+    else if (dtype == PCLIP_DT_BF16) rc = forward<__bf16>(A, activation, nullptr, st);
+    else rc = forward<_Float16>(A, activation, nullptr, st);
     return rc ? rc : pclip_check_launch("linear_fwd");
+}
+
+extern "C" int pclip_linear_fwd(const void* x, const void* w, const void* bias, const void* residual, int M, int K, int N, int dtype, int activation,
+                                void* y, void* slope, void* stream) {
+    return pclip_linear_fwd_ws(x, w, bias, residual, M, K, N, dtype, activation, y, slope, nullptr, 0, stream);
 }
 
 extern "C" int pclip_linear_tile(int M, int K, int N, int dtype, int product, int aligned) {
@@ -878,7 +959,7 @@ extern "C" size_t pclip_linear_bwd_workspace_bytes(int M, int K, int N, int dtyp
     if (check_sizes("linear_bwd", M, K, N, dtype, activation)) return 0;
     size_t most = 0;   // whichever gradients are wanted, at whatever addresses
     for (int k = 0; k < 3; k++) {
-        const size_t bytes = backward_layout(M, K, N, dtype, activation, k > 0, k == 0, k == 2).bytes;
+        const size_t bytes = backward_layout(M, K, N, dtype, activation, true, k > 0, k == 0, k == 2).bytes;
         if (bytes > most) most = bytes;
     }
     return most;

@@ -272,8 +272,14 @@ def linear_fwd(x, w, bias=None, residual=None, activation: str = "none", want_sl
     b, r = _operand(bias, "bias", w.shape[:1], dtype, dev), _operand(residual, "residual", shape, dtype, dev)
     y = _empty(shape, dtype, dev)
     slope = _empty(shape, _slope_type(dtype), dev) if want_slope else None
-    _launch(dev, _lib.load().pclip_linear_fwd, "pclip_linear_fwd", x.data_ptr(), w.data_ptr(), b, r, M, K, N, code, ACTIVATIONS[activation], y.data_ptr(),
-            slope.data_ptr() if want_slope else None, stream_of(x))
+    lib = _lib.load()
+    args = (x.data_ptr(), w.data_ptr(), b, r, M, K, N, code, ACTIVATIONS[activation], y.data_ptr(), slope.data_ptr() if want_slope else None)
+    nbytes = lib.pclip_linear_fwd_workspace_bytes(M, K, N, code) if dtype == F32 else 0
+    if nbytes:
+        ws = _empty((nbytes,), torch.uint8, dev)   # the call's own, see linear_bwd
+        _launch(dev, lib.pclip_linear_fwd_ws, "pclip_linear_fwd_ws", *args, ws.data_ptr(), nbytes, stream_of(x))
+    else:
+        _launch(dev, lib.pclip_linear_fwd, "pclip_linear_fwd", *args, stream_of(x))
     return y, slope
 
 

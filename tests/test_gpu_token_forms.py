@@ -45,6 +45,51 @@ def test_linear_forms(ops, t, rows, width, out, name, has_bias, has_res, tiles, 
         assert off <= 3 * R.half(t) + 4e-6 + (1e-3 if name == "relu" and n != "y" else 0), f"{n}: {off:.2e} in the 2-norm"
 
 
+@pytest.mark.parametrize("rows,width,out,name,has_bias,has_res,splits", F.SPLIT)
+def test_split_products(ops, rows, width, out, name, has_bias, has_res, splits):
+    """The split contraction like any other, the same bits on every call, and from the entry that takes no scratch the unsplit result."""
+    from protein_clip_amd import _lib
+    from protein_clip_amd._lib import ptr, stream_of
+    test_linear_forms(ops, F32, rows, width, out, name, has_bias, has_res, None, None)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, w = _make(g, F32, rows, width), _make(g, F32, out, width, std=width ** -0.5)
+    y = [ops.linear_act(x, w) for _ in range(2)]
+    assert torch.equal(*y)
+    unsplit = torch.empty_like(y[0])
+    _lib.check(_lib.load().pclip_linear_fwd(ptr(x), ptr(w), None, None, rows, width, out, 0, 0, ptr(unsplit), None, stream_of(x)), "pclip_linear_fwd")
+    size = x.double().abs() @ w.double().abs().t()
+    assert ((unsplit.double() - y[0].double()).abs() <= 2 * (width + 2) * R.U * size).all()
+
+
+def test_split_products_captured(ops):
+    """A graph with a split forward and dx, replayed on new values between eager calls of other sizes."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x, w, dy = _make(g, F32, 60, 2560).requires_grad_(True), _make(g, F32, 2560, 2560, std=0.02), _make(g, F32, 60, 2560)
+
+    def step():
+        y = ops.linear_act(x, w, activation="gelu")
+        return [y.detach(), torch.autograd.grad(y, x, dy)[0]]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for turn in range(3):
+        with torch.no_grad():
+            x.mul_(-0.5)
+        want = step()
+        ops.linear_act(x[:7].detach(), w)
+        for o in outs:
+            o.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)), f"turn {turn}"
+
+
 @pytest.mark.parametrize("t", [F32, BF16, F16], ids=str)
 @pytest.mark.parametrize("case", F.NORM, ids=str)
 def test_norm_forms(ops, t, case):

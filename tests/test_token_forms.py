@@ -37,6 +37,26 @@ def test_linear_sizes_take_their_tiles_in_f32(lib):
     assert seen >= {(p, a, 64) for p in range(3) for a in (True, False)} | {(2, True, 128)}
 
 
+def test_split_sizes_split(lib):
+    """dx is the product of dy with the weight, its contraction the layer's width out: a forward of these sizes."""
+    for rows, width, out, _, _, _, splits in F.SPLIT:
+        assert (lib.pclip_linear_fwd_workspace_bytes(rows, width, out, F32) > 0, lib.pclip_linear_fwd_workspace_bytes(rows, out, width, F32) > 0) == splits
+        assert lib.pclip_linear_fwd_workspace_bytes(rows, width, out, BF16) == lib.pclip_linear_fwd_workspace_bytes(rows, width, out, F16) == 0
+    assert lib.pclip_linear_fwd_workspace_bytes(300, 320, 320, F32) == lib.pclip_linear_fwd_workspace_bytes(16384, 1280, 1280, F32) == 0
+
+
+def test_scratch_of_the_forward_is_checked(lib):
+    one, err = ctypes.c_void_p(64), lambda: lib.pclip_last_error().decode()
+    need = lib.pclip_linear_fwd_workspace_bytes(60, 2560, 2560, F32)
+
+    def call(ws=one, n=need):
+        return lib.pclip_linear_fwd_ws(one, one, None, None, 60, 2560, 2560, F32, 0, one, None, ws, n, None)
+
+    assert call(n=need - 1) == -1 and "workspace too small" in err()
+    assert call(ws=ctypes.c_void_p(72)) == -1 and "16-byte aligned" in err()
+    assert lib.pclip_linear_fwd_ws(None, one, None, None, 60, 2560, 2560, F32, 0, one, None, one, need, None) == -1 and "null pointer" in err()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_norm_widths_reach_every_form(lib, dtype):
     def form(d):

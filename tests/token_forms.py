@@ -18,6 +18,19 @@ LINEAR = [
     (301, 1999, 2001, "relu", True, True, (64, 64), False),
 ]
 
+# f32 products of few tiles, whose contraction is split over workgroups: rows, width, out, activation, bias, residual; whether the forward and dx split
+SPLIT = [
+    (60, 2560, 2560, "gelu", True, True, (True, True)),
+    (1, 2560, 130, "silu", True, False, (True, False)),
+    (37, 2369, 1281, "relu", True, True, (True, True)),             # rows at no multiple of 16 bytes, remainders everywhere
+    (1040, 2560, 320, "relu", True, False, (True, False)),
+    (1108, 2562, 639, "none", True, True, (True, False)),
+    (260, 72, 2560, "silu", False, True, (False, True)),
+    (3, 33, 5000, "gelu", True, False, (False, True)),
+    (8926, 1617, 80, "silu", True, False, (True, False)),
+    (4096, 2560, 640, "gelu", True, True, (True, False)),
+]
+
 # batch, tokens, width, gate, after, before, kind, residual, scale: aligned rows of every width that is held another way
 NORM = [
     (3, 50, 16, "element", "affine", "affine", "layer", True, 0.5), (3, 50, 64, "sequence", "affine", "affine", "rms", True, 0.5),
