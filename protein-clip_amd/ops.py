@@ -141,6 +141,16 @@ def embedding_head(pooled: torch.Tensor, params, temperature: torch.Tensor, keep
 ACTIVATIONS = tuple(_hip_kernels.ACTIVATIONS)
 
 
+def _first_derivatives_only(backward):
+    """``once_differentiable``, whose own work is skipped where no graph of the backward is asked for (grad mode is off then)."""
+    checked = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return staticmethod(run)
+
+
 class _LinearAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, K):
@@ -153,8 +163,7 @@ class _LinearAct(torch.autograd.Function):
         ctx.save_for_backward(x if need_w else None, weight if need_x else None, y if output and product else slope)   # no operand that no gradient reads
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_first_derivatives_only
     def backward(ctx, dy):
         x, weight, saved = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
@@ -226,15 +235,12 @@ class _NormGate(torch.autograd.Function):
     def forward(ctx, u, r, gate, wa, ba, wb, bb, cfg):
         ctx.set_materialize_grads(False)
         u, r, gate, wa, ba, wb, bb = map(_contiguous, (u, r, gate, wa, ba, wb, bb))
-        _, _, after, before, _, _ = cfg
         y, n, stats = _norm_fwd(u, r, gate, wa, ba, wb, bb, cfg, True)
-        # without a norm and the gate's gradient, du is dy through the gate; the residual is read only to make y again for the second norm
-        ctx.cfg, ctx.plain = cfg, after is None and before is None and not ctx.needs_input_grad[2]
-        ctx.save_for_backward(None if ctx.plain else u, r if before else None, gate, wa, ba, wb, bb, stats)
+        ctx.cfg = cfg
+        ctx.save_for_backward(u, r if n is not None else None, gate, wa, ba, wb, bb, stats)   # r only makes y again for the second norm
         return y if n is None else (y, n)
 
-    @staticmethod
-    @once_differentiable
+    @_first_derivatives_only
     def backward(ctx, dy, dn=None):
         u, r, gate, wa, ba, wb, bb, stats = ctx.saved_tensors
         gate_rows, scale, after, before, eps, K = ctx.cfg
@@ -245,11 +251,31 @@ class _NormGate(torch.autograd.Function):
         if like.numel() == 0:
             return tuple(torch.zeros_like(t) if w else None for t, w in zip((like, like, gate, wa, ba, wb, bb), need)) + (None,)
         dy, dn = _contiguous(dy), _contiguous(dn)
-        dr = dy if need[1] and not before else None
-        if ctx.plain:
-            return (K.norm_gate_fwd(dy, None, gate, gate_rows, scale)[0] if need[0] else None, dr) + (None,) * 6
-        grads = K.norm_gate_bwd(u, r, gate, gate_rows, scale, after, wa, ba, before, wb, bb, eps, stats, dy, dn, (need[0], need[1] and dr is None, *need[2:]))
-        return (grads[0], grads[1] if dr is None else dr, *grads[2:], None)
+        if before is None:   # the residual's gradient is dy itself
+            need = (need[0], False, *need[2:])
+        grads = K.norm_gate_bwd(u, r, gate, gate_rows, scale, after, wa, ba, before, wb, bb, eps, stats, dy, dn, need)
+        return (grads[0], dy if before is None and ctx.needs_input_grad[1] else grads[1], *grads[2:], None)
+
+
+class _Gated(torch.autograd.Function):
+    """``r + scale * gate * u`` where the gate takes no gradient: du is dy through the gate, and nothing else is kept."""
+
+    @staticmethod
+    def forward(ctx, u, r, gate, gate_rows, scale, K):
+        u, r, gate = _contiguous(u), _contiguous(r), _contiguous(gate)
+        ctx.cfg = gate_rows, scale, K
+        ctx.save_for_backward(gate)
+        return K.norm_gate_fwd(u, r, gate, gate_rows, scale)[0] if u.numel() else torch.empty_like(u)
+
+    @_first_derivatives_only
+    def backward(ctx, dy):
+        gate, = ctx.saved_tensors
+        gate_rows, scale, K = ctx.cfg
+        need_u, need_r = ctx.needs_input_grad[:2]
+        dy = _contiguous(dy)
+        if need_u:
+            du = K.norm_gate_fwd(dy, None, gate, gate_rows, scale)[0] if dy.numel() else torch.zeros_like(dy)
+        return du if need_u else None, dy if need_r else None, None, None, None, None
 
 
 def _norm_fwd(u, r, gate, wa, ba, wb, bb, cfg, want_stats):
@@ -310,7 +336,8 @@ def norm_gate_residual(u: torch.Tensor, residual: Optional[torch.Tensor] = None,
         if gate.dtype == torch.bool:
             gate = gate.view(torch.uint8)
         if gate.dtype == torch.uint8:
-            gate = gate.expand(u.shape)
+            if gate.shape != u.shape:
+                gate = gate.expand(u.shape)
         else:
             if gate.dtype != u.dtype:
                 gate = gate.to(u.dtype)
@@ -324,6 +351,8 @@ def norm_gate_residual(u: torch.Tensor, residual: Optional[torch.Tensor] = None,
             residual = residual.expand(u.shape)
     cfg = (gate_rows, float(scale), norm if after is not None else None, norm if before is not None else None, float(eps), K)
     if _wants_autograd(u, residual, gate, wa, ba, wb, bb):
+        if after is None and before is None and (gate is None or not gate.requires_grad):
+            return _Gated.apply(u, residual, gate, gate_rows, float(scale), K)
         return _NormGate.apply(u, residual, gate, wa, ba, wb, bb, cfg)
     y, n, _ = _norm_fwd(*map(_contiguous, (u, residual, gate, wa, ba, wb, bb)), cfg, False)
     return y if n is None else (y, n)
