@@ -62,7 +62,7 @@ def _loss_scaler(model, scaler, device):
     subnormal numbers (steps of 6e-8) or below them."""
     if scaler is not None and scaler.is_enabled():
         return scaler
-    if any(getattr(m, "token_dtype", None) == torch.float16 for m in model.modules()):
+    if any(getattr(m, "token_dtype", None) == torch.float16 for m in getattr(model, "modules", list)()):
         return torch.amp.GradScaler(torch.device(device).type)
     return scaler
 

@@ -130,3 +130,27 @@ def test_gradients_of_some_operands_only(ops, t, rows, width, out, name):
         names = [n for v, n in zip(leaves, ("x", "weight", "bias")) if v.requires_grad]
         for got, n in zip(torch.autograd.grad(y, wanted, dy.cuda()), names):
             R.assert_within(got, *want[n], f"{mask}: {n}")
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("name", ["none", "relu", "silu"])
+def test_wanted_gradients_whatever_operands_are_given(ops, t, name):
+    """The wrapper of the kernels with every choice of wanted gradients, with all operands and with those that the choice needs."""
+    from protein_clip_amd import kernels as K
+    g = torch.Generator(device="cuda").manual_seed(4)
+    make = lambda *s: torch.randn(*s, generator=g, device="cuda").to(t)
+    x, w, b, dy = make(700, 72), make(56, 72), make(56), make(700, 56)
+    y, slope = K.linear_fwd(x, w, b, None, name, name == "silu")
+    saved = {"none": (None, False), "relu": (y, True), "silu": (slope, False)}[name]
+    full = K.linear_bwd(x, w, dy, *saved, name)
+    for mask in range(1, 8):
+        want = [bool(mask >> i & 1) for i in range(3)]
+        for got in (K.linear_bwd(x, w, dy, *saved, name, *want), K.linear_bwd(x if want[1] else None, w if want[0] else None, dy, *saved, name, *want)):
+            for i in range(3):
+                if not want[i]:
+                    assert got[i] is None
+                elif i < 2:
+                    assert torch.equal(got[i], full[i])
+                else:   # the column sum alone, or with the weight's product: the same 700 terms in another order, each sum rounded once
+                    size = dy.double().abs().sum(0) * 1.13
+                    assert ((got[i].double() - full[i].double()).abs() <= 2 * 708 * R.U * size + 2 * R.half(t) * full[i].double().abs()).all()
