@@ -225,8 +225,8 @@ __device__ __forceinline__ void add_rows(const typename Mfma<T>::Frag (&fp)[FI],
     }
 }
 
-// f32 products are summed in runs of RUN steps (256 k values), whose sums are added: one chain over 2560 k values ends up 1e-6 off,
-// twice what a library's product is.  16-bit results do not show it.
+// f32 products are summed in runs of RUN steps (256 k values), whose sums are added: one chain over 2560 k values ends up 1e-6 off, runs
+// 3e-7, for some twenty registers a 64 x 64 tile and a few hundredths of the time.  16-bit results do not show it.
 constexpr int RUN = 8;
 template <typename T, int FI, int FJ>
 struct Runs {
@@ -452,8 +452,8 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_kernel(const GemmArgs A)
 // LDS is enough, because a wave takes all its fragments of a step into registers first; the next tile is on its way while
 // the matrix cores work, and two or three workgroups share a compute unit.  Chunks outside the matrix are read at an offset
 // beyond the descriptor's range, which writes zeros.  Bound by the matrix cores and the reads of LDS (a 64 x 64 part of a
-// tile reads 16 KB for 32 matrix instructions, 128 x 64 24 KB for 64): 65,536 x 2560 -> 640 bf16 235 us, 910 TFLOP/s; dW 263 us,
-// 820; 16,384 x 1280 -> 1280 52.5 us, 1023.  The staged form: 521 at 16,383 x 1283 -> 1279.
+// tile reads 16 KB for 32 matrix instructions, 128 x 64 24 KB for 64): 65,536 x 2560 -> 640 bf16 220 us, 978 TFLOP/s; dW 269 us,
+// 797; 16,384 x 1280 -> 1280 54.5 us, 986.  The staged form: 541 at 16,383 x 1283 -> 1279.
 template <typename T, int BI, int BJ, int WI, int WJ, bool PK, bool QK, int EPI>
 __global__ __launch_bounds__(64 * WI * WJ, 2) void gemm_direct_kernel(const GemmArgs A) {
     typedef Tile<T, BI, PK> TP;
@@ -596,9 +596,12 @@ __global__ __launch_bounds__(256) void slab_sum_kernel(const SlabSum A) {
     if (part == 0 && valid > 0) store_f32<T, 4>((T*)A.out[which] + e, valid, s);
 }
 
-// Bound by memory: 1.0 GB for 65,536 x 2560 bf16 in 206 us, 4.9 TB/s (before the column sums were added: 180-197 us, with one access under
+// Bound by memory: 1.0 GB for 65,536 x 2560 bf16 in 204 us, 4.9 TB/s (before the column sums were added: 180-197 us, with one access under
 // way instead of four 245).
-// dz = dy * slope, or dy where the output is positive, rounded; and the column sums of the unrounded products, from which the
+// dz = dy * slope, or dy where the output is not +0, rounded to the operands' type: a choice, since the matrix cores take no wider operand
+// beside a 16-bit one.  It leaves dx and dW 1.4 times as far from the exact ones as one rounding at the end would (bf16 0.0024 instead of
+// 0.0017 in the 2-norm, f16 0.00029 and 0.00021); a second 16-bit part of dz would halve the rate of both products, half of the time of
+// a training pass.  And the column sums of the unrounded products, from which the
 // bias's gradient comes (the rounded ones would bring it the errors of M roundings).  `lanes` neighbouring threads take a row's
 // vectors, 256 / lanes rows at once; a workgroup takes `rows` rows of its columns, with four accesses of each operand under way.
 struct SlopeArgs {
@@ -746,8 +749,8 @@ int launch_product(const GemmArgs& A, int bi, int bj, hipStream_t st) {
 // area, over what the tile reaches of the matrix cores when several share a unit (16-bit: 256 x 128 a little more than
 // 128 x 128, 64 x 64 0.62 of it: 232, 241 and 371 us for 65,536 x 640 -> 2560) and 0.6 of that for one alone, which waits for its own
 // loads (4096 x 2560 -> 640: 39 us with one 128 x 128 tile on some units, 31 with three of 64 x 64).  16,384 x 1280 -> 1280: 3 * 256 x 128
-// tiles a unit 63 us, 5 * 128 x 128 56 us.  f32 products wait for the matrix cores whatever the tile, so the smallest,
-// which divides most evenly, always wins (8192 x 640 -> 640: 61 us; 128 x 128 85).
+// tiles a unit 63 us, 5 * 128 x 128 56 us.  f32 products wait for the matrix cores whatever the tile, so they take the smallest,
+// which divides most evenly and leaves room for the runs' sums (8192 x 640 -> 640: 54.5 us, 123 of 154 TFLOP/s).
 int row_tile(int I, int J, int dtype) {
     if (dtype == PCLIP_DT_F32) return 64;
     int best = 64;
@@ -805,8 +808,8 @@ int launch_rows(GemmArgs A, float* slab, hipStream_t st) {
 }
 
 // The product over the rows (dW): tile size, the number of splits and their length.  The tile is 128 x 128, or 64 x 64 where a side is
-// no longer, and for f32 with few tiles: 16 waves then share a compute unit instead of 8 (4096 x 640 -> 128: 22 us instead
-// of 28; 16,384 x 1280 -> 1280, a hundred tiles: 658 instead of 492), and where f32 operands are staged, whose fetched registers and the
+// no longer, and for f32 with few tiles: 16 waves then share a compute unit instead of 8 (4096 x 640 -> 128: 16 us instead
+// of 22; 16,384 x 1280 -> 1280, a hundred tiles: 711 instead of 493), and where f32 operands are staged, whose fetched registers and the
 // runs' sums of a 128 x 128 tile do not fit (spilled, 16,383 x 1283 -> 1279 846 us instead of 674; 600 x 2049 -> 2047 120 instead of 79).
 struct RowPlan { int tile, splits; long long k_split; };
 RowPlan row_plan(int M, int K, int N, int dtype, bool staged) {
