@@ -19,7 +19,8 @@
 // waves spent more time on those than on the rows (45 -> 32 us forward, 113 -> 53 us backward with its column sums for 32,768 x 640 bf16 with
 // gate, residual and both norms; 168 and 252 MB, that is 5.3 and 4.8 TB/s).  What the backward still spills are scalar registers (23 to 100,
 // the descriptors themselves, into vector lanes), and at widths of 513 to 768 that do not divide into vectors 22 to 30 vector registers: a
-// single wave a SIMD would hold them, and is slower (65,536 x 637 bf16: 196 us instead of 174).
+// single wave a SIMD would hold them, and is slower (65,536 x 637 bf16: 196 us instead of 174).  16-bit rows beyond 2048 use 12 bytes of scratch
+// a lane.
 #include "elem.h"
 
 namespace {

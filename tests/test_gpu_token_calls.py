@@ -87,3 +87,29 @@ def test_linear_of_more_rows_than_a_grid_has_threads(ops):
             del dx, dy
         del x, y
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("gate", ["none", "keep", "channel", "sequence", "element", "number"])
+@pytest.mark.parametrize("shape", [(3, 50, 96), (2, 7, 33), (5, 1, 1), (2, 0, 8)])
+def test_joins_without_norms(ops, t, gate, shape):
+    """``r + scale * gate * u`` with a gate that takes no gradient: values, du through the gate, dr, each wanted or not."""
+    import token_ref as R
+    g = torch.Generator().manual_seed(6)
+    make = lambda *s: torch.randn(*s, generator=g).to(t)
+    u, r, dy = make(*shape), make(*shape), make(*shape)
+    gt = {"none": None, "keep": torch.rand(*shape, generator=g) > 0.3, "channel": make(shape[-1]), "sequence": make(shape[0], 1, shape[-1]), "element": make(*shape),
+          "number": make(1)[0]}[gate]
+    scale = torch.tensor(1.3).item()
+    factor = scale * (torch.ones(1) if gt is None else gt).double().expand(shape)
+    for need_u, need_r in ((True, True), (True, False), (False, True)):
+        us, rs = u.cuda().requires_grad_(need_u), r.cuda().requires_grad_(need_r)
+        y = ops.norm_gate_residual(us, rs, None if gt is None else gt.cuda(), scale=scale)
+        want = factor * u.double() + r.double()
+        R.assert_within(y, want, R.rounded(want, 3 * R.U * ((factor * u.double()).abs() + want.abs()), t), "y")
+        grads = iter(torch.autograd.grad(y, [v for v in (us, rs) if v.requires_grad], dy.cuda()))
+        if need_u:
+            du = factor * dy.double()
+            R.assert_within(next(grads), du, R.rounded(du, 3 * R.U * du.abs(), t), "du")
+        if need_r:
+            assert torch.equal(next(grads).cpu(), dy)
